@@ -284,6 +284,76 @@ int trnopt_plan_log_row_sums(const double* x, int n, const double* y, int m, int
                              const double* log_a, const double* log_b, double eps, double* out, void* workspace,
                              size_t ws_bytes, void* stream);
 
+/* trnopt_plan_log_rows: the same rows as log P[rows[r], :] (no underflow: entries below exp's range keep their log). */
+int trnopt_plan_log_rows(const double* x, int n, const double* y, int m, int d, const double* f, const double* g,
+                         const double* log_a, const double* log_b, double eps, const int* rows, int nrows, double* out,
+                         void* stream);
+
+/* Operators over an explicit score matrix S (rows x cols, row-major: element (i, j) at scores[i * ld + j], j < cols),
+ * for assignments whose scores a program already holds. No reference counterpart. `type` is the scores' type; a row
+ * pitch ld of any size >= 0 is allowed, and pointers need the alignment of their own type only. */
+enum { TRNOPT_F32 = 0, TRNOPT_F16 = 1, TRNOPT_BF16 = 2, TRNOPT_F64 = 3 };
+
+/* Row softmax p = softmax(S / temperature) of every row: per row the log-probabilities of n_targets given columns, the
+ * entropy, the log-sum-exp of S / temperature, and the `top` best columns (score descending, equal scores by lower
+ * index) with their log-probabilities. Values are float32 (float64 for TRNOPT_F64 scores).
+ *   targets (rows, n_targets)  column indices; negative: padding, log_prob 0; >= cols: log_prob NaN, nothing is read
+ *   log_prob (rows, n_targets), entropy (rows,), lse (rows,)
+ *   top_log_prob, top_index (rows, top)   0 <= top <= 64; slots beyond the columns above -inf: -inf and index -1
+ *   row_max, log_sum (rows,)   the row's largest score and log sum_j exp((S_j - max) / temperature), for the gradient
+ *                              (both NULL where none is wanted)
+ * A column of score -inf has probability 0. A row of nothing else has lse = log_prob = -inf and entropy 0. A row with
+ * NaN or +inf has NaN values and top_index -1. Deterministic. */
+int trnopt_log_probs(int type, const void* scores, long long ld, long long rows, int cols, double temperature,
+                     const long long* targets, int n_targets, int top, void* log_prob, void* entropy, void* lse,
+                     void* top_log_prob, long long* top_index, void* row_max, void* log_sum, void* stream);
+
+/* The gradient of trnopt_log_probs: grad (rows, cols; pitch ld_grad >= cols; the scores' type) from the upstream
+ * gradients of its outputs (each NULL where there is none) and the forward call's row_max, log_sum, entropy and
+ * top_index. Columns named more than once add up; padding and out-of-range targets add nothing; rows of nothing but
+ * -inf have gradient 0. Deterministic. n_targets + top <= 1088. */
+int trnopt_log_probs_grad(int type, const void* scores, long long ld, long long rows, int cols, double temperature,
+                          const long long* targets, int n_targets, const long long* top_index, int top,
+                          const void* row_max, const void* log_sum, const void* entropy, const void* d_log_prob,
+                          const void* d_entropy, const void* d_lse, const void* d_top_log_prob, void* grad,
+                          long long ld_grad, void* stream);
+
+/* Sinkhorn on a score matrix: `iters` iterations of
+ *     f_i = -eps LSE_j(log b_j + (g_j + S_ij) / eps),   g_j = -eps LSE_i(log a_i + (f_i + S_ij) / eps)
+ * (the half-steps of sinkhorn.py:108-119 for the cost -S), from g = g0 (NULL: 0). a (rows,) and b (cols,) are masses
+ * >= 0 (NULL: 1 / rows, 1 / cols); rows or columns of mass 0 send nothing and still get their potential. A row or
+ * column whose terms are all zero has potential 0. f (rows,) and g (cols,) are float32. cols <= 1024; types F32, F16,
+ * BF16. Deterministic. Workspace of trnopt_balance_workspace_size bytes (256-byte aligned, no initialisation); one
+ * workspace per call in flight. */
+size_t trnopt_balance_workspace_size(int rows, int cols);
+int trnopt_balance(int type, const void* scores, long long ld, int rows, int cols, double eps, int iters,
+                   const float* a, const float* b, const float* g0, float* f, float* g, void* workspace,
+                   size_t ws_bytes, void* stream);
+
+/* Each row's `top` best columns and their weights.
+ *   kind        share = softmax of the row, or sigmoid of each score
+ *   bias        (cols,) or NULL, in the choice only: added to the shares (TRNOPT_ROUTE_BIAS_SCORES) or to the scores
+ *               themselves (TRNOPT_ROUTE_BIAS_LOGITS; trnopt_balance's g). -inf closes a column
+ *   groups      the columns form `groups` equal runs; the top_groups runs with the largest sum of their group_top (1 or
+ *               2) largest biased shares (bias on the logits: biased scores) stay open
+ *   weight      scale * share, or with `renormalize` scale * share / (sum of the row's chosen shares)
+ *   index, weight (rows, top), best first, equal keys by lower index; load (cols,) or NULL: rows that chose a column
+ * Columns of score -inf are closed. Slots that no open column fills hold index -1, weight 0; a row with NaN or +inf (or
+ * a NaN bias) chooses nothing: index -1, weight NaN. The order is that of the keys in 64 bits. Deterministic.
+ * cols <= 1024, top <= 32, groups <= 32, types F32, F16, BF16. */
+enum { TRNOPT_ROUTE_SOFTMAX = 0, TRNOPT_ROUTE_SIGMOID = 1 };
+enum { TRNOPT_ROUTE_BIAS_SCORES = 0, TRNOPT_ROUTE_BIAS_LOGITS = 1 };
+int trnopt_route(int type, const void* scores, long long ld, long long rows, int cols, int top, int kind,
+                 const float* bias, int bias_on, int groups, int top_groups, int group_top, int renormalize,
+                 float scale, long long* index, float* weight, int* load, void* stream);
+
+/* The gradient of trnopt_route's weights with respect to the scores (the choice itself is constant): grad (rows, cols;
+ * pitch ld_grad >= cols; the scores' type). Slots of index outside [0, cols) add nothing; a row that chose nothing has
+ * gradient 0. */
+int trnopt_route_grad(int type, const void* scores, long long ld, long long rows, int cols, int top, int kind,
+                      int renormalize, float scale, const long long* index, const float* d_weight, void* grad,
+                      long long ld_grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

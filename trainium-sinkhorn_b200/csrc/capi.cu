@@ -6,6 +6,7 @@
 
 #include "../../include/trnopt_cuda.h"
 #include "kernels.h"
+#include "scores.h"
 
 namespace trnopt {
 
@@ -433,6 +434,124 @@ int trnopt_plan_log_row_sums(const double* x, int n, const double* y, int m, int
   if (!aligned(x, 8) || !aligned(y, 8) || !aligned(out, 8) || !aligned(workspace, 8)) return TRNOPT_ERR_ALIGNMENT;
   return cuda_status(plan_lse_launch(dev, x, n, y, m, d, f, g, log_a, log_b, eps, out, workspace,
                                      reinterpret_cast<cudaStream_t>(stream)));
+}
+
+int trnopt_plan_log_rows(const double* x, int n, const double* y, int m, int d, const double* f, const double* g,
+                         const double* log_a, const double* log_b, double eps, const int* rows, int nrows, double* out,
+                         void* stream) {
+  if (!plan_args_ok(x, n, y, m, d, eps) || nrows < 0 || (nrows > 0 && (!rows || !out)))
+    return TRNOPT_ERR_INVALID_ARGUMENT;
+  if (nrows == 0) return TRNOPT_OK;
+  if (!aligned(x, 8) || !aligned(y, 8) || !aligned(out, 8) || !aligned(rows, 4)) return TRNOPT_ERR_ALIGNMENT;
+  return cuda_status(plan_log_rows_launch(x, n, y, m, d, f, g, log_a, log_b, eps, rows, nrows, out,
+                                          reinterpret_cast<cudaStream_t>(stream)));
+}
+
+// Shared checks of the score-matrix calls: a known type, sizes, and the alignment of the type.
+static int check_scores(int type, const void* scores, long long ld, long long rows, int cols, bool f64_ok) {
+  if (type < TRNOPT_F32 || type > (f64_ok ? TRNOPT_F64 : TRNOPT_BF16)) return TRNOPT_ERR_UNSUPPORTED;
+  if (rows < 0 || cols < 1 || ld < 0 || (rows > 0 && !scores)) return TRNOPT_ERR_INVALID_ARGUMENT;
+  const size_t size = type == TRNOPT_F64 ? 8 : type == TRNOPT_F32 ? 4 : 2;
+  return aligned(scores, size) ? TRNOPT_OK : TRNOPT_ERR_ALIGNMENT;
+}
+
+static bool temperature_ok(double t) { return t >= 1e-30 && t <= 1e30; }
+
+int trnopt_log_probs(int type, const void* scores, long long ld, long long rows, int cols, double temperature,
+                     const long long* targets, int n_targets, int top, void* log_prob, void* entropy, void* lse,
+                     void* top_log_prob, long long* top_index, void* row_max, void* log_sum, void* stream) {
+  const int st = check_scores(type, scores, ld, rows, cols, true);
+  if (st != TRNOPT_OK) return st;
+  if (!temperature_ok(temperature) || n_targets < 0 || n_targets > 1024 || top < 0 || top > 64)
+    return TRNOPT_ERR_INVALID_ARGUMENT;
+  if (rows == 0) return TRNOPT_OK;
+  if (!entropy || !lse || (n_targets > 0 && (!targets || !log_prob)) || (top > 0 && (!top_log_prob || !top_index)) ||
+      !row_max != !log_sum)
+    return TRNOPT_ERR_INVALID_ARGUMENT;
+  const size_t size = type == TRNOPT_F64 ? 8 : 4;
+  if (!aligned(targets, 8) || !aligned(top_index, 8) || !aligned(log_prob, size) || !aligned(entropy, size) ||
+      !aligned(lse, size) || !aligned(top_log_prob, size) || !aligned(row_max, size) || !aligned(log_sum, size))
+    return TRNOPT_ERR_ALIGNMENT;
+  const LogProbsProblem p{scores, ld, rows, cols, temperature, targets, n_targets, top, log_prob, entropy, lse,
+                          top_log_prob, top_index, row_max, log_sum};
+  return cuda_status(log_probs_launch(type, p, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+int trnopt_log_probs_grad(int type, const void* scores, long long ld, long long rows, int cols, double temperature,
+                          const long long* targets, int n_targets, const long long* top_index, int top,
+                          const void* row_max, const void* log_sum, const void* entropy, const void* d_log_prob,
+                          const void* d_entropy, const void* d_lse, const void* d_top_log_prob, void* grad,
+                          long long ld_grad, void* stream) {
+  int st = check_scores(type, scores, ld, rows, cols, true);
+  if (st == TRNOPT_OK) st = check_scores(type, grad, ld_grad, rows, cols, true);
+  if (st != TRNOPT_OK) return st;
+  if (!temperature_ok(temperature) || n_targets < 0 || n_targets > 1024 || top < 0 || top > 64 || ld_grad < cols)
+    return TRNOPT_ERR_INVALID_ARGUMENT;
+  if (rows == 0) return TRNOPT_OK;
+  if (!row_max || !log_sum || !entropy || (n_targets > 0 && !targets) || (top > 0 && !top_index))
+    return TRNOPT_ERR_INVALID_ARGUMENT;
+  const size_t size = type == TRNOPT_F64 ? 8 : 4;
+  if (!aligned(targets, 8) || !aligned(top_index, 8) || !aligned(row_max, size) || !aligned(log_sum, size) ||
+      !aligned(entropy, size) || !aligned(d_log_prob, size) || !aligned(d_entropy, size) || !aligned(d_lse, size) ||
+      !aligned(d_top_log_prob, size))
+    return TRNOPT_ERR_ALIGNMENT;
+  const LogProbsGradProblem p{scores, ld, rows, cols, temperature, targets, n_targets, top_index, top, row_max,
+                              log_sum, entropy, d_log_prob, d_entropy, d_lse, d_top_log_prob, grad, ld_grad};
+  return cuda_status(log_probs_grad_launch(type, p, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+size_t trnopt_balance_workspace_size(int rows, int cols) {
+  if (rows < 1 || cols < 1 || cols > 1024) return 0;
+  return balance_workspace_bytes(current_device(), rows, cols);
+}
+
+int trnopt_balance(int type, const void* scores, long long ld, int rows, int cols, double eps, int iters,
+                   const float* a, const float* b, const float* g0, float* f, float* g, void* workspace,
+                   size_t ws_bytes, void* stream) {
+  const int st = check_scores(type, scores, ld, rows, cols, false);
+  if (st != TRNOPT_OK) return st;
+  if (rows < 1 || iters < 1 || !(eps >= 1e-30 && eps <= 1e30) || !f || !g) return TRNOPT_ERR_INVALID_ARGUMENT;
+  if (cols > 1024) return TRNOPT_ERR_UNSUPPORTED;
+  const int dev = current_device();
+  if (!workspace || ws_bytes < balance_workspace_bytes(dev, rows, cols)) return TRNOPT_ERR_WORKSPACE;
+  if (!aligned(workspace, 256) || !aligned(a, 4) || !aligned(b, 4) || !aligned(g0, 4) || !aligned(f, 4) ||
+      !aligned(g, 4))
+    return TRNOPT_ERR_ALIGNMENT;
+  const BalanceProblem p{scores, ld, rows, cols, iters, eps, a, b, g0, f, g};
+  return cuda_status(balance_launch(dev, type, p, workspace, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+int trnopt_route(int type, const void* scores, long long ld, long long rows, int cols, int top, int kind,
+                 const float* bias, int bias_on, int groups, int top_groups, int group_top, int renormalize,
+                 float scale, long long* index, float* weight, int* load, void* stream) {
+  const int st = check_scores(type, scores, ld, rows, cols, false);
+  if (st != TRNOPT_OK) return st;
+  if (cols > 1024 || top > 32 || groups > 32) return TRNOPT_ERR_UNSUPPORTED;
+  if (groups < 1 || cols % groups != 0 || top_groups < 1 || top_groups > groups || top < 1 ||
+      top > top_groups * (cols / groups) || group_top < 1 || group_top > 2 || !isfinite(scale) ||
+      (kind != TRNOPT_ROUTE_SOFTMAX && kind != TRNOPT_ROUTE_SIGMOID) ||
+      (bias_on != TRNOPT_ROUTE_BIAS_SCORES && bias_on != TRNOPT_ROUTE_BIAS_LOGITS) ||
+      (rows > 0 && (!index || !weight)))
+    return TRNOPT_ERR_INVALID_ARGUMENT;
+  if (!aligned(bias, 4) || !aligned(index, 8) || !aligned(weight, 4) || !aligned(load, 4)) return TRNOPT_ERR_ALIGNMENT;
+  const RouteProblem p{scores, ld, rows, cols, top, kind, bias, bias_on, groups, top_groups, group_top, renormalize,
+                       scale, index, weight, load};
+  return cuda_status(route_launch(type, p, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+int trnopt_route_grad(int type, const void* scores, long long ld, long long rows, int cols, int top, int kind,
+                      int renormalize, float scale, const long long* index, const float* d_weight, void* grad,
+                      long long ld_grad, void* stream) {
+  int st = check_scores(type, scores, ld, rows, cols, false);
+  if (st == TRNOPT_OK) st = check_scores(type, grad, ld_grad, rows, cols, false);
+  if (st != TRNOPT_OK) return st;
+  if (cols > 1024 || top > 32) return TRNOPT_ERR_UNSUPPORTED;
+  if (top < 1 || !isfinite(scale) || ld_grad < cols ||
+      (kind != TRNOPT_ROUTE_SOFTMAX && kind != TRNOPT_ROUTE_SIGMOID) || (rows > 0 && (!index || !d_weight)))
+    return TRNOPT_ERR_INVALID_ARGUMENT;
+  if (!aligned(index, 8) || !aligned(d_weight, 4)) return TRNOPT_ERR_ALIGNMENT;
+  const RouteGradProblem p{scores, ld, rows, cols, top, kind, renormalize, scale, index, d_weight, grad, ld_grad};
+  return cuda_status(route_grad_launch(type, p, reinterpret_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -63,6 +63,9 @@ size_t plan_lse_workspace_bytes(int device, int n, int m);
 cudaError_t plan_rows_launch(const double* x, int n, const double* y, int m, int d, const double* f, const double* g,
                              const double* la, const double* lb, double eps, const int* rows, int nrows, double* out,
                              cudaStream_t stream);
+cudaError_t plan_log_rows_launch(const double* x, int n, const double* y, int m, int d, const double* f, const double* g,
+                                 const double* la, const double* lb, double eps, const int* rows, int nrows, double* out,
+                                 cudaStream_t stream);
 cudaError_t plan_lse_launch(int device, const double* x, int n, const double* y, int m, int d, const double* f,
                             const double* g, const double* la, const double* lb, double eps, double* out, void* ws,
                             cudaStream_t stream);

@@ -4,7 +4,7 @@
 // This is the plan of the reference's transport_plan (src/trnopt/sinkhorn.py:397-403) with its direct-difference
 // cost. Two kernels share one 64 x 64 cost tile (C for 64 rows of x and 64 rows of y, coordinates staged through
 // shared memory 32 at a time, each of 256 threads holding a 4 x 4 block of the tile):
-//   plan_rows        the full rows P_{r,:} for a list of row indices r (transport_plan / wot_tmap row by row,
+//   plan_rows        the full rows P_{r,:}, or log P_{r,:}, for a list of row indices r (transport_plan / wot_tmap row by row,
 //                    src/trnopt/singlecell.py:89-92);
 //   plan_lse         out_i = log sum_j P_ij, per-(row, column split) partial (max, sum) pairs merged by a second
 //                    kernel in a fixed order (deterministic). With x and y swapped it gives log column sums, so
@@ -71,7 +71,8 @@ __device__ __forceinline__ void cost_tile(PlanSmem& s, const double* __restrict_
 __device__ __forceinline__ double opt_load(const double* p, int i) { return p ? p[i] : 0.0; }
 
 // grid.x = ceil(nrows / 64) * ceil(m / 64); out is (nrows, m) row-major. A row index outside [0, n) gives a row of
-// NaN (nothing is read for it).
+// NaN (nothing is read for it). kLog: log P instead of P.
+template <bool kLog>
 __global__ void __launch_bounds__(PTHREADS) plan_rows_kernel(const double* __restrict__ x, int n,
                                                              const double* __restrict__ y, int m, int d,
                                                              const double* __restrict__ f,
@@ -114,7 +115,8 @@ __global__ void __launch_bounds__(PTHREADS) plan_rows_kernel(const double* __res
     for (int b = 0; b < 4; ++b) {
       const int j = c0 + tc + 16 * b;
       if (j >= m) continue;
-      out[(size_t)r * m + j] = i >= 0 ? exp(lai + lbj[b] + (fi + gj[b] - c[a][b]) / eps) : nan("");
+      const double lp = lai + lbj[b] + (fi + gj[b] - c[a][b]) / eps;
+      out[(size_t)r * m + j] = i < 0 ? nan("") : kLog ? lp : exp(lp);
     }
   }
 }
@@ -214,14 +216,27 @@ size_t plan_lse_workspace_bytes(int device, int n, int m) {
   return (size_t)2 * plan_lse_splits(device, n, m) * (size_t)n * sizeof(double);
 }
 
-cudaError_t plan_rows_launch(const double* x, int n, const double* y, int m, int d, const double* f, const double* g,
-                             const double* la, const double* lb, double eps, const int* rows, int nrows, double* out,
-                             cudaStream_t stream) {
+template <bool kLog>
+static cudaError_t rows_launch(const double* x, int n, const double* y, int m, int d, const double* f, const double* g,
+                               const double* la, const double* lb, double eps, const int* rows, int nrows, double* out,
+                               cudaStream_t stream) {
   const long long tiles = (long long)((nrows + PT - 1) / PT) * ((m + PT - 1) / PT);
   if (tiles < 1) return cudaSuccess;
   if (tiles > 0x7fffffffLL) return cudaErrorInvalidValue;
-  plan_rows_kernel<<<(unsigned)tiles, PTHREADS, 0, stream>>>(x, n, y, m, d, f, g, la, lb, eps, rows, nrows, out);
+  plan_rows_kernel<kLog><<<(unsigned)tiles, PTHREADS, 0, stream>>>(x, n, y, m, d, f, g, la, lb, eps, rows, nrows, out);
   return cudaGetLastError();
+}
+
+cudaError_t plan_rows_launch(const double* x, int n, const double* y, int m, int d, const double* f, const double* g,
+                             const double* la, const double* lb, double eps, const int* rows, int nrows, double* out,
+                             cudaStream_t stream) {
+  return rows_launch<false>(x, n, y, m, d, f, g, la, lb, eps, rows, nrows, out, stream);
+}
+
+cudaError_t plan_log_rows_launch(const double* x, int n, const double* y, int m, int d, const double* f, const double* g,
+                                 const double* la, const double* lb, double eps, const int* rows, int nrows, double* out,
+                                 cudaStream_t stream) {
+  return rows_launch<true>(x, n, y, m, d, f, g, la, lb, eps, rows, nrows, out, stream);
 }
 
 cudaError_t plan_lse_launch(int device, const double* x, int n, const double* y, int m, int d, const double* f,

@@ -32,6 +32,7 @@ def _load():
 lib = _load()
 
 _P, _I, _F, _D, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_double, ctypes.c_size_t
+_L = ctypes.c_longlong
 _SIGS = {
     "trnopt_version": (_I, []),
     "trnopt_status_string": (ctypes.c_char_p, [_I]),
@@ -76,6 +77,13 @@ _SIGS = {
     "trnopt_plan_rows": (_I, [_P, _I, _P, _I, _I, _P, _P, _P, _P, _D, _P, _I, _P, _P]),
     "trnopt_plan_workspace_size": (_Z, [_I, _I]),
     "trnopt_plan_log_row_sums": (_I, [_P, _I, _P, _I, _I, _P, _P, _P, _P, _D, _P, _P, _Z, _P]),
+    "trnopt_plan_log_rows": (_I, [_P, _I, _P, _I, _I, _P, _P, _P, _P, _D, _P, _I, _P, _P]),
+    "trnopt_log_probs": (_I, [_I, _P, _L, _L, _I, _D, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "trnopt_log_probs_grad": (_I, [_I, _P, _L, _L, _I, _D, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
+    "trnopt_balance_workspace_size": (_Z, [_I, _I]),
+    "trnopt_balance": (_I, [_I, _P, _L, _I, _I, _D, _I, _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "trnopt_route": (_I, [_I, _P, _L, _L, _I, _I, _I, _P, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P]),
+    "trnopt_route_grad": (_I, [_I, _P, _L, _L, _I, _I, _I, _I, _F, _P, _P, _P, _L, _P]),
 }
 for _name, (_res, _args) in _SIGS.items():
     _fn = getattr(lib, _name)
@@ -238,16 +246,25 @@ def _plan_args(x, y, f, g, log_a, log_b):
                 raise ValueError(f"{nm} must have shape ({n},)")
 
 
-def plan_rows(x, y, f, g, log_a, log_b, eps, rows: torch.Tensor) -> torch.Tensor:
-    """Rows P[rows, :] of P = exp(log_a + log_b^T + (f + g^T - C) / eps), float64 (n, d) / (m, d) clouds."""
+def _plan_rows(call, x, y, f, g, log_a, log_b, eps, rows: torch.Tensor) -> torch.Tensor:
     _plan_args(x, y, f, g, log_a, log_b)
     _need(rows, "rows", torch.int32)
     n, d = x.shape
     m = y.shape[0]
     out = torch.empty((rows.numel(), m), dtype=torch.float64, device=x.device)
-    check(lib.trnopt_plan_rows(_ptr(x), n, _ptr(y), m, d, _ptr(f), _ptr(g), _ptr(log_a), _ptr(log_b), float(eps),
-                               _ptr(rows), rows.numel(), _ptr(out), _stream()), "trnopt_plan_rows")
+    check(getattr(lib, call)(_ptr(x), n, _ptr(y), m, d, _ptr(f), _ptr(g), _ptr(log_a), _ptr(log_b), float(eps),
+                             _ptr(rows), rows.numel(), _ptr(out), _stream()), call)
     return out
+
+
+def plan_rows(x, y, f, g, log_a, log_b, eps, rows: torch.Tensor) -> torch.Tensor:
+    """Rows P[rows, :] of P = exp(log_a + log_b^T + (f + g^T - C) / eps), float64 (n, d) / (m, d) clouds."""
+    return _plan_rows("trnopt_plan_rows", x, y, f, g, log_a, log_b, eps, rows)
+
+
+def plan_log_rows(x, y, f, g, log_a, log_b, eps, rows: torch.Tensor) -> torch.Tensor:
+    """Rows log P[rows, :], float64."""
+    return _plan_rows("trnopt_plan_log_rows", x, y, f, g, log_a, log_b, eps, rows)
 
 
 def plan_log_row_sums(x, y, f, g, log_a, log_b, eps) -> torch.Tensor:

@@ -14,16 +14,21 @@ built from it, on the host with NumPy in float64; here the same float64 arithmet
                                               (examples/sinkhorn_libs_compare.py:43-56)
     pull_back(x0, x1, res, log_v1)            normalized log(P v), the ancestor pull-back
                                               (examples/singlecell_figures.py:35-47)
+    descendants(x, y, res, rows, targets, top, a, b)
+                                              rows of P as distributions over y: log-probabilities of given points,
+                                              entropy, the most probable points (trnopt.scores.log_probs)
 
 The sums are float64 log-sum-exps, so rows whose terms all underflow exp() still come out right in log form.
 """
 
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import numpy as np
 import torch
 
-from . import _capi
+from . import _capi, scores
 
 
 def _device() -> torch.device:
@@ -65,13 +70,17 @@ def _inputs(x, y, res, a, b):
     return dev, _dev(x, dev), _dev(y, dev), _dev(res.f, dev), _dev(res.g, dev), _dev(la, dev), _dev(lb, dev)
 
 
-def plan_rows(x, y, res, rows, a=None, b=None) -> np.ndarray:
-    """Rows P[rows, :] (len(rows), m) in float64. Row indices follow NumPy rules (negative counts from the end)."""
-    n = len(x)
+def _row_index(rows, n: int) -> np.ndarray:
+    """Row numbers 0 .. n - 1 from NumPy-style indices (negative ones count from the end)."""
     idx = np.asarray(rows, dtype=np.int64).reshape(-1)
     if np.any(idx < -n) or np.any(idx >= n):
         raise IndexError(f"row index out of range for {n} rows")
-    idx = np.where(idx < 0, idx + n, idx).astype(np.int32)
+    return np.where(idx < 0, idx + n, idx).astype(np.int32)
+
+
+def plan_rows(x, y, res, rows, a=None, b=None) -> np.ndarray:
+    """Rows P[rows, :] (len(rows), m) in float64. Row indices follow NumPy rules (negative counts from the end)."""
+    idx = _row_index(rows, len(x))
     dev, xd, yd, f, g, la, lb = _inputs(x, y, res, a, b)
     out = _capi.plan_rows(xd, yd, f, g, la, lb, res.eps, torch.as_tensor(idx).to(dev))
     return out.cpu().numpy()
@@ -116,3 +125,43 @@ def pull_back(x0, x1, res, log_v1) -> np.ndarray:
     out = _capi.plan_log_row_sums(_dev(x, dev), _dev(y, dev), _dev(res.f, dev), _dev(res.g, dev), None,
                                   _dev(lv, dev), res.eps)
     return (out - torch.logsumexp(out, 0)).cpu().numpy()
+
+
+class Descendants(NamedTuple):
+    log_prob: np.ndarray | None      # (rows,) or (rows, T): log P(y = targets | x = row); None without targets
+    entropy: np.ndarray              # (rows,) entropy of P(y | x = row), nats
+    log_mass: np.ndarray             # (rows,) log of the plan's row sum
+    top_log_prob: np.ndarray         # (rows, top) log-probabilities of the most probable points, best first
+    top_index: np.ndarray            # (rows, top) their indices in y, -1 where y has fewer points
+
+
+_BLOCK = 1 << 25                     # plan entries evaluated at a time by descendants (256 MB of float64)
+
+
+def descendants(x, y, res, rows=None, targets=None, top: int = 10, a=None, b=None) -> Descendants:
+    """Rows of the plan as distributions over y: P(y_j | x_i) = P_ij / sum_j P_ij, for the given rows (None: all).
+    targets (len(rows),) or (len(rows), T) asks for the log-probabilities of given points of y per row (-1: padding,
+    0 is returned). The plan's rows are evaluated in float64 a block at a time and go through
+    trnopt.scores.log_probs, so nothing of size n x m is kept. With x and y swapped (and the result's f and g, a and b)
+    the same call gives ancestors."""
+    idx = np.arange(len(x), dtype=np.int32) if rows is None else _row_index(rows, len(x))
+    if not 0 <= top <= scores.MAX_TOP:
+        raise ValueError(f"top must lie in 0 .. {scores.MAX_TOP}")
+    if targets is not None:
+        targets = np.asarray(targets)
+        if targets.dtype.kind not in "iu" or targets.ndim not in (1, 2) or len(targets) != len(idx):
+            raise ValueError("targets must be whole numbers of shape (rows,) or (rows, T)")
+        if np.any(targets >= len(y)):
+            raise IndexError(f"target index out of range for {len(y)} points")
+    dev, xd, yd, f, g, la, lb = _inputs(x, y, res, a, b)
+    idx = torch.as_tensor(idx).to(dev)
+    step = max(1, _BLOCK // len(y))
+    parts = []
+    for r in range(0, max(1, len(idx)), step):
+        log_rows = _capi.plan_log_rows(xd, yd, f, g, la, lb, res.eps, idx[r:r + step])
+        t = None if targets is None else torch.as_tensor(targets[r:r + step].astype(np.int64)).to(dev)
+        parts.append(scores.log_probs(log_rows, t, top=top))
+    cat = lambda name: torch.cat([getattr(p, name) for p in parts]).cpu().numpy()
+    best = (cat("top_log_prob"), cat("top_index")) if top else (np.empty((len(idx), 0)),
+                                                                 np.empty((len(idx), 0), dtype=np.int64))
+    return Descendants(None if targets is None else cat("log_prob"), cat("entropy"), cat("lse"), *best)

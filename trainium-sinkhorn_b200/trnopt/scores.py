@@ -1,0 +1,299 @@
+"""Assignment of rows to columns from a score matrix that a program already holds, on the GPU.
+
+sinkhorn() and trnopt.plan take two point clouds and never store their scores. Here the scores S (rows x columns) are
+given, as by a model's output layer or a router, and three operators work on them:
+
+    log_probs(S, targets, top=k)   each row's softmax: log-probabilities of given columns, entropy, log-sum-exp, the k
+                                   best columns; differentiable
+    balance(S, eps=, iters=)       Sinkhorn on S: the potentials f, g of the entropic transport plan between rows and
+                                   columns, P_ij = a_i b_j exp((f_i + g_j + S_ij) / eps)
+    route(S, k, ...)               each row's k best columns by softmax or sigmoid scores, with a bias for balance
+                                   (balance's g, or one of the program's own), groups and weights; differentiable
+
+A balanced router is the three in a row: g = balance(S).g; r = route(S, k, bias=g, bias_on="logits"); the entropy of
+log_probs(S) tells how decided the rows are. trnopt.plan.descendants applies log_probs to the rows of a plan.
+
+Scores are CUDA tensors of any leading shape and row pitch (a last dimension that is not contiguous is copied first).
+The calls queue on the scores' device, on that device's current stream, return without waiting, and can be captured into
+a CUDA graph. There is no CPU path. What a call rejects it rejects before anything is queued, with ValueError; values on
+the device (an index out of range, NaN) never raise and show in the results as described.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from . import _capi
+
+MAX_TOP = 64             # log_probs: best columns per row
+MAX_TARGETS = 1024       # log_probs: given columns per row
+MAX_COLUMNS = 1024       # balance, route: columns
+MAX_CHOICES = 32         # route: choices per row, groups
+
+_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float64: 3}
+_KIND = {"softmax": 0, "sigmoid": 1}
+_BIAS_ON = {"scores": 0, "logits": 1}
+
+
+class LogProbs(NamedTuple):
+    log_prob: torch.Tensor | None       # targets' shape
+    entropy: torch.Tensor               # scores.shape[:-1], nats
+    lse: torch.Tensor                   # scores.shape[:-1]: log sum_j exp(S_j / temperature)
+    top_log_prob: torch.Tensor | None   # scores.shape[:-1] + (top,), best first
+    top_index: torch.Tensor | None      # the same shape, int64
+
+
+class Balance(NamedTuple):
+    f: torch.Tensor                     # scores.shape[:-1], float32
+    g: torch.Tensor                     # (columns,), float32
+
+
+class Routing(NamedTuple):
+    index: torch.Tensor                 # scores.shape[:-1] + (top,), int64, best first
+    weight: torch.Tensor                # the same shape, float32
+    load: torch.Tensor | None           # (columns,) int32: rows that chose each column
+
+
+def _matrix(scores: torch.Tensor, double: bool) -> torch.Tensor:
+    """The scores as a 2-d view with unit column stride (a copy only where there is no such view)."""
+    if not isinstance(scores, torch.Tensor) or not scores.is_cuda:
+        raise ValueError("scores must be a CUDA tensor (the score kernels have no CPU path)")
+    if scores.dtype not in _TYPE or (scores.dtype == torch.float64 and not double):
+        raise ValueError(f"scores of type {scores.dtype} are not supported")
+    if scores.dim() < 1 or scores.shape[-1] < 1:
+        raise ValueError("scores need at least one column")
+    if scores.shape[-1] >= 2 ** 31:
+        raise ValueError("scores have too many columns")
+    s = scores if scores.dim() == 2 else scores.reshape(-1, scores.shape[-1])
+    return s if s.stride(1) == 1 or s.shape[1] == 1 else s.contiguous()
+
+
+def _small(t: torch.Tensor | None, n: int, name: str, like: torch.Tensor) -> torch.Tensor | None:
+    """A float32 vector of n values on the scores' device."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype != torch.float32 or t.numel() != n:
+        raise ValueError(f"{name} must hold {n} float32 values on {like.device}")
+    return t.detach().contiguous()
+
+
+def _call(name: str, like: torch.Tensor, *args) -> None:
+    """A C call on the device of `like`, on that device's current stream."""
+    index = like.device.index
+    fn = getattr(_capi.lib, name)
+    if index == torch.cuda.current_device():
+        status = fn(*args, ctypes.c_void_p(torch.cuda.current_stream(index).cuda_stream))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, ctypes.c_void_p(torch.cuda.current_stream(index).cuda_stream))
+    _capi.check(status, name)
+
+
+def _at(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+# log_probs -----------------------------------------------------------------------------------------------------------
+
+def _log_probs_forward(s, targets, top, temperature, keep):
+    rows, cols = s.shape
+    wide = torch.float64 if s.dtype == torch.float64 else torch.float32
+    n_targets = 0 if targets is None else targets.shape[1]
+
+    def new(*shape, dtype=wide):
+        return torch.empty(shape, dtype=dtype, device=s.device)
+
+    log_prob, entropy, lse = new(rows, n_targets), new(rows), new(rows)
+    top_log_prob, top_index = new(rows, top), new(rows, top, dtype=torch.int64)
+    row_max, log_sum = (new(rows), new(rows)) if keep else (None, None)
+    _call("trnopt_log_probs", s, _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, temperature, _at(targets),
+          n_targets, top, _at(log_prob), _at(entropy), _at(lse), _at(top_log_prob), _at(top_index), _at(row_max),
+          _at(log_sum))
+    return log_prob, entropy, lse, top_log_prob, top_index, row_max, log_sum
+
+
+class _LogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, s, targets, top, temperature):
+        *out, row_max, log_sum = _log_probs_forward(s, targets, top, temperature, True)
+        ctx.save_for_backward(s, targets, out[4], row_max, log_sum, out[1])
+        ctx.top, ctx.temperature = top, temperature
+        ctx.mark_non_differentiable(out[4])
+        ctx.set_materialize_grads(False)
+        return tuple(out)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_log_prob, d_entropy, d_lse, d_top, _):
+        s, targets, top_index, row_max, log_sum, entropy = ctx.saved_tensors
+        rows, cols = s.shape
+        grad = torch.empty((rows, cols), dtype=s.dtype, device=s.device)
+        up = [None if d is None else d.contiguous() for d in (d_log_prob, d_entropy, d_lse, d_top)]
+        _call("trnopt_log_probs_grad", s, _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, ctx.temperature,
+              _at(targets), 0 if targets is None else targets.shape[1], _at(top_index), ctx.top, _at(row_max),
+              _at(log_sum), _at(entropy), *map(_at, up), _at(grad), cols)
+        return grad, None, None, None
+
+
+def log_probs(scores: torch.Tensor, targets: torch.Tensor | None = None, *, top: int = 0,
+              temperature: float = 1.0) -> LogProbs:
+    """The softmax of scores / temperature over the last dimension, never stored: the log-probabilities of given
+    columns, the entropy (nats), the log-sum-exp, and the `top` best columns (score descending, equal scores by lower
+    index).
+
+    scores   float32, float16, bfloat16 or float64, any leading shape L and row pitch
+    targets  int64 (int32 is converted), of shape L or L + (T,): column indices per row. Negative ones are padding
+             (log_prob 0, no gradient), ones past the last column give NaN (and no gradient)
+    Results are float32 (float64 for float64 scores). Columns of score -inf are closed: probability 0. In a row of
+    nothing else log_prob and lse are -inf, entropy 0, and gradients 0; best columns beyond the open ones are -inf with
+    index -1. A row holding NaN or +inf has NaN values and top_index -1. All floating outputs are differentiable with
+    respect to the scores (once); the gradient has the scores' type."""
+    s = _matrix(scores, True)
+    if not 0 <= top <= MAX_TOP:
+        raise ValueError(f"top must lie in 0 .. {MAX_TOP}")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError("temperature must be positive and finite (1e-30 .. 1e30)")
+    lead = scores.shape[:-1]
+    t = None
+    if targets is not None:
+        if not isinstance(targets, torch.Tensor) or targets.device != scores.device or \
+                targets.dtype not in (torch.int64, torch.int32):
+            raise ValueError(f"targets must be an int64 or int32 tensor on {scores.device}")
+        if targets.shape != lead and targets.shape[:-1] != lead:
+            raise ValueError(f"targets must have shape {tuple(lead)} or {tuple(lead)} + (T,)")
+        per_row = 1 if targets.shape == lead else targets.shape[-1]
+        if per_row > MAX_TARGETS:
+            raise ValueError(f"at most {MAX_TARGETS} targets a row")
+        t = targets.reshape(s.shape[0], per_row).to(torch.int64).contiguous()
+    if s.requires_grad and torch.is_grad_enabled():
+        log_prob, entropy, lse, top_log_prob, top_index = _LogProbs.apply(s, t, int(top), float(temperature))
+    else:
+        log_prob, entropy, lse, top_log_prob, top_index, _, _ = _log_probs_forward(s.detach(), t, int(top),
+                                                                                   float(temperature), False)
+    return LogProbs(None if t is None else log_prob.view(targets.shape), entropy.view(lead), lse.view(lead),
+                    top_log_prob.view(*lead, top) if top else None, top_index.view(*lead, top) if top else None)
+
+
+# balance -------------------------------------------------------------------------------------------------------------
+
+def balance(scores: torch.Tensor, *, eps: float = 0.05, iters: int = 20, a: torch.Tensor | None = None,
+            b: torch.Tensor | None = None, g: torch.Tensor | None = None) -> Balance:
+    """`iters` Sinkhorn iterations on a score matrix, from the column potential g (None: 0):
+
+        f_i = -eps LSE_j(log b_j + (g_j + S_ij) / eps),   g_j = -eps LSE_i(log a_i + (f_i + S_ij) / eps)
+
+    the half-steps of sinkhorn() for the cost -S. After the last one the columns of P_ij = a_i b_j exp((f_i + g_j +
+    S_ij) / eps) sum to b exactly and its rows to a as far as the iteration has converged; route(..., bias=g,
+    bias_on="logits") chooses each row's largest entries of P / b.
+
+    scores   float32, float16 or bfloat16, at most 1024 columns
+    a, b     row and column masses, float32, >= 0 (None: 1 / rows, 1 / columns). Padding rows have mass 0: they move no
+             column, and still get their f. Masses are used as given (their sums should agree)
+    g        a starting potential, for instance the last step's
+    A row or column whose terms are all zero (scores -inf, masses 0) has potential 0. The potentials are constants to
+    autograd."""
+    s = _matrix(scores, False).detach()
+    rows, cols = s.shape
+    if cols > MAX_COLUMNS:
+        raise ValueError(f"at most {MAX_COLUMNS} columns")
+    if rows < 1 or rows >= 2 ** 31:
+        raise ValueError("scores need between 1 and 2**31 - 1 rows")
+    if not 1e-30 <= eps <= 1e30:
+        raise ValueError("eps must be positive and finite (1e-30 .. 1e30)")
+    if iters < 1:
+        raise ValueError("iters must be at least 1")
+    a, b, g = _small(a, rows, "a", s), _small(b, cols, "b", s), _small(g, cols, "g", s)
+    f = torch.empty(rows, dtype=torch.float32, device=s.device)
+    g_out = torch.empty(cols, dtype=torch.float32, device=s.device)
+    with torch.cuda.device(s.device):
+        nbytes = int(_capi.lib.trnopt_balance_workspace_size(rows, cols))
+    ws = torch.empty(max(256, nbytes), dtype=torch.uint8, device=s.device)
+    _call("trnopt_balance", s, _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, float(eps), int(iters), _at(a),
+          _at(b), _at(g), _at(f), _at(g_out), _at(ws), ws.numel())
+    return Balance(f.view(scores.shape[:-1]), g_out)
+
+
+# route ---------------------------------------------------------------------------------------------------------------
+
+def _route_forward(s, top, kind, bias, bias_on, groups, top_groups, group_top, renormalize, scale, load):
+    rows, cols = s.shape
+    index = torch.empty((rows, top), dtype=torch.int64, device=s.device)
+    weight = torch.empty((rows, top), dtype=torch.float32, device=s.device)
+    counts = torch.empty(cols, dtype=torch.int32, device=s.device) if load else None
+    _call("trnopt_route", s, _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, top, kind, _at(bias), bias_on,
+          groups, top_groups, group_top, renormalize, scale, _at(index), _at(weight), _at(counts))
+    return weight, index, counts
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, s, top, kind, bias, bias_on, groups, top_groups, group_top, renormalize, scale, load):
+        weight, index, counts = _route_forward(s, top, kind, bias, bias_on, groups, top_groups, group_top,
+                                               renormalize, scale, load)
+        ctx.save_for_backward(s, index)
+        ctx.call = (top, kind, renormalize, scale)
+        ctx.mark_non_differentiable(*((index,) if counts is None else (index, counts)))
+        return weight, index, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_weight, *_):
+        s, index = ctx.saved_tensors
+        rows, cols = s.shape
+        grad = torch.empty((rows, cols), dtype=s.dtype, device=s.device)
+        d_weight = d_weight.contiguous()
+        _call("trnopt_route_grad", s, _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, *ctx.call, _at(index),
+              _at(d_weight), _at(grad), cols)
+        return (grad,) + (None,) * 10
+
+
+def route(scores: torch.Tensor, top: int, *, kind: str = "softmax", bias: torch.Tensor | None = None,
+          bias_on: str = "scores", groups: int = 1, top_groups: int | None = None, group_top: int = 2,
+          renormalize: bool = True, scale: float = 1.0, load: bool = False) -> Routing:
+    """Each row's `top` best columns and their weights.
+
+    kind         a column's share of a row: "softmax" over the row, or "sigmoid" of its score
+    bias         (columns,) float32, in the choice only: added to the shares (bias_on="scores") or to the scores
+                 themselves (bias_on="logits": balance's g). -inf closes a column. Without a bias columns go by their
+                 scores
+    groups       columns form `groups` equal runs; the `top_groups` (None: all) runs with the largest sum of their
+                 `group_top` (1 or 2) largest biased shares (bias on the logits: biased scores) stay open
+    weight       scale * share, or with renormalize scale * share / (sum of the row's chosen shares)
+    load         count the rows that chose each column
+
+    scores are float32, float16 or bfloat16, of at most 1024 columns; top and groups are at most 32. The order is that
+    of the keys in 64 bits, equal keys by lower index. Columns of score -inf are closed; slots that no open column fills
+    hold index -1 and weight 0. A row holding NaN or +inf (or a NaN bias) chooses nothing: index -1, weight NaN. The
+    weights are differentiable with respect to the scores (once; the choice and the bias are constants); a row that
+    chose nothing has gradient 0."""
+    s = _matrix(scores, False)
+    rows, cols = s.shape
+    if cols > MAX_COLUMNS:
+        raise ValueError(f"at most {MAX_COLUMNS} columns")
+    if kind not in _KIND:
+        raise ValueError(f"kind={kind!r}: choose 'softmax' or 'sigmoid'")
+    if bias_on not in _BIAS_ON:
+        raise ValueError(f"bias_on={bias_on!r}: choose 'scores' or 'logits'")
+    if not 1 <= groups <= MAX_CHOICES or cols % groups:
+        raise ValueError(f"groups must divide the columns and lie in 1 .. {MAX_CHOICES}")
+    top_groups = groups if top_groups is None else top_groups
+    if not 1 <= top_groups <= groups:
+        raise ValueError("top_groups must lie in 1 .. groups")
+    if group_top not in (1, 2):
+        raise ValueError("group_top must be 1 or 2")
+    if not 1 <= top <= min(MAX_CHOICES, top_groups * (cols // groups)):
+        raise ValueError(f"top must lie in 1 .. {MAX_CHOICES} and not exceed the columns of the open groups")
+    if not abs(scale) < 1e30:
+        raise ValueError("scale must be finite")
+    bias = _small(bias, cols, "bias", s)
+    args = (int(top), _KIND[kind], bias, _BIAS_ON[bias_on], int(groups), int(top_groups), int(group_top),
+            int(bool(renormalize)), float(scale), bool(load))
+    if s.requires_grad and torch.is_grad_enabled():
+        weight, index, counts = _Route.apply(s, *args)
+    else:
+        weight, index, counts = _route_forward(s.detach(), *args)
+    lead = scores.shape[:-1]
+    return Routing(index.view(*lead, top), weight.view(*lead, top), counts)
