@@ -8,15 +8,23 @@
 // Sums in float32 (float64 for float64 scores).
 //
 // Forward: one pass over the scores. A row belongs to one CTA, or to the CTAs of a cluster when there are few rows;
-// each thread holds 64 bytes of scores at a time (and the next 64 in flight), and keeps its own (m, s, sum e d),
-// rescaled when its maximum rises. The best columns come out of the same pass: a bound below the K-th largest score is
-// kept from the threads' running maxima (the K / warps-th largest of each warp's 32: at least K scores reach the
-// smallest of these), raised after 1, 2, 4, 8, ... chunks, and the few scores above it are collected in a list that is
-// ranked at the end. Where ties or ascending scores overflow the list, the chunk in registers and the list are cut to
-// the K best by bisection.
+// each thread works on 64 bytes of scores at a time, which it brings through shared memory itself (asynchronous copies,
+// two more chunks in flight, no barrier), and keeps its own state: the largest score
+// m, and with M = m c rounded (c = log2 e / T, or 1 / T in float64) the sums s = sum exp(x c - M) and
+// t = sum exp(x c - M) (x c - M), both rescaled when m rises. M is a shift like any other, so its rounding cancels. Rows
+// whose M would not be an ordinary number (scores near the type's lowest value throughout) are summed again by the
+// differences x - m.
+// The best columns come out of the same pass: a bound below the K-th largest score is kept from the threads' running
+// maxima (the K / warps-th largest of each warp's 32: at least K scores reach the smallest of these), raised after 1, 2,
+// 4, 8, ... chunks, and each warp collects the few scores that reach it in a list of its own. The lists are ranked at
+// the end. Where ties or ascending scores overflow a list, the warp cuts the list and the chunk it holds to their K best
+// by bisection. Nothing but the first bound makes warps wait for one another.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "common.cuh"
+#include "kernels.h"
 #include "score_types.cuh"
 #include "scores.h"
 
@@ -28,7 +36,8 @@ namespace {
 
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int LP_VECS = 4;          // 16-byte vectors a thread holds of a chunk
-constexpr int LP_LIST = 1024;       // candidates held for the best columns
+constexpr int LP_LIST = 96;         // candidates for the best columns that a warp holds (more than 64)
+constexpr float kWide = 1e30f;      // shifts M beyond this are not used
 
 // exp and log in the units of the sums: base 2 for float32, base e for float64. unit() turns such a logarithm into nats.
 struct Base2 {
@@ -46,18 +55,22 @@ struct BaseE {
 template <typename T> struct Base { using type = Base2; };
 template <> struct Base<double> { using type = BaseE; };
 
-// (S - m) c, at least -1e30: -inf scores (and -inf maxima) give exp() = 0 and a finite factor.
-__device__ __forceinline__ float down(float x, float m, float c) { return fmaxf((x - m) * c, -1e30f); }
-__device__ __forceinline__ double down(double x, double m, double c) { return fmax((x - m) * c, -1e30); }
+// At least -1e30: differences to scores (or maxima) of -inf give exp() = 0 and a finite factor; NaN becomes -1e30 too.
+__device__ __forceinline__ float floored(float d) { return fmaxf(d, -1e30f); }
+__device__ __forceinline__ double floored(double d) { return fmax(d, -1e30); }
 
-// A softmax's running state: the largest score m, s = sum exp(d), t = sum exp(d) d.
+// M: the rounded product itself, never contracted into what uses it.
+__device__ __forceinline__ float shift(float m, float c) { return __fmul_rn(m, c); }
+__device__ __forceinline__ double shift(double m, double c) { return __dmul_rn(m, c); }
+
+// A softmax's running state: the largest score m; s and t relative to M = m c.
 template <typename A, typename B>
 struct Sums {
   A m, s, t;
   __device__ __forceinline__ void raise(A to, A c) {          // to the larger maximum `to`
-    const A d = down(m, to, c), w = B::exp(d);
-    t = w * (t + s * d);
-    s = w * s;
+    const A d = floored(shift(m, c) - shift(to, c)), w = B::exp(d);
+    t = w > 0 ? w * (t + s * d) : 0;                          // (sums about an M of -inf are no numbers)
+    s = w > 0 ? w * s : 0;
     m = to;
   }
   __device__ __forceinline__ void add(Sums o, A c) {
@@ -115,94 +128,111 @@ struct Candidate {
 template <typename A>
 __device__ __forceinline__ bool better(A x, int j, A ox, int oj) { return x > ox || (x == ox && j < oj); }
 
-template <typename A, int NW>
-struct TopSmem {
-  Candidate<A> list[LP_LIST], kept[LP_LIST];
-  A bound[NW];
-  int count, kept_count, wcount[NW];
-};
-
-template <typename A, int NW>
+// Shared memory of a CTA of NW warps. The ring holds kStages chunks; after the scores it serves as `kept`, the
+// candidates brought together (NW lists, or 64 best columns of each of a cluster's 8 CTAs).
+template <typename A, int NW, bool kTop>
 struct LogProbsSmem {
+  static constexpr int kStages = NW == 8 ? 3 : 2;
+  uint4 ring[kStages * LP_VECS * 32 * NW];
+  Candidate<A> list[kTop ? NW : 1][kTop ? LP_LIST : 1];
+  volatile A bound[NW];
+  int count[NW], kept_count;
   A m[NW], s[NW], t[NW];
-  Sums<A, typename Base<A>::type> part[8];                 // of a cluster's CTAs (written into the first one's)
+  Sums<A, typename std::conditional<sizeof(A) == 8, BaseE, Base2>::type> part[8];   // of a cluster's CTAs (the first's)
+  __device__ __forceinline__ Candidate<A>* kept() { return reinterpret_cast<Candidate<A>*>(ring); }
 };
 
-// Number of threads' items over the CTA (every thread gets it).
-template <typename A, int NW>
-__device__ __forceinline__ int block_count(TopSmem<A, NW>& sh, int n) {
-  n = __reduce_add_sync(kAll, n);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh.wcount[threadIdx.x >> 5] = n;
-  __syncthreads();
-  int r = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) r += sh.wcount[w];
-  return r;
-}
+template <typename A>
+struct Collected {
+  int n;       // the warp's candidates
+  A own;       // at least this many reach it: the list's K-th value once the list was cut
+};
 
-// The K best of the list's first n candidates and the chunk in registers, as the new list: bisection on the K-th value,
-// then on the column up to which columns of just that value are taken. Returns that value; all threads must call it.
-template <typename T, typename A, int NW>
-__device__ __noinline__ A cut_to_best(TopSmem<A, NW>& sh, const Vec<T> (&q)[LP_VECS], long long col0, int n, int top) {
-  constexpr int NT = 32 * NW, kN = Vec<T>::kN, kOwn = LP_LIST / NT;
+// Adds the scores of the warp's chunk that reach `bound` and exceed `own` to its list. A thread's vectors are
+// mine[i * stride] and hold the columns from col0 + i * step on. If the list overflows, it is cut to the K best of its
+// first n candidates and the chunk: bisection on the K-th value, then on the column up to which columns of just that
+// value are taken.
+template <typename T, typename A>
+__device__ __noinline__ Collected<A> collect(const uint4* mine, int stride, long long col0, int step,
+                                             Candidate<A>* list, int* count, int n, A bound, A own, int top) {
+  constexpr int kN = Vec<T>::kN, kOwn = LP_LIST / 32;
   using Key = decltype(order(A()));
-  Candidate<A> own[kOwn];
-  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (int i = 0; i < LP_VECS; ++i) {
+    const Vec<T> q{mine[i * stride]};
+    const A peak = q.peak();
+    if (!(peak >= bound && peak > own)) continue;
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      const A x = q.get(e);
+      if (x >= bound && x > own) {
+        const int at = atomicAdd(count, 1);
+        if (at < LP_LIST) list[at] = {x, (int)(col0 + (long long)i * step + e)};
+      }
+    }
+  }
+  __syncwarp();
+  const int found = *(volatile int*)count;
+  if (found <= LP_LIST) return {found, own};
+
+  Candidate<A> old[kOwn];
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
-    const int e = threadIdx.x + i * NT;
-    own[i].x = e < n ? sh.list[e].x : (A)-INFINITY;
-    own[i].j = e < n ? sh.list[e].j : 0;
+    const int e = lane + i * 32;
+    old[i].x = e < n ? list[e].x : (A)-INFINITY;
+    old[i].j = e < n ? list[e].j : 0;
   }
   auto each = [&](auto&& f) {
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) f(own[i].x, own[i].j);
+    for (int i = 0; i < kOwn; ++i) f(old[i].x, old[i].j);
+    for (int i = 0; i < LP_VECS; ++i) {
+      const Vec<T> q{mine[i * stride]};
 #pragma unroll
-    for (int i = 0; i < LP_VECS; ++i)
-#pragma unroll
-      for (int e = 0; e < kN; ++e) f(q[i].get(e), (int)(col0 + (long long)i * NT * kN + e));
+      for (int e = 0; e < kN; ++e) f(q.get(e), (int)(col0 + (long long)i * step + e));
+    }
   };
+  // bfloat16 scores differ in the upper 16 bits of their keys alone (the lower ones are 0, or 1 for negative scores)
+  constexpr int kLowBit = std::is_same<T, __nv_bfloat16>::value ? 16 : 0;
   Key k = 0;                                               // the largest key that at least `top` scores reach
-  for (int bit = 8 * (int)sizeof(Key) - 1; bit >= 0; --bit) {
+  for (int bit = 8 * (int)sizeof(Key) - 1; bit >= kLowBit; --bit) {
     const Key next = k | ((Key)1 << bit);
-    const A bound = value(next);
+    const A at = value(next);
     int c = 0;
-    if (bound > (A)-INFINITY) {                            // (keys of NaN are above every score's)
-      each([&](A x, int) { c += x >= bound; });
-    } else {
+    if (at > (A)-INFINITY) {
+      each([&](A x, int) { c += x >= at; });
+    } else {                                               // -inf and below it, or past every score (keys of NaN)
       c = next <= order((A)-INFINITY) ? LP_LIST : 0;
     }
-    if (block_count(sh, c) >= top) k = next;
+    if ((int)__reduce_add_sync(kAll, c) >= top) k = next;
   }
+  if (kLowBit > 0 && !(k >> (8 * sizeof(Key) - 1))) k |= ((Key)1 << kLowBit) - 1;
   const A kth = value(k);
   const bool all = !(kth > (A)-INFINITY);                  // fewer open columns than `top`: take them all
-  int more = 0;
-  each([&](A x, int) { more += x > (all ? (A)-INFINITY : kth); });
-  const int wanted = all ? 0 : top - block_count(sh, more);
   int last = -1;                                           // columns of the K-th value are taken up to this one
   if (!all) {
+    int more = 0;
+    each([&](A x, int) { more += x > kth; });
+    const int wanted = top - (int)__reduce_add_sync(kAll, more);
     int low = 0, high = 0x7fffffff;
     while (low < high) {                                   // the smallest column that gives `wanted` of them
       const int mid = low + (high - low) / 2;
       int c = 0;
       each([&](A x, int j) { c += x == kth && j <= mid; });
-      if (block_count(sh, c) >= wanted) high = mid;
+      if ((int)__reduce_add_sync(kAll, c) >= wanted) high = mid;
       else low = mid + 1;
     }
     last = low;
   }
-  __syncthreads();
-  if (threadIdx.x == 0) sh.count = 0;
-  __syncthreads();
+  if (lane == 0) *count = 0;
+  __syncwarp();
   each([&](A x, int j) {
     if (all ? x > (A)-INFINITY : (x > kth || (x == kth && j <= last))) {
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < LP_LIST) sh.list[at] = {x, j};
+      const int at = atomicAdd(count, 1);
+      if (at < LP_LIST) list[at] = {x, j};
     }
   });
-  __syncthreads();
-  return all ? (A)-INFINITY : kth;
+  __syncwarp();
+  return {min(*(volatile int*)count, LP_LIST), all ? own : fmax(own, kth)};
 }
 
 // The candidates of `in` ranked by (score, lower column): the `top` best into out (in order), the others dropped.
@@ -216,14 +246,60 @@ __device__ __forceinline__ void rank_into(const Candidate<A>* in, int n, int top
   }
 }
 
+// One chunk's sums relative to M: exp(d) and exp(d) d over the vectors, d = x c - M.
+template <typename T, typename A, typename B>
+__device__ __forceinline__ void chunk_sums(const Vec<T> (&q)[LP_VECS], A c, A M, A& s, A& t) {
+  constexpr int kN = Vec<T>::kN;
+  if constexpr (sizeof(A) == 4) {
+    const uint64_t c2 = pack2(c, c), m2 = pack2(-M, -M);
+    uint64_t s2 = 0, t2 = 0;                                // two sums each, of the even and the odd scores
+#pragma unroll
+    for (int i = 0; i < LP_VECS; ++i)
+#pragma unroll
+      for (int e = 0; e < kN; e += 2) {
+        const uint64_t d2 = fma2(pack2(q[i].get(e), q[i].get(e + 1)), c2, m2);
+        float d0, d1;
+        unpack2(d2, d0, d1);
+        const uint64_t x2 = pack2(B::exp(d0), B::exp(d1));
+        s2 = add2(s2, x2);
+        t2 = fma2(x2, d2, t2);
+      }
+    float a, b;
+    unpack2(s2, a, b);
+    s = a + b;
+    unpack2(t2, a, b);
+    t = a + b;
+  } else {
+    s = t = 0;
+#pragma unroll
+    for (int i = 0; i < LP_VECS; ++i)
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const A d = fma(q[i].get(e), c, -M), x = B::exp(d);
+        s += x;
+        t = fma(x, d, t);
+      }
+  }
+  if (!(t == t)) {                                          // a score of -inf (0 * -inf) or NaN: the same with a floor
+    s = t = 0;
+    for (int i = 0; i < LP_VECS; ++i)
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const A d = floored(fma(q[i].get(e), c, -M)), x = B::exp(d);
+        s += x;
+        t = fma(x, d, t);
+      }
+  }
+}
+
 template <typename T, int NW, bool kTop>
-__global__ void __launch_bounds__(32 * NW) log_probs_kernel(LogProbsProblem p, int parts) {
+__global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsProblem p, int parts) {
   using A = typename Acc<T>::type;
   using B = typename Base<T>::type;
-  constexpr int NT = 32 * NW, kN = Vec<T>::kN;
-  __shared__ LogProbsSmem<A, NW> sh;
-  __shared__ __align__(16) unsigned char top_bytes[kTop ? sizeof(TopSmem<A, NW>) : 16];
-  TopSmem<A, NW>& st = *reinterpret_cast<TopSmem<A, NW>*>(top_bytes);
+  using Smem = LogProbsSmem<A, NW, kTop>;
+  constexpr int NT = 32 * NW, kN = Vec<T>::kN, kChunk = NT * LP_VECS, kStages = Smem::kStages;
+  extern __shared__ __align__(16) unsigned char smem_bytes[];
+  Smem& sh = *reinterpret_cast<Smem*>(smem_bytes);
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const long long row = blockIdx.x / parts;
   const int part = (int)(blockIdx.x % parts);
@@ -231,6 +307,26 @@ __global__ void __launch_bounds__(32 * NW) log_probs_kernel(LogProbsProblem p, i
   const RowVectors<T> rv(scores, p.cols);
   const long long per = (rv.count + parts - 1) / parts, v0 = part * per, v1 = min(rv.count, v0 + per);
   const A c = B::scale(p.temperature), inf = (A)INFINITY;
+
+  uint4* mine = sh.ring + tid;                              // stage s, vector i: mine[(s * LP_VECS + i) * NT]
+  auto fetch = [&](long long v, int stage) {                // the thread's vectors of the chunk at v, as one copy group
+    uint4* to = mine + stage * LP_VECS * NT;
+    if (v + kChunk <= v1 && rv.inside(v, kChunk)) {
+      const T* at = scores + rv.column(v + tid);
+#pragma unroll
+      for (int i = 0; i < LP_VECS; ++i) copy_async16(to + i * NT, at + i * NT * kN);
+    } else if (v < v1) {
+#pragma unroll
+      for (int i = 0; i < LP_VECS; ++i) {
+        const long long at = v + i * NT + tid;
+        if (at < v1 && rv.inside(at)) copy_async16(to + i * NT, scores + rv.column(at));
+        else to[i * NT] = rv.load(at, v1).q;
+      }
+    }
+    copy_async_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < kStages - 1; ++k) fetch(v0 + (long long)k * kChunk, k);
 
   // the first CTA answers for the row: its given columns' scores are fetched now
   A given = 0;
@@ -240,137 +336,138 @@ __global__ void __launch_bounds__(32 * NW) log_probs_kernel(LogProbsProblem p, i
     if (given_j >= 0 && given_j < p.cols) given = widen(scores[given_j]);
   }
   if (kTop) {
-    if (tid == 0) st.count = st.kept_count = 0;
-    if (tid < NW) st.bound[tid] = -inf;
+    if (tid == 0) sh.kept_count = 0;
+    if (tid < NW) { sh.bound[tid] = -inf; sh.count[tid] = 0; }
     __syncthreads();
   }
 
   Sums<A, B> a{-inf, 0, 0};
-  A bound = -inf;
-  int listed = 0;                                           // candidates before this chunk
-  const int each = (p.top + NW - 1) / NW;                   // scores that every warp vouches for
-  Vec<T> q[LP_VECS];
-#pragma unroll
-  for (int i = 0; i < LP_VECS; ++i) q[i] = rv.load(v0 + i * NT + tid, v1);
-  int chunk = 0;
-  for (long long v = v0; v < v1; v += NT * LP_VECS, ++chunk) {
-    Vec<T> next[LP_VECS];
-    if (v + NT * LP_VECS < v1) {
-#pragma unroll
-      for (int i = 0; i < LP_VECS; ++i) next[i] = rv.load(v + (i + LP_VECS) * NT + tid, v1);
+  // warps with scores to vouch for (all but those past the row's end), and how many each of them vouches for
+  const int vouching = (int)max(1LL, min((long long)NW, (v1 - v0) / 32)), each = (p.top + vouching - 1) / vouching;
+  A bound = -inf, own = -inf;                               // shared bound; the K-th of this warp's list once it was cut
+  int listed = 0;                                           // the warp's candidates before this chunk
+  auto refresh = [&]() {
+    auto key = order(a.m);
+    decltype(key) found = 0;
+    for (int r = 0; r < each; ++r) {                        // the warp's each-th largest running maximum
+      found = warp_max_key(key);
+      const unsigned holds = __ballot_sync(kAll, key == found);
+      if (lane == __ffs(holds) - 1) key = 0;
     }
+    if (lane == 0) sh.bound[w] = each <= 32 ? value(found) : -inf;
+  };
+  auto shared_bound = [&]() {
+    A low = sh.bound[0];
+    for (int k = 1; k < vouching; ++k) low = fmin(low, sh.bound[k]);
+    bound = fmax(bound, low);
+  };
+  int chunk = 0, stage = 0;
+  for (long long v = v0; v < v1; v += kChunk, ++chunk) {
+    fetch(v + (long long)(kStages - 1) * kChunk, stage == 0 ? kStages - 1 : stage - 1);
+    copy_async_wait<kStages - 1>();
+    const uint4* from = mine + stage * LP_VECS * NT;
+    Vec<T> q[LP_VECS];
+#pragma unroll
+    for (int i = 0; i < LP_VECS; ++i) q[i].q = from[i * NT];
     A peak = q[0].peak();
 #pragma unroll
     for (int i = 1; i < LP_VECS; ++i) peak = max_nan(peak, q[i].peak());
     if (!(peak <= a.m)) a.raise(max_nan(peak, a.m), c);
-#pragma unroll
-    for (int i = 0; i < LP_VECS; ++i)
-#pragma unroll
-      for (int e = 0; e < kN; ++e) {
-        const A d = down(q[i].get(e), a.m, c), x = B::exp(d);
-        a.s += x;
-        a.t += x * d;
-      }
+    A s, t;
+    chunk_sums<T, A, B>(q, c, shift(a.m, c), s, t);
+    a.s += s;
+    a.t += t;
     if (kTop) {
-      const bool refresh = (chunk & (chunk - 1)) == 0;
-      if (refresh) {
-        auto key = order(a.m);
-        decltype(key) found = 0;
-        for (int r = 0; r < each; ++r) {                    // the warp's each-th largest running maximum
-          found = warp_max_key(key);
-          const unsigned holds = __ballot_sync(kAll, key == found);
-          if (lane == __ffs(holds) - 1) key = 0;
-        }
-        if (lane == 0) st.bound[w] = value(found);
-        __syncthreads();
-        A low = st.bound[0];
-#pragma unroll
-        for (int k = 1; k < NW; ++k) low = fmin(low, st.bound[k]);
-        bound = fmax(bound, low);
+      if ((chunk & (chunk - 1)) == 0) {
+        refresh();
+        if (chunk == 0) __syncthreads();                    // later bounds may be a refresh behind: still bounds
+        else __syncwarp();
+        shared_bound();
       }
-      // in a chunk that the bound knows of, scores equal to it may be among the K best; in a later one they may not
-      if (refresh ? peak >= bound : peak > bound) {
-#pragma unroll
-        for (int i = 0; i < LP_VECS; ++i)
-#pragma unroll
-          for (int e = 0; e < kN; ++e) {
-            const A x = q[i].get(e);
-            if ((refresh ? x >= bound : x > bound) && x > -inf) {
-              const int at = atomicAdd(&st.count, 1);
-              if (at < LP_LIST) st.list[at] = {x, (int)(rv.column(v + i * NT + tid) + e)};
-            }
-          }
+      if (__any_sync(kAll, peak >= bound && peak > own)) {
+        const Collected<A> r = collect<T, A>(from, NT, rv.column(v + tid), NT * kN, sh.list[w], &sh.count[w], listed,
+                                             bound, own, p.top);
+        listed = r.n;
+        own = r.own;
       }
-      __syncthreads();
-      int n = st.count;
-      if (n > LP_LIST) {
-        bound = fmax(bound, cut_to_best<T, A, NW>(st, q, rv.column(v + tid), listed, p.top));
-        n = st.count;
-      }
-      __syncthreads();                                      // the count is read before the next chunk raises it
-      listed = n;
     }
-#pragma unroll
-    for (int i = 0; i < LP_VECS; ++i) q[i] = next[i];
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
 
   // the CTA's sums: a common maximum per warp, then over the warps
   {
+    if (kTop) refresh();
     const A m = warp_max(a.m);
     a.raise(m, c);
     a.s = warp_sum(a.s);
     a.t = warp_sum(a.t);
     if (lane == 0) { sh.m[w] = a.m; sh.s[w] = a.s; sh.t[w] = a.t; }
   }
+  __syncthreads();                                          // (and the ring is free)
+  Candidate<A>* best = sh.list[0];                          // in the lists' place once they are ranked
+  int n_best = 0;
   if (kTop) {
-    // candidates still above the last bound
-    for (int e = tid; e < listed; e += NT) {
-      const Candidate<A> cand = st.list[e];
-      if (cand.x >= bound) st.kept[atomicAdd(&st.kept_count, 1)] = cand;
+    // candidates that reach the last bounds
+    shared_bound();
+    for (int e = lane; e < listed; e += 32) {
+      const Candidate<A> cand = sh.list[w][e];
+      if (cand.x >= bound) sh.kept()[atomicAdd(&sh.kept_count, 1)] = cand;
     }
+    __syncthreads();
+    n_best = min(sh.kept_count, p.top);
+    rank_into(sh.kept(), sh.kept_count, p.top, NT, best);
+    __syncthreads();
   }
-  __syncthreads();
   a = {sh.m[0], sh.s[0], sh.t[0]};
 #pragma unroll
   for (int k = 1; k < NW; ++k) a.add({sh.m[k], sh.s[k], sh.t[k]}, c);
 
-  Candidate<A>* best = nullptr;
-  int n_best = 0;
-  if (kTop) {
-    n_best = min(st.kept_count, p.top);
-    rank_into(st.kept, st.kept_count, p.top, NT, st.list);
-    best = st.list;
-    __syncthreads();
-  }
   if (parts > 1) {
     // the cluster's CTAs bring their sums and best columns into the first one's shared memory
     cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();                                         // every CTA runs; the first one's list is ranked
-    LogProbsSmem<A, NW>* sh0 = cluster.map_shared_rank(&sh, 0);
+    cluster.sync();                                         // every CTA runs; the first one's lists are ranked
+    Smem* sh0 = cluster.map_shared_rank(&sh, 0);
     if (tid == 0) sh0->part[part] = a;
-    if (kTop) {
-      TopSmem<A, NW>* st0 = cluster.map_shared_rank(&st, 0);
-      for (int e = tid; e < p.top; e += NT)
-        st0->kept[part * p.top + e] = e < n_best ? best[e] : Candidate<A>{-inf, 0x7fffffff - (part * p.top + e)};
-    }
+    if (kTop)
+      for (int e = tid; e < p.top; e += NT) {
+        const int at = part * p.top + e;                    // empty slots: -inf, columns of their own
+        sh0->kept()[at] = e < n_best ? best[e] : Candidate<A>{-inf, 0x7fffffff - at};
+      }
     cluster.sync();
     if (part != 0) return;
     for (int k = 1; k < parts; ++k) a.add(sh.part[k], c);
     if (kTop) {
-      // empty slots (-inf, columns of their own) rank behind every candidate, each in a place of its own
-      rank_into(st.kept, parts * p.top, p.top, NT, st.list);
+      rank_into(sh.kept(), parts * p.top, p.top, NT, best);
       __syncthreads();
       n_best = p.top;
     }
   }
 
   const bool empty = a.m == -inf, bad = !(a.m < inf);
-  const A inv_t = (A)(1.0 / p.temperature), log_s = bad ? (A)NAN : empty ? -inf : B::log(a.s) * B::unit();
+  A past = fma(a.m, c, -shift(a.m, c));                       // m c - M: s is relative to M, log_s below to m c
+  if (!empty && !bad && !(fabs(shift(a.m, c)) <= (A)kWide)) {
+    // M is not an ordinary number: s and t once more, by the differences x - m
+    past = 0;
+    A s = 0, t = 0;
+    for (int j = tid; j < p.cols; j += NT) {
+      const A d = floored((widen(scores[j]) - a.m) * c), x = B::exp(d);
+      s += x;
+      t += x * d;
+    }
+    s = warp_sum(s);
+    t = warp_sum(t);
+    __syncthreads();
+    if (lane == 0) { sh.s[w] = s; sh.t[w] = t; }
+    __syncthreads();
+    a.s = a.t = 0;
+    for (int k = 0; k < NW; ++k) { a.s += sh.s[k]; a.t += sh.t[k]; }
+  }
+  const A inv_t = (A)(1.0 / p.temperature), log_s = bad ? (A)NAN : empty ? -inf : (B::log(a.s) - past) * B::unit();
   // in nats from the start: a lowest-value score may be finite here and not in base 2
   auto log_p = [&](A x) { return empty ? -inf : (x - a.m) * inv_t - log_s; };
   if (tid == 0) {
     static_cast<A*>(p.lse)[row] = empty ? -inf : a.m * inv_t + log_s;
-    static_cast<A*>(p.entropy)[row] = empty ? (A)0 : log_s - a.t / a.s * B::unit();
+    static_cast<A*>(p.entropy)[row] = empty ? (A)0 : (B::log(a.s) - a.t / a.s) * B::unit();
     if (p.row_max) {
       static_cast<A*>(p.row_max)[row] = a.m;
       static_cast<A*>(p.log_sum)[row] = log_s;
@@ -447,12 +544,19 @@ template <typename T, int NW>
 int row_parts(const LogProbsProblem& p) {
   const long long chunk = 32LL * NW * LP_VECS * Vec<T>::kN;
   int parts = 1;
-  while (parts < 8 && p.rows * parts < 148 * 2 && (long long)p.cols > chunk * parts) parts *= 2;
+  if (NW == 8)
+    while (parts < 8 && p.rows * parts < 148 * 2 && (long long)p.cols > chunk * parts) parts *= 2;
   return parts;
 }
 
 template <typename T, int NW, bool kTop>
 cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
+  using Smem = LogProbsSmem<typename Acc<T>::type, NW, kTop>;
+  if (sizeof(Smem) > 48 * 1024) {
+    static std::atomic<int> done[kMaxDevices];
+    const cudaError_t e = smem_attr_once(reinterpret_cast<const void*>(log_probs_kernel<T, NW, kTop>), sizeof(Smem), done);
+    if (e != cudaSuccess) return e;
+  }
   const int parts = row_parts<T, NW>(p);
   const long long per = (1 << 30) / parts;                  // rows per launch: a grid's x stays below 2^31
   for (long long r = 0; r < p.rows; r += per) {
@@ -472,6 +576,7 @@ cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(q.rows * parts));
     cfg.blockDim = dim3(32 * NW);
+    cfg.dynamicSmemBytes = sizeof(Smem);
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -486,6 +591,10 @@ cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
+  // as many warps as the row has chunks for, up to 8
+  const long long warp_cols = 32LL * LP_VECS * Vec<T>::kN;
+  if (p.cols <= warp_cols) return p.top > 0 ? launch<T, 1, true>(p, stream) : launch<T, 1, false>(p, stream);
+  if (p.cols <= 3 * warp_cols) return p.top > 0 ? launch<T, 2, true>(p, stream) : launch<T, 2, false>(p, stream);
   return p.top > 0 ? launch<T, 8, true>(p, stream) : launch<T, 8, false>(p, stream);
 }
 

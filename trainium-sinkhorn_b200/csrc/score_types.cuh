@@ -21,6 +21,37 @@ __device__ __forceinline__ void narrow(float v, __half* p) { *p = __float2half_r
 __device__ __forceinline__ void narrow(float v, __nv_bfloat16* p) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void narrow(double v, double* p) { *p = v; }
 
+// Asynchronous 16-byte copies into shared memory, waited for by the thread that made them.
+__device__ __forceinline__ void copy_async16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+               : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>                       // until at most kLeft of the thread's groups are outstanding
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+
+// Two float32 operations in one instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // max that keeps a NaN
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -118,14 +149,23 @@ struct RowVectors {
   __device__ __forceinline__ bool inside(long long v) const {
     return column(v) >= 0 && column(v) + Vec<T>::kN <= cols;
   }
+  // whether the vectors [v, v + n) all lie wholly inside the row
+  __device__ __forceinline__ bool inside(long long v, int n) const {
+    return column(v) >= 0 && column(v + n) <= cols;
+  }
+  static __device__ __forceinline__ Vec<T> read(const T* at) {
+    Vec<T> r;
+    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+        : "=r"(r.q.x), "=r"(r.q.y), "=r"(r.q.z), "=r"(r.q.w)
+        : "l"(at));
+    return r;
+  }
   __device__ __forceinline__ Vec<T> load(long long v, long long end) const {
     constexpr int kN = Vec<T>::kN;
     Vec<T> r;
     const long long j = column(v);
     if (v < end && inside(v)) {
-      asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-          : "=r"(r.q.x), "=r"(r.q.y), "=r"(r.q.z), "=r"(r.q.w)
-          : "l"(row + j));
+      r = read(row + j);
     } else {
 #pragma unroll
       for (int i = 0; i < kN; ++i)
