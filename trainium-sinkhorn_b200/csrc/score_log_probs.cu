@@ -16,9 +16,11 @@
 // differences x - m.
 // The best columns come out of the same pass: a bound below the K-th largest score is kept from the threads' running
 // maxima (the K / warps-th largest of each warp's 32: at least K scores reach the smallest of these), raised after 1, 2,
-// 4, 8, ... chunks, and each warp collects the few scores that reach it in a list of its own. The lists are ranked at
-// the end. Where ties or ascending scores overflow a list, the warp cuts the list and the chunk it holds to their K best
-// by bisection. Nothing but the first bound makes warps wait for one another.
+// 4, 8, ... chunks, and each warp lists the few 16-byte vectors whose largest score reaches it. The K best scores lie in
+// the K best vectors by (largest score, position): each of these holds a better score than any other vector does. So
+// where ties or ascending scores overflow a list, the warp cuts it to its K best vectors by bisection, and at the end
+// the vectors that still reach the bound are read again (from L2), and their scores ranked. Nothing but the first bound
+// makes warps wait for one another.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -36,7 +38,8 @@ namespace {
 
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int LP_VECS = 4;          // 16-byte vectors a thread holds of a chunk
-constexpr int LP_LIST = 96;         // candidates for the best columns that a warp holds (more than 64)
+constexpr int LP_TOP = 64;          // most best columns
+constexpr int LP_LIST = 96;         // vectors with candidates for them that a warp lists (more than LP_TOP)
 constexpr float kWide = 1e30f;      // shifts M beyond this are not used
 
 // exp and log in the units of the sums: base 2 for float32, base e for float64. unit() turns such a logarithm into nats.
@@ -128,111 +131,85 @@ struct Candidate {
 template <typename A>
 __device__ __forceinline__ bool better(A x, int j, A ox, int oj) { return x > ox || (x == ox && j < oj); }
 
-// Shared memory of a CTA of NW warps. The ring holds kStages chunks; after the scores it serves as `kept`, the
-// candidates brought together (NW lists, or 64 best columns of each of a cluster's 8 CTAs).
-template <typename A, int NW, bool kTop>
+// Shared memory of a CTA of NW warps. The ring holds kStages chunks; after the scores it serves as `kept`: the listed
+// vectors, then the scores of the K best vectors, or the best columns of each of a cluster's 8 CTAs. Where there are
+// more than kRanked vectors, they are ranked and cut to K first.
+template <typename T, int NW, bool kTop>
 struct LogProbsSmem {
-  static constexpr int kStages = NW == 8 ? 3 : 2;
-  uint4 ring[kStages * LP_VECS * 32 * NW];
-  Candidate<A> list[kTop ? NW : 1][kTop ? LP_LIST : 1];
+  using A = typename Acc<T>::type;
+  static constexpr int kStages = NW == 8 ? 3 : 2, kRing = kStages * LP_VECS * 32 * NW * 16;
+  static constexpr int kRanked = 128, kScores = kRanked * Vec<T>::kN;
+  static constexpr int kBest = NW == 8 ? 8 * LP_TOP : LP_TOP;
+  static constexpr int kKept = (kScores > kBest ? kScores : kBest) * (int)sizeof(Candidate<A>);
+  union {
+    uint4 ring[kRing / 16];
+    unsigned char kept_bytes[kTop ? (kRing > kKept ? kRing : kKept) : 16];
+  };
+  Candidate<A> list[kTop ? NW * LP_LIST : 1];
+  Candidate<A> best[kTop ? (NW * LP_LIST > kRanked ? NW * LP_LIST : kRanked) : 1];
   volatile A bound[NW];
-  int count[NW], kept_count;
+  int count[NW], kept_count, best_count;
   A m[NW], s[NW], t[NW];
-  Sums<A, typename std::conditional<sizeof(A) == 8, BaseE, Base2>::type> part[8];   // of a cluster's CTAs (the first's)
-  __device__ __forceinline__ Candidate<A>* kept() { return reinterpret_cast<Candidate<A>*>(ring); }
+  Sums<A, typename Base<T>::type> part[8];                   // of a cluster's CTAs (in the first one's)
+  __device__ __forceinline__ Candidate<A>* kept() { return reinterpret_cast<Candidate<A>*>(kept_bytes); }
 };
 
 template <typename A>
-struct Collected {
-  int n;       // the warp's candidates
-  A own;       // at least this many reach it: the list's K-th value once the list was cut
+struct Cut {
+  int n;       // vectors left on the list
+  A own;       // at least this many vectors reach it
 };
 
-// Adds the scores of the warp's chunk that reach `bound` and exceed `own` to its list. A thread's vectors are
-// mine[i * stride] and hold the columns from col0 + i * step on. If the list overflows, it is cut to the K best of its
-// first n candidates and the chunk: bisection on the K-th value, then on the column up to which columns of just that
-// value are taken.
+// A warp's overflowing list, cut: the `top` best of its first n vectors and of the chunk (vectors mine[i * stride],
+// numbers first + i * stride) by (largest score, lower number). Bisection on the K-th value, then on the number up to
+// which vectors of just that value are taken.
 template <typename T, typename A>
-__device__ __noinline__ Collected<A> collect(const uint4* mine, int stride, long long col0, int step,
-                                             Candidate<A>* list, int* count, int n, A bound, A own, int top) {
-  constexpr int kN = Vec<T>::kN, kOwn = LP_LIST / 32;
+__device__ __noinline__ Cut<A> cut_list(const uint4* mine, int stride, int first, Candidate<A>* list, int* count,
+                                        int n, A own, int top) {
+  constexpr int kOld = LP_LIST / 32, kAllOf = kOld + LP_VECS;
   using Key = decltype(order(A()));
   const int lane = threadIdx.x & 31;
-  for (int i = 0; i < LP_VECS; ++i) {
-    const Vec<T> q{mine[i * stride]};
-    const A peak = q.peak();
-    if (!(peak >= bound && peak > own)) continue;
+  Candidate<A> c[kAllOf];
+  Key key[kAllOf];
 #pragma unroll
-    for (int e = 0; e < kN; ++e) {
-      const A x = q.get(e);
-      if (x >= bound && x > own) {
-        const int at = atomicAdd(count, 1);
-        if (at < LP_LIST) list[at] = {x, (int)(col0 + (long long)i * step + e)};
-      }
-    }
+  for (int i = 0; i < kAllOf; ++i) {
+    const int e = lane + i * 32, v = i - kOld;
+    if (v < 0) c[i] = e < n ? list[e] : Candidate<A>{(A)-INFINITY, 0};
+    else c[i] = {Vec<T>{mine[v * stride]}.peak(), first + v * stride};
+    key[i] = c[i].x == c[i].x ? order(c[i].x) : 0;           // (a row with NaN has no best columns)
+  }
+  Key k = 0;                                               // the largest key that at least `top` vectors reach
+  for (int bit = 8 * (int)sizeof(Key) - 1; bit >= 0; --bit) {
+    const Key next = k | ((Key)1 << bit);
+    int reach = 0;
+#pragma unroll
+    for (int i = 0; i < kAllOf; ++i) reach += key[i] >= next;
+    if ((int)__reduce_add_sync(kAll, reach) >= top) k = next;
+  }
+  int more = 0;
+#pragma unroll
+  for (int i = 0; i < kAllOf; ++i) more += key[i] > k;
+  const int wanted = top - (int)__reduce_add_sync(kAll, more);
+  int low = 0, high = 0x7fffffff;
+  while (low < high) {                                     // the smallest number that gives `wanted` of them
+    const int mid = low + (high - low) / 2;
+    int reach = 0;
+#pragma unroll
+    for (int i = 0; i < kAllOf; ++i) reach += key[i] == k && c[i].j <= mid;
+    if ((int)__reduce_add_sync(kAll, reach) >= wanted) high = mid;
+    else low = mid + 1;
   }
   __syncwarp();
-  const int found = *(volatile int*)count;
-  if (found <= LP_LIST) return {found, own};
-
-  Candidate<A> old[kOwn];
-#pragma unroll
-  for (int i = 0; i < kOwn; ++i) {
-    const int e = lane + i * 32;
-    old[i].x = e < n ? list[e].x : (A)-INFINITY;
-    old[i].j = e < n ? list[e].j : 0;
-  }
-  auto each = [&](auto&& f) {
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) f(old[i].x, old[i].j);
-    for (int i = 0; i < LP_VECS; ++i) {
-      const Vec<T> q{mine[i * stride]};
-#pragma unroll
-      for (int e = 0; e < kN; ++e) f(q.get(e), (int)(col0 + (long long)i * step + e));
-    }
-  };
-  // bfloat16 scores differ in the upper 16 bits of their keys alone (the lower ones are 0, or 1 for negative scores)
-  constexpr int kLowBit = std::is_same<T, __nv_bfloat16>::value ? 16 : 0;
-  Key k = 0;                                               // the largest key that at least `top` scores reach
-  for (int bit = 8 * (int)sizeof(Key) - 1; bit >= kLowBit; --bit) {
-    const Key next = k | ((Key)1 << bit);
-    const A at = value(next);
-    int c = 0;
-    if (at > (A)-INFINITY) {
-      each([&](A x, int) { c += x >= at; });
-    } else {                                               // -inf and below it, or past every score (keys of NaN)
-      c = next <= order((A)-INFINITY) ? LP_LIST : 0;
-    }
-    if ((int)__reduce_add_sync(kAll, c) >= top) k = next;
-  }
-  if (kLowBit > 0 && !(k >> (8 * sizeof(Key) - 1))) k |= ((Key)1 << kLowBit) - 1;
-  const A kth = value(k);
-  const bool all = !(kth > (A)-INFINITY);                  // fewer open columns than `top`: take them all
-  int last = -1;                                           // columns of the K-th value are taken up to this one
-  if (!all) {
-    int more = 0;
-    each([&](A x, int) { more += x > kth; });
-    const int wanted = top - (int)__reduce_add_sync(kAll, more);
-    int low = 0, high = 0x7fffffff;
-    while (low < high) {                                   // the smallest column that gives `wanted` of them
-      const int mid = low + (high - low) / 2;
-      int c = 0;
-      each([&](A x, int j) { c += x == kth && j <= mid; });
-      if ((int)__reduce_add_sync(kAll, c) >= wanted) high = mid;
-      else low = mid + 1;
-    }
-    last = low;
-  }
   if (lane == 0) *count = 0;
   __syncwarp();
-  each([&](A x, int j) {
-    if (all ? x > (A)-INFINITY : (x > kth || (x == kth && j <= last))) {
+#pragma unroll
+  for (int i = 0; i < kAllOf; ++i)
+    if (c[i].x > (A)-INFINITY && (key[i] > k || (key[i] == k && c[i].j <= low))) {
       const int at = atomicAdd(count, 1);
-      if (at < LP_LIST) list[at] = {x, j};
+      if (at < LP_LIST) list[at] = c[i];
     }
-  });
   __syncwarp();
-  return {min(*(volatile int*)count, LP_LIST), all ? own : fmax(own, kth)};
+  return {min(*(volatile int*)count, LP_LIST), fmax(own, value(k))};
 }
 
 // The candidates of `in` ranked by (score, lower column): the `top` best into out (in order), the others dropped.
@@ -296,7 +273,7 @@ template <typename T, int NW, bool kTop>
 __global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsProblem p, int parts) {
   using A = typename Acc<T>::type;
   using B = typename Base<T>::type;
-  using Smem = LogProbsSmem<A, NW, kTop>;
+  using Smem = LogProbsSmem<T, NW, kTop>;
   constexpr int NT = 32 * NW, kN = Vec<T>::kN, kChunk = NT * LP_VECS, kStages = Smem::kStages;
   extern __shared__ __align__(16) unsigned char smem_bytes[];
   Smem& sh = *reinterpret_cast<Smem*>(smem_bytes);
@@ -336,7 +313,7 @@ __global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsPro
     if (given_j >= 0 && given_j < p.cols) given = widen(scores[given_j]);
   }
   if (kTop) {
-    if (tid == 0) sh.kept_count = 0;
+    if (tid == 0) sh.kept_count = sh.best_count = 0;
     if (tid < NW) { sh.bound[tid] = -inf; sh.count[tid] = 0; }
     __syncthreads();
   }
@@ -345,7 +322,7 @@ __global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsPro
   // warps with scores to vouch for (all but those past the row's end), and how many each of them vouches for
   const int vouching = (int)max(1LL, min((long long)NW, (v1 - v0) / 32)), each = (p.top + vouching - 1) / vouching;
   A bound = -inf, own = -inf;                               // shared bound; the K-th of this warp's list once it was cut
-  int listed = 0;                                           // the warp's candidates before this chunk
+  int listed = 0;                                           // vectors on the warp's list before this chunk
   auto refresh = [&]() {
     auto key = order(a.m);
     decltype(key) found = 0;
@@ -385,10 +362,23 @@ __global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsPro
         shared_bound();
       }
       if (__any_sync(kAll, peak >= bound && peak > own)) {
-        const Collected<A> r = collect<T, A>(from, NT, rv.column(v + tid), NT * kN, sh.list[w], &sh.count[w], listed,
-                                             bound, own, p.top);
-        listed = r.n;
-        own = r.own;
+#pragma unroll
+        for (int i = 0; i < LP_VECS; ++i) {
+          const A x = q[i].peak();
+          if (x >= bound && x > own) {
+            const int at = atomicAdd(&sh.count[w], 1);
+            if (at < LP_LIST) sh.list[w * LP_LIST + at] = {x, (int)(v + i * NT + tid)};
+          }
+        }
+        __syncwarp();
+        const int n = *(volatile int*)&sh.count[w];
+        if (n > LP_LIST) {
+          const Cut<A> r = cut_list<T, A>(from, NT, (int)(v + tid), &sh.list[w * LP_LIST], &sh.count[w], listed, own, p.top);
+          listed = r.n;
+          own = r.own;
+        } else {
+          listed = n;
+        }
       }
     }
     stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -404,28 +394,43 @@ __global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsPro
     if (lane == 0) { sh.m[w] = a.m; sh.s[w] = a.s; sh.t[w] = a.t; }
   }
   __syncthreads();                                          // (and the ring is free)
-  Candidate<A>* best = sh.list[0];                          // in the lists' place once they are ranked
   int n_best = 0;
   if (kTop) {
-    // candidates that reach the last bounds
+    // vectors that reach the last bounds
     shared_bound();
     for (int e = lane; e < listed; e += 32) {
-      const Candidate<A> cand = sh.list[w][e];
-      if (cand.x >= bound) sh.kept()[atomicAdd(&sh.kept_count, 1)] = cand;
+      const Candidate<A> cand = sh.list[w * LP_LIST + e];
+      if (cand.x >= bound) sh.best[atomicAdd(&sh.best_count, 1)] = cand;
+    }
+    __syncthreads();
+    int n = sh.best_count;
+    const Candidate<A>* vectors = sh.best;
+    if (n > Smem::kRanked) {
+      rank_into(sh.best, n, p.top, NT, sh.list);
+      vectors = sh.list;
+      n = p.top;
+      __syncthreads();
+    }
+    // their scores, read again
+    for (int e = tid; e < n * kN; e += NT) {
+      const long long j = rv.column(vectors[e / kN].j) + e % kN;
+      if (j < 0 || j >= p.cols) continue;
+      const A x = widen(scores[j]);
+      if (x >= bound && x > -inf) sh.kept()[atomicAdd(&sh.kept_count, 1)] = {x, (int)j};
     }
     __syncthreads();
     n_best = min(sh.kept_count, p.top);
-    rank_into(sh.kept(), sh.kept_count, p.top, NT, best);
+    rank_into(sh.kept(), sh.kept_count, p.top, NT, sh.best);
     __syncthreads();
   }
   a = {sh.m[0], sh.s[0], sh.t[0]};
 #pragma unroll
   for (int k = 1; k < NW; ++k) a.add({sh.m[k], sh.s[k], sh.t[k]}, c);
-
+  const Candidate<A>* best = sh.best;
   if (parts > 1) {
     // the cluster's CTAs bring their sums and best columns into the first one's shared memory
     cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();                                         // every CTA runs; the first one's lists are ranked
+    cluster.sync();                                         // every CTA runs; the first one's `kept` is ranked
     Smem* sh0 = cluster.map_shared_rank(&sh, 0);
     if (tid == 0) sh0->part[part] = a;
     if (kTop)
@@ -437,7 +442,7 @@ __global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsPro
     if (part != 0) return;
     for (int k = 1; k < parts; ++k) a.add(sh.part[k], c);
     if (kTop) {
-      rank_into(sh.kept(), parts * p.top, p.top, NT, best);
+      rank_into(sh.kept(), parts * p.top, p.top, NT, sh.best);
       __syncthreads();
       n_best = p.top;
     }
@@ -551,7 +556,7 @@ int row_parts(const LogProbsProblem& p) {
 
 template <typename T, int NW, bool kTop>
 cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
-  using Smem = LogProbsSmem<typename Acc<T>::type, NW, kTop>;
+  using Smem = LogProbsSmem<T, NW, kTop>;
   if (sizeof(Smem) > 48 * 1024) {
     static std::atomic<int> done[kMaxDevices];
     const cudaError_t e = smem_attr_once(reinterpret_cast<const void*>(log_probs_kernel<T, NW, kTop>), sizeof(Smem), done);
