@@ -123,13 +123,51 @@ __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
   return k;
 }
 
+// The k-th largest (1 .. 32) of a warp's keys: by removal for the first ones, else by sorting the lanes.
+template <typename K>
+__device__ __forceinline__ K kth_key(K key, int k) {
+  const int lane = threadIdx.x & 31;
+  if (k <= 3) {
+    K found = warp_max_key(key);
+    for (int r = 1; r < k; ++r) {
+      const unsigned holds = __ballot_sync(kAll, key == found);
+      if (lane == __ffs(holds) - 1) key = 0;
+      found = warp_max_key(key);
+    }
+    return found;
+  }
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int o = size / 2; o > 0; o /= 2) {
+      const K x = __shfl_xor_sync(kAll, key, o);
+      const bool larger = ((lane & o) == 0) == ((lane & size) == 0);      // this lane keeps the larger key
+      key = (x > key) == larger ? x : key;
+    }
+  return __shfl_sync(kAll, key, (k - 1) & 31);
+}
+
+// A score (or a vector's largest score) and its column (or the vector's number). Of two, the larger score comes first,
+// of equal ones the lower number; float32 candidates carry both in one whole number.
 template <typename A>
 struct Candidate {
-  A x;
+  double x;
   int j;
+  Candidate() = default;
+  __device__ __forceinline__ Candidate(double x_, int j_) : x(x_), j(j_) {}
+  __device__ __forceinline__ double score() const { return x; }
+  __device__ __forceinline__ int number() const { return j; }
+  __device__ __forceinline__ bool before(const Candidate& o) const { return x > o.x || (x == o.x && j < o.j); }
 };
-template <typename A>
-__device__ __forceinline__ bool better(A x, int j, A ox, int oj) { return x > ox || (x == ox && j < oj); }
+template <>
+struct Candidate<float> {
+  uint64_t k;
+  Candidate() = default;
+  __device__ __forceinline__ Candidate(float x, int j) : k((uint64_t)order(x) << 32 | (0x7fffffffu - (uint32_t)j)) {}
+  __device__ __forceinline__ float score() const { return value((uint32_t)(k >> 32)); }
+  __device__ __forceinline__ int number() const { return (int)(0x7fffffffu - (uint32_t)k); }
+  __device__ __forceinline__ bool before(const Candidate& o) const { return k > o.k; }
+};
 
 // Shared memory of a CTA of NW warps. The ring holds kStages chunks; after the scores it serves as `kept`: the listed
 // vectors, then the scores of the K best vectors, or the best columns of each of a cluster's 8 CTAs. Where there are
@@ -138,7 +176,7 @@ template <typename T, int NW, bool kTop>
 struct LogProbsSmem {
   using A = typename Acc<T>::type;
   static constexpr int kStages = NW == 8 ? 3 : 2, kRing = kStages * LP_VECS * 32 * NW * 16;
-  static constexpr int kRanked = 128, kScores = kRanked * Vec<T>::kN;
+  static constexpr int kRanked = 64, kScores = kRanked * Vec<T>::kN;
   static constexpr int kBest = NW == 8 ? 8 * LP_TOP : LP_TOP;
   static constexpr int kKept = (kScores > kBest ? kScores : kBest) * (int)sizeof(Candidate<A>);
   union {
@@ -169,14 +207,15 @@ __device__ __noinline__ Cut<A> cut_list(const uint4* mine, int stride, int first
   constexpr int kOld = LP_LIST / 32, kAllOf = kOld + LP_VECS;
   using Key = decltype(order(A()));
   const int lane = threadIdx.x & 31;
-  Candidate<A> c[kAllOf];
+  A x[kAllOf];
+  int j[kAllOf];
   Key key[kAllOf];
 #pragma unroll
   for (int i = 0; i < kAllOf; ++i) {
     const int e = lane + i * 32, v = i - kOld;
-    if (v < 0) c[i] = e < n ? list[e] : Candidate<A>{(A)-INFINITY, 0};
-    else c[i] = {Vec<T>{mine[v * stride]}.peak(), first + v * stride};
-    key[i] = c[i].x == c[i].x ? order(c[i].x) : 0;           // (a row with NaN has no best columns)
+    x[i] = v >= 0 ? Vec<T>{mine[v * stride]}.peak() : e < n ? list[e].score() : (A)-INFINITY;
+    j[i] = v >= 0 ? first + v * stride : e < n ? list[e].number() : 0;
+    key[i] = x[i] == x[i] ? order(x[i]) : 0;                 // (a row with NaN has no best columns)
   }
   Key k = 0;                                               // the largest key that at least `top` vectors reach
   for (int bit = 8 * (int)sizeof(Key) - 1; bit >= 0; --bit) {
@@ -195,7 +234,7 @@ __device__ __noinline__ Cut<A> cut_list(const uint4* mine, int stride, int first
     const int mid = low + (high - low) / 2;
     int reach = 0;
 #pragma unroll
-    for (int i = 0; i < kAllOf; ++i) reach += key[i] == k && c[i].j <= mid;
+    for (int i = 0; i < kAllOf; ++i) reach += key[i] == k && j[i] <= mid;
     if ((int)__reduce_add_sync(kAll, reach) >= wanted) high = mid;
     else low = mid + 1;
   }
@@ -204,21 +243,22 @@ __device__ __noinline__ Cut<A> cut_list(const uint4* mine, int stride, int first
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < kAllOf; ++i)
-    if (c[i].x > (A)-INFINITY && (key[i] > k || (key[i] == k && c[i].j <= low))) {
+    if (x[i] > (A)-INFINITY && (key[i] > k || (key[i] == k && j[i] <= low))) {
       const int at = atomicAdd(count, 1);
-      if (at < LP_LIST) list[at] = c[i];
+      if (at < LP_LIST) list[at] = Candidate<A>(x[i], j[i]);
     }
   __syncwarp();
   return {min(*(volatile int*)count, LP_LIST), fmax(own, value(k))};
 }
 
-// The candidates of `in` ranked by (score, lower column): the `top` best into out (in order), the others dropped.
+// The candidates of `in` ranked: the `top` first into out (in order), the others dropped.
 template <typename A>
 __device__ __forceinline__ void rank_into(const Candidate<A>* in, int n, int top, int threads, Candidate<A>* out) {
   for (int e = threadIdx.x; e < n; e += threads) {
     const Candidate<A> c = in[e];
     int rank = 0;
-    for (int o = 0; o < n; ++o) rank += better(in[o].x, in[o].j, c.x, c.j);
+#pragma unroll 4
+    for (int o = 0; o < n; ++o) rank += in[o].before(c);
     if (rank < top) out[rank] = c;
   }
 }
@@ -270,7 +310,7 @@ __device__ __forceinline__ void chunk_sums(const Vec<T> (&q)[LP_VECS], A c, A M,
 }
 
 template <typename T, int NW, bool kTop>
-__global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsProblem p, int parts) {
+__global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_probs_kernel(LogProbsProblem p, int parts) {
   using A = typename Acc<T>::type;
   using B = typename Base<T>::type;
   using Smem = LogProbsSmem<T, NW, kTop>;
@@ -324,14 +364,8 @@ __global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsPro
   A bound = -inf, own = -inf;                               // shared bound; the K-th of this warp's list once it was cut
   int listed = 0;                                           // vectors on the warp's list before this chunk
   auto refresh = [&]() {
-    auto key = order(a.m);
-    decltype(key) found = 0;
-    for (int r = 0; r < each; ++r) {                        // the warp's each-th largest running maximum
-      found = warp_max_key(key);
-      const unsigned holds = __ballot_sync(kAll, key == found);
-      if (lane == __ffs(holds) - 1) key = 0;
-    }
-    if (lane == 0) sh.bound[w] = each <= 32 ? value(found) : -inf;
+    const auto key = kth_key(order(a.m), each);             // the warp's each-th largest running maximum
+    if (lane == 0) sh.bound[w] = each <= 32 ? value(key) : -inf;
   };
   auto shared_bound = [&]() {
     A low = sh.bound[0];
@@ -367,7 +401,7 @@ __global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsPro
           const A x = q[i].peak();
           if (x >= bound && x > own) {
             const int at = atomicAdd(&sh.count[w], 1);
-            if (at < LP_LIST) sh.list[w * LP_LIST + at] = {x, (int)(v + i * NT + tid)};
+            if (at < LP_LIST) sh.list[w * LP_LIST + at] = Candidate<A>(x, (int)(v + i * NT + tid));
           }
         }
         __syncwarp();
@@ -400,7 +434,7 @@ __global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsPro
     shared_bound();
     for (int e = lane; e < listed; e += 32) {
       const Candidate<A> cand = sh.list[w * LP_LIST + e];
-      if (cand.x >= bound) sh.best[atomicAdd(&sh.best_count, 1)] = cand;
+      if (cand.score() >= bound) sh.best[atomicAdd(&sh.best_count, 1)] = cand;
     }
     __syncthreads();
     int n = sh.best_count;
@@ -413,10 +447,10 @@ __global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsPro
     }
     // their scores, read again
     for (int e = tid; e < n * kN; e += NT) {
-      const long long j = rv.column(vectors[e / kN].j) + e % kN;
+      const long long j = rv.column(vectors[e / kN].number()) + e % kN;
       if (j < 0 || j >= p.cols) continue;
       const A x = widen(scores[j]);
-      if (x >= bound && x > -inf) sh.kept()[atomicAdd(&sh.kept_count, 1)] = {x, (int)j};
+      if (x >= bound && x > -inf) sh.kept()[atomicAdd(&sh.kept_count, 1)] = Candidate<A>(x, (int)j);
     }
     __syncthreads();
     n_best = min(sh.kept_count, p.top);
@@ -436,7 +470,7 @@ __global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsPro
     if (kTop)
       for (int e = tid; e < p.top; e += NT) {
         const int at = part * p.top + e;                    // empty slots: -inf, columns of their own
-        sh0->kept()[at] = e < n_best ? best[e] : Candidate<A>{-inf, 0x7fffffff - at};
+        sh0->kept()[at] = e < n_best ? best[e] : Candidate<A>(-inf, 0x7fffffff - at);
       }
     cluster.sync();
     if (part != 0) return;
@@ -488,9 +522,10 @@ __global__ void __launch_bounds__(32 * NW, 32 / NW) log_probs_kernel(LogProbsPro
   }
   if (kTop)
     for (int k = tid; k < p.top; k += NT) {
-      const bool open = !bad && k < n_best && best[k].x > -inf;
-      p.top_index[row * p.top + k] = open ? best[k].j : -1;
-      static_cast<A*>(p.top_log_prob)[row * p.top + k] = bad ? (A)NAN : open ? log_p(best[k].x) : -inf;
+      const A x = k < n_best ? best[k].score() : -inf;
+      const bool open = !bad && x > -inf;
+      p.top_index[row * p.top + k] = open ? best[k].number() : -1;
+      static_cast<A*>(p.top_log_prob)[row * p.top + k] = bad ? (A)NAN : open ? log_p(x) : -inf;
     }
 }
 
@@ -596,10 +631,16 @@ cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
-  // as many warps as the row has chunks for, up to 8
+  // The fewest warps per row that fill half of the SMs' 32 warp slots, and no more than the row has chunks for: what a
+  // row costs besides its scores (ranking, joining sums) grows with its warps. Measured at 8 / 4 / 2 / 1 warps, bfloat16,
+  // 5 best columns: 8192 x 32768 224 / 160 / 136 / 121 us, 8192 x 1000 139 / 66 / 35 / 21 us, 600 x 5000
+  // 16 / 12 / 10 / 12 us, 300 x 131072 33 / 37 / 52 / 70 us.
   const long long warp_cols = 32LL * LP_VECS * Vec<T>::kN;
-  if (p.cols <= warp_cols) return p.top > 0 ? launch<T, 1, true>(p, stream) : launch<T, 1, false>(p, stream);
-  if (p.cols <= 3 * warp_cols) return p.top > 0 ? launch<T, 2, true>(p, stream) : launch<T, 2, false>(p, stream);
+  int nw = 1;
+  while (nw < 8 && p.rows * nw < 148 * 16 && (long long)p.cols > nw * warp_cols) nw *= 2;
+  if (nw == 1) return p.top > 0 ? launch<T, 1, true>(p, stream) : launch<T, 1, false>(p, stream);
+  if (nw == 2) return p.top > 0 ? launch<T, 2, true>(p, stream) : launch<T, 2, false>(p, stream);
+  if (nw == 4) return p.top > 0 ? launch<T, 4, true>(p, stream) : launch<T, 4, false>(p, stream);
   return p.top > 0 ? launch<T, 8, true>(p, stream) : launch<T, 8, false>(p, stream);
 }
 
