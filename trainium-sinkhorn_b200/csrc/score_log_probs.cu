@@ -263,8 +263,9 @@ __device__ __forceinline__ void rank_into(const Candidate<A>* in, int n, int top
   }
 }
 
-// One chunk's sums relative to M: exp(d) and exp(d) d over the vectors, d = x c - M.
-template <typename T, typename A, typename B>
+// One chunk's sums relative to M: exp(d) and exp(d) d over the vectors, d = x c - M; kFloor for chunks with scores of
+// -inf, whose d would make t no number.
+template <typename T, typename A, typename B, bool kFloor>
 __device__ __forceinline__ void chunk_sums(const Vec<T> (&q)[LP_VECS], A c, A M, A& s, A& t) {
   constexpr int kN = Vec<T>::kN;
   if constexpr (sizeof(A) == 4) {
@@ -274,9 +275,14 @@ __device__ __forceinline__ void chunk_sums(const Vec<T> (&q)[LP_VECS], A c, A M,
     for (int i = 0; i < LP_VECS; ++i)
 #pragma unroll
       for (int e = 0; e < kN; e += 2) {
-        const uint64_t d2 = fma2(pack2(q[i].get(e), q[i].get(e + 1)), c2, m2);
+        uint64_t d2 = fma2(pack2(q[i].get(e), q[i].get(e + 1)), c2, m2);
         float d0, d1;
         unpack2(d2, d0, d1);
+        if (kFloor) {
+          d0 = floored(d0);
+          d1 = floored(d1);
+          d2 = pack2(d0, d1);
+        }
         const uint64_t x2 = pack2(B::exp(d0), B::exp(d1));
         s2 = add2(s2, x2);
         t2 = fma2(x2, d2, t2);
@@ -292,17 +298,9 @@ __device__ __forceinline__ void chunk_sums(const Vec<T> (&q)[LP_VECS], A c, A M,
     for (int i = 0; i < LP_VECS; ++i)
 #pragma unroll
       for (int e = 0; e < kN; ++e) {
-        const A d = fma(q[i].get(e), c, -M), x = B::exp(d);
-        s += x;
-        t = fma(x, d, t);
-      }
-  }
-  if (!(t == t)) {                                          // a score of -inf (0 * -inf) or NaN: the same with a floor
-    s = t = 0;
-    for (int i = 0; i < LP_VECS; ++i)
-#pragma unroll
-      for (int e = 0; e < kN; ++e) {
-        const A d = floored(fma(q[i].get(e), c, -M)), x = B::exp(d);
+        A d = fma(q[i].get(e), c, -M);
+        if (kFloor) d = floored(d);
+        const A x = B::exp(d);
         s += x;
         t = fma(x, d, t);
       }
@@ -372,6 +370,7 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_
     for (int k = 1; k < vouching; ++k) low = fmin(low, sh.bound[k]);
     bound = fmax(bound, low);
   };
+  bool closed = false;                                      // whether the warp has met scores of -inf (or NaN)
   int chunk = 0, stage = 0;
   for (long long v = v0; v < v1; v += kChunk, ++chunk) {
     fetch(v + (long long)(kStages - 1) * kChunk, stage == 0 ? kStages - 1 : stage - 1);
@@ -385,7 +384,11 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_
     for (int i = 1; i < LP_VECS; ++i) peak = max_nan(peak, q[i].peak());
     if (!(peak <= a.m)) a.raise(max_nan(peak, a.m), c);
     A s, t;
-    chunk_sums<T, A, B>(q, c, shift(a.m, c), s, t);
+    if (!closed) {
+      chunk_sums<T, A, B, false>(q, c, shift(a.m, c), s, t);
+      closed = __any_sync(kAll, !(t == t));                 // from here on the warp floors its differences
+    }
+    if (closed) chunk_sums<T, A, B, true>(q, c, shift(a.m, c), s, t);
     a.s += s;
     a.t += t;
     if (kTop) {
@@ -529,55 +532,92 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_
     }
 }
 
-constexpr int LP_THREADS = 256;
-
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) log_probs_grad_kernel(LogProbsGradProblem p) {
+// Gradient: a CTA takes NT x LP_VECS vectors of one row, placed on the gradient's 16-byte boundaries. With the row's m and
+// log s a score needs no sum: p (A + B log p), with A = -(g + g_H H) / T, B = -g_H / T and g the sum of the upstream
+// gradients of the row's given and best columns (less that of lse). Those columns are written once more, by the first
+// entry that names them, with the entries that repeat it added in order. Bound by the two matrices' bytes.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) log_probs_grad_kernel(LogProbsGradProblem p, int parts) {
   using A = typename Acc<T>::type;
+  using B = typename Base<T>::type;
+  constexpr int kN = Vec<T>::kN;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const long long row = blockIdx.x / parts, v0 = (long long)(blockIdx.x % parts) * NT * LP_VECS;
+  const T* s = static_cast<const T*>(p.scores) + row * p.ld;
+  T* out = static_cast<T*>(p.grad) + row * p.ld_grad;
+  const RowVectors<T> rv(out, p.cols);
+  const long long first = rv.column(v0), end = rv.column(v0 + NT * LP_VECS);    // the CTA's columns
+  const bool vectors = (reinterpret_cast<uintptr_t>(s + first) & 15) == 0;     // the scores' vectors fall together
+  Vec<T> q[LP_VECS];
+#pragma unroll
+  for (int i = 0; i < LP_VECS; ++i) {
+    const long long v = v0 + i * NT + tid, j = rv.column(v);
+    if (vectors && rv.inside(v)) {
+      q[i] = RowVectors<T>::read(s + j);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) q[i].set(e, j + e >= 0 && j + e < p.cols ? s[j + e] : lowest_inf<T>());
+    }
+  }
+
   const A inv_t = (A)(1.0 / p.temperature), inf = (A)INFINITY;
   const int extra = p.n_targets + p.top;
-  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const T* s = static_cast<const T*>(p.scores) + row * p.ld;
-    T* out = static_cast<T*>(p.grad) + row * p.ld_grad;
-    const long long* tg = p.targets + row * p.n_targets;
-    const long long* ti = p.top_index + row * p.top;
-    const A* gt = p.d_log_prob ? static_cast<const A*>(p.d_log_prob) + row * p.n_targets : nullptr;
-    const A* gk = p.d_top ? static_cast<const A*>(p.d_top) + row * p.top : nullptr;
-    // entry q < n_targets is a given column, the others are the best columns
-    auto column = [&](int q) { return q < p.n_targets ? tg[q] : ti[q - p.n_targets]; };
-    auto upstream = [&](int q) { return q < p.n_targets ? (gt ? gt[q] : (A)0) : (gk ? gk[q - p.n_targets] : (A)0); };
-    const A m = static_cast<const A*>(p.row_max)[row], log_sum = static_cast<const A*>(p.log_sum)[row];
-    const bool empty = m == -inf;
-    const A h = static_cast<const A*>(p.entropy)[row];
-    const A gh = p.d_entropy ? static_cast<const A*>(p.d_entropy)[row] : (A)0;
-    A total = p.d_lse ? -static_cast<const A*>(p.d_lse)[row] : (A)0;
-    for (int q = 0; q < extra; ++q) {
-      const long long j = column(q);
-      if (j >= 0 && j < p.cols) total += upstream(q);
+  // entry k < n_targets is a given column, the others are the best columns
+  const long long* tg = p.targets + row * p.n_targets;
+  const long long* ti = p.top_index + row * p.top;
+  const A* gt = p.d_log_prob ? static_cast<const A*>(p.d_log_prob) + row * p.n_targets : nullptr;
+  const A* gk = p.d_top ? static_cast<const A*>(p.d_top) + row * p.top : nullptr;
+  auto column = [&](int k) { return k < p.n_targets ? tg[k] : ti[k - p.n_targets]; };
+  auto upstream = [&](int k) { return k < p.n_targets ? (gt ? gt[k] : (A)0) : (gk ? gk[k - p.n_targets] : (A)0); };
+  const A m = static_cast<const A*>(p.row_max)[row], log_s = static_cast<const A*>(p.log_sum)[row];
+  const A h = static_cast<const A*>(p.entropy)[row];
+  const A gh = p.d_entropy ? static_cast<const A*>(p.d_entropy)[row] : (A)0;
+  A total = 0;
+  for (int k = lane; k < extra; k += 32) {
+    const long long j = column(k);
+    const A g = upstream(k);
+    if (j >= 0 && j < p.cols) total += g;
+  }
+  total = warp_sum(total);
+  if (p.d_lse) total -= static_cast<const A*>(p.d_lse)[row];
+  const bool empty = m == -inf;
+  const A c = B::scale(p.temperature), ls = log_s / B::unit(), fa = -inv_t * (total + gh * h), fb = -inv_t * gh * B::unit();
+  auto dense = [&](A x) {
+    const A lp = floored(fma(x - m, c, -ls));
+    return empty ? (A)0 : B::exp(lp) * fma(fb, lp, fa);
+  };
+#pragma unroll
+  for (int i = 0; i < LP_VECS; ++i) {
+    const long long v = v0 + i * NT + tid, j = rv.column(v);
+    Vec<T> r;
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      T x;
+      narrow(dense(q[i].get(e)), &x);
+      r.set(e, x);
     }
-    auto dense = [&](A x) {
-      if (empty || x == -inf) return (A)0;
-      const A lp = (x - m) * inv_t - log_sum;
-      return -exp(lp) * (total + gh * (lp + h)) * inv_t;
-    };
-    for (int j = threadIdx.x; j < p.cols; j += LP_THREADS) narrow(dense(widen(s[j])), out + j);
-    __syncthreads();
-    for (int q = threadIdx.x; q < extra; q += LP_THREADS) {
-      const long long j = column(q);
-      if (j < 0 || j >= p.cols || empty) continue;
-      bool first = true;                       // a column given more than once is written by its first entry
-      for (int r = 0; r < q; ++r) first = first && column(r) != j;
-      if (!first) continue;
-      A g = upstream(q);
-      for (int r = q + 1; r < extra; ++r)
-        if (column(r) == j) g += upstream(r);
-      narrow(dense(widen(s[j])) + g * inv_t, out + j);
+    if (rv.inside(v)) {
+      *reinterpret_cast<uint4*>(out + j) = r.q;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kN; ++e)
+        if (j + e >= 0 && j + e < p.cols) narrow(dense(q[i].get(e)), out + j + e);
     }
-    __syncthreads();
+  }
+  if (extra == 0 || empty) return;
+  __syncthreads();                                         // the named columns follow the CTA's others
+  for (int k = tid; k < extra; k += NT) {
+    const long long j = column(k);
+    if (j < 0 || j >= p.cols || j < first || j >= end) continue;
+    bool again = false;
+    for (int r = 0; r < k; ++r) again = again || column(r) == j;
+    if (again) continue;
+    A g = upstream(k);
+    for (int r = k + 1; r < extra; ++r)
+      if (column(r) == j) g += upstream(r);
+    narrow(fma(g, inv_t, dense(widen(s[j]))), out + j);
   }
 }
-
-unsigned row_grid(long long rows) { return (unsigned)(rows < 65535 ? rows : 65535); }
 
 // CTAs per row: a cluster where the rows alone leave SMs empty, as long as each CTA has a chunk of its own.
 template <typename T, int NW>
@@ -634,14 +674,46 @@ cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
   // The fewest warps per row that fill half of the SMs' 32 warp slots, and no more than the row has chunks for: what a
   // row costs besides its scores (ranking, joining sums) grows with its warps. Measured at 8 / 4 / 2 / 1 warps, bfloat16,
   // 5 best columns: 8192 x 32768 224 / 160 / 136 / 121 us, 8192 x 1000 139 / 66 / 35 / 21 us, 600 x 5000
-  // 16 / 12 / 10 / 12 us, 300 x 131072 33 / 37 / 52 / 70 us.
+  // 16 / 12 / 10 / 12 us, 300 x 131072 33 / 37 / 52 / 70 us. A warp vouches for 24 best columns at most (of its 32
+  // lanes' maxima the 32nd is a poor bound): 2048 x 32000 with 64 best columns, 130 us with 2 warps, 91 us with 8.
   const long long warp_cols = 32LL * LP_VECS * Vec<T>::kN;
   int nw = 1;
-  while (nw < 8 && p.rows * nw < 148 * 16 && (long long)p.cols > nw * warp_cols) nw *= 2;
+  while (nw < 8 && (p.rows * nw < 148 * 16 || p.top > 24 * nw) && (long long)p.cols > nw * warp_cols) nw *= 2;
   if (nw == 1) return p.top > 0 ? launch<T, 1, true>(p, stream) : launch<T, 1, false>(p, stream);
   if (nw == 2) return p.top > 0 ? launch<T, 2, true>(p, stream) : launch<T, 2, false>(p, stream);
   if (nw == 4) return p.top > 0 ? launch<T, 4, true>(p, stream) : launch<T, 4, false>(p, stream);
   return p.top > 0 ? launch<T, 8, true>(p, stream) : launch<T, 8, false>(p, stream);
+}
+
+template <typename T, int NT>
+cudaError_t grad_launch(const LogProbsGradProblem& p, cudaStream_t stream) {
+  constexpr long long kCols = (long long)NT * LP_VECS * Vec<T>::kN;
+  const int parts = (int)((p.cols + Vec<T>::kN - 1 + kCols - 1) / kCols);      // (a row may start inside a vector)
+  const long long per = (1LL << 30) / parts;
+  const size_t size = sizeof(typename Acc<T>::type);
+  for (long long r = 0; r < p.rows; r += per) {
+    auto at = [&](const void* base, long long n) { return base ? static_cast<const char*>(base) + n * size : nullptr; };
+    LogProbsGradProblem q = p;
+    q.rows = p.rows - r < per ? p.rows - r : per;
+    q.scores = static_cast<const T*>(p.scores) + r * p.ld;
+    q.grad = static_cast<T*>(p.grad) + r * p.ld_grad;
+    q.targets = p.targets ? p.targets + r * p.n_targets : nullptr;
+    q.top_index = p.top_index ? p.top_index + r * p.top : nullptr;
+    q.row_max = at(p.row_max, r);
+    q.log_sum = at(p.log_sum, r);
+    q.entropy = at(p.entropy, r);
+    q.d_log_prob = at(p.d_log_prob, r * p.n_targets);
+    q.d_entropy = at(p.d_entropy, r);
+    q.d_lse = at(p.d_lse, r);
+    q.d_top = at(p.d_top, r * p.top);
+    log_probs_grad_kernel<T, NT><<<(unsigned)(q.rows * parts), NT, 0, stream>>>(q, parts);
+  }
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t grad_launch(const LogProbsGradProblem& p, cudaStream_t stream) {
+  return p.cols <= 64 * LP_VECS * Vec<T>::kN ? grad_launch<T, 64>(p, stream) : grad_launch<T, 256>(p, stream);
 }
 
 }  // namespace
@@ -656,14 +728,12 @@ cudaError_t log_probs_launch(int type, const LogProbsProblem& p, cudaStream_t st
 }
 
 cudaError_t log_probs_grad_launch(int type, const LogProbsGradProblem& p, cudaStream_t stream) {
-  const unsigned grid = row_grid(p.rows);
   switch (type) {
-    case TRNOPT_F32: log_probs_grad_kernel<float><<<grid, LP_THREADS, 0, stream>>>(p); break;
-    case TRNOPT_F16: log_probs_grad_kernel<__half><<<grid, LP_THREADS, 0, stream>>>(p); break;
-    case TRNOPT_BF16: log_probs_grad_kernel<__nv_bfloat16><<<grid, LP_THREADS, 0, stream>>>(p); break;
-    default: log_probs_grad_kernel<double><<<grid, LP_THREADS, 0, stream>>>(p); break;
+    case TRNOPT_F32: return grad_launch<float>(p, stream);
+    case TRNOPT_F16: return grad_launch<__half>(p, stream);
+    case TRNOPT_BF16: return grad_launch<__nv_bfloat16>(p, stream);
+    default: return grad_launch<double>(p, stream);
   }
-  return cudaGetLastError();
 }
 
 }  // namespace trnopt
