@@ -47,13 +47,15 @@ struct Base2 {
   static __device__ __forceinline__ float exp(float x) { return ex2_approx(x); }
   static __device__ __forceinline__ float log(float x) { return log2f(x); }
   static __device__ __forceinline__ float unit() { return 0.6931471805599453f; }
-  static __device__ __forceinline__ float scale(double t) { return (float)(1.4426950408889634 / t); }
+  static __device__ __forceinline__ float per_unit() { return 1.4426950408889634f; }
+  static float scale(double t) { return (float)(1.4426950408889634 / t); }
 };
 struct BaseE {
   static __device__ __forceinline__ double exp(double x) { return ::exp(x); }
   static __device__ __forceinline__ double log(double x) { return ::log(x); }
   static __device__ __forceinline__ double unit() { return 1.0; }
-  static __device__ __forceinline__ double scale(double t) { return 1.0 / t; }
+  static __device__ __forceinline__ double per_unit() { return 1.0; }
+  static double scale(double t) { return 1.0 / t; }
 };
 template <typename T> struct Base { using type = Base2; };
 template <> struct Base<double> { using type = BaseE; };
@@ -308,7 +310,8 @@ __device__ __forceinline__ void chunk_sums(const Vec<T> (&q)[LP_VECS], A c, A M,
 }
 
 template <typename T, int NW, bool kTop>
-__global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_probs_kernel(LogProbsProblem p, int parts) {
+__global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_probs_kernel(LogProbsProblem p, int parts, typename Acc<T>::type c,
+                                                                                 typename Acc<T>::type inv_t) {
   using A = typename Acc<T>::type;
   using B = typename Base<T>::type;
   using Smem = LogProbsSmem<T, NW, kTop>;
@@ -316,12 +319,13 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_
   extern __shared__ __align__(16) unsigned char smem_bytes[];
   Smem& sh = *reinterpret_cast<Smem*>(smem_bytes);
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const long long row = blockIdx.x / parts;
-  const int part = (int)(blockIdx.x % parts);
+  const long long row = blockIdx.x / (unsigned)parts;
+  const int part = (int)(blockIdx.x - (unsigned)row * (unsigned)parts);
   const T* scores = static_cast<const T*>(p.scores) + row * p.ld;
   const RowVectors<T> rv(scores, p.cols);
-  const long long per = (rv.count + parts - 1) / parts, v0 = part * per, v1 = min(rv.count, v0 + per);
-  const A c = B::scale(p.temperature), inf = (A)INFINITY;
+  // (parts is a power of two)
+  const long long per = (rv.count + parts - 1) >> (31 - __clz(parts)), v0 = part * per, v1 = min(rv.count, v0 + per);
+  const A inf = (A)INFINITY;
 
   uint4* mine = sh.ring + tid;                              // stage s, vector i: mine[(s * LP_VECS + i) * NT]
   auto fetch = [&](long long v, int stage) {                // the thread's vectors of the chunk at v, as one copy group
@@ -504,7 +508,7 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_
     a.s = a.t = 0;
     for (int k = 0; k < NW; ++k) { a.s += sh.s[k]; a.t += sh.t[k]; }
   }
-  const A inv_t = (A)(1.0 / p.temperature), log_s = bad ? (A)NAN : empty ? -inf : (B::log(a.s) - past) * B::unit();
+  const A log_s = bad ? (A)NAN : empty ? -inf : (B::log(a.s) - past) * B::unit();
   // in nats from the start: a lowest-value score may be finite here and not in base 2
   auto log_p = [&](A x) { return empty ? -inf : (x - a.m) * inv_t - log_s; };
   if (tid == 0) {
@@ -532,35 +536,50 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_
     }
 }
 
-// Gradient: a CTA takes NT x LP_VECS vectors of one row, placed on the gradient's 16-byte boundaries. With the row's m and
-// log s a score needs no sum: p (A + B log p), with A = -(g + g_H H) / T, B = -g_H / T and g the sum of the upstream
-// gradients of the row's given and best columns (less that of lse). Those columns are written once more, by the first
-// entry that names them, with the entries that repeat it added in order. Bound by the two matrices' bytes.
+// Gradient: a CTA takes `chunks` x NT x LP_VECS vectors of one row, placed on the gradient's 16-byte boundaries, the next
+// chunk on its way while one is worked on. With the row's m and log s a score needs no sum: p (A + B log p), with
+// A = -(g + g_H H) / T, B = -g_H / T and g the sum of the upstream gradients of the row's given and best columns (less
+// that of lse). Those columns are written once more, by the first entry that names them, with the entries that repeat it
+// added in order. Bound by the two matrices' bytes.
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT) log_probs_grad_kernel(LogProbsGradProblem p, int parts) {
+__global__ void __launch_bounds__(NT, 1024 / NT) log_probs_grad_kernel(LogProbsGradProblem p, int parts, int chunks,
+                                                                       typename Acc<T>::type c,
+                                                                       typename Acc<T>::type inv_t) {
   using A = typename Acc<T>::type;
   using B = typename Base<T>::type;
-  constexpr int kN = Vec<T>::kN;
+  constexpr int kN = Vec<T>::kN, kChunk = NT * LP_VECS;
   const int tid = threadIdx.x, lane = tid & 31;
-  const long long row = blockIdx.x / parts, v0 = (long long)(blockIdx.x % parts) * NT * LP_VECS;
+  const long long row = blockIdx.x / (unsigned)parts;
+  const long long v0 = (long long)(blockIdx.x - (unsigned)row * (unsigned)parts) * chunks * kChunk;
   const T* s = static_cast<const T*>(p.scores) + row * p.ld;
   T* out = static_cast<T*>(p.grad) + row * p.ld_grad;
   const RowVectors<T> rv(out, p.cols);
-  const long long first = rv.column(v0), end = rv.column(v0 + NT * LP_VECS);    // the CTA's columns
+  const long long v1 = min(rv.count, v0 + (long long)chunks * kChunk);
+  const long long first = rv.column(v0), end = rv.column(v1);                   // the CTA's columns
   const bool vectors = (reinterpret_cast<uintptr_t>(s + first) & 15) == 0;     // the scores' vectors fall together
-  Vec<T> q[LP_VECS];
+  auto fetch = [&](Vec<T>(&q)[LP_VECS], long long v) {
+    if (vectors && v + kChunk <= v1 && rv.inside(v, kChunk)) {
+      const T* at = s + rv.column(v + tid);
 #pragma unroll
-  for (int i = 0; i < LP_VECS; ++i) {
-    const long long v = v0 + i * NT + tid, j = rv.column(v);
-    if (vectors && rv.inside(v)) {
-      q[i] = RowVectors<T>::read(s + j);
+      for (int i = 0; i < LP_VECS; ++i) q[i] = RowVectors<T>::read(at + i * NT * kN);
     } else {
 #pragma unroll
-      for (int e = 0; e < kN; ++e) q[i].set(e, j + e >= 0 && j + e < p.cols ? s[j + e] : lowest_inf<T>());
+      for (int i = 0; i < LP_VECS; ++i) {
+        const long long at = v + i * NT + tid, j = rv.column(at);
+        if (vectors && at < v1 && rv.inside(at)) {
+          q[i] = RowVectors<T>::read(s + j);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kN; ++e)
+            q[i].set(e, at < v1 && j + e >= 0 && j + e < p.cols ? s[j + e] : lowest_inf<T>());
+        }
+      }
     }
-  }
+  };
+  Vec<T> q[LP_VECS];
+  fetch(q, v0);
 
-  const A inv_t = (A)(1.0 / p.temperature), inf = (A)INFINITY;
+  const A inf = (A)INFINITY;
   const int extra = p.n_targets + p.top;
   // entry k < n_targets is a given column, the others are the best columns
   const long long* tg = p.targets + row * p.n_targets;
@@ -581,28 +600,52 @@ __global__ void __launch_bounds__(NT) log_probs_grad_kernel(LogProbsGradProblem 
   total = warp_sum(total);
   if (p.d_lse) total -= static_cast<const A*>(p.d_lse)[row];
   const bool empty = m == -inf;
-  const A c = B::scale(p.temperature), ls = log_s / B::unit(), fa = -inv_t * (total + gh * h), fb = -inv_t * gh * B::unit();
+  const A ls = log_s * B::per_unit(), fa = -inv_t * (total + gh * h), fb = -inv_t * gh * B::unit();
   auto dense = [&](A x) {
     const A lp = floored(fma(x - m, c, -ls));
-    return empty ? (A)0 : B::exp(lp) * fma(fb, lp, fa);
+    return B::exp(lp) * fma(fb, lp, fa);
   };
+  for (long long v = v0; v < v1; v += kChunk) {
+    Vec<T> next[LP_VECS];
+    if (v + kChunk < v1) fetch(next, v + kChunk);
 #pragma unroll
-  for (int i = 0; i < LP_VECS; ++i) {
-    const long long v = v0 + i * NT + tid, j = rv.column(v);
-    Vec<T> r;
+    for (int i = 0; i < LP_VECS; ++i) {
 #pragma unroll
-    for (int e = 0; e < kN; ++e) {
-      T x;
-      narrow(dense(q[i].get(e)), &x);
-      r.set(e, x);
+      for (int e = 0; e < kN; e += 2) {
+        if constexpr (sizeof(A) == 4) {
+          float a, b;
+          unpack2(fma2(add2(pack2(q[i].get(e), q[i].get(e + 1)), pack2(-m, -m)), pack2(c, c), pack2(-ls, -ls)), a, b);
+          a = floored(a);
+          b = floored(b);
+          const uint64_t f = fma2(pack2(a, b), pack2(fb, fb), pack2(fa, fa));
+          unpack2(mul2(pack2(B::exp(a), B::exp(b)), f), a, b);
+          q[i].set_pair(e, a, b);
+        } else {
+          q[i].set_pair(e, dense(q[i].get(e)), dense(q[i].get(e + 1)));
+        }
+      }
+      if (empty) q[i].q = make_uint4(0, 0, 0, 0);
     }
-    if (rv.inside(v)) {
-      *reinterpret_cast<uint4*>(out + j) = r.q;
+    if (v + kChunk <= v1 && rv.inside(v, kChunk)) {
+      T* at = out + rv.column(v + tid);
+#pragma unroll
+      for (int i = 0; i < LP_VECS; ++i) *reinterpret_cast<uint4*>(at + i * NT * kN) = q[i].q;
     } else {
 #pragma unroll
-      for (int e = 0; e < kN; ++e)
-        if (j + e >= 0 && j + e < p.cols) narrow(dense(q[i].get(e)), out + j + e);
+      for (int i = 0; i < LP_VECS; ++i) {
+        const long long at = v + i * NT + tid, j = rv.column(at);
+        if (at >= v1) continue;
+        if (rv.inside(at)) {
+          *reinterpret_cast<uint4*>(out + j) = q[i].q;
+        } else {
+#pragma unroll
+          for (int e = 0; e < kN; ++e)
+            if (j + e >= 0 && j + e < p.cols) out[j + e] = q[i].stored(e);
+        }
+      }
     }
+#pragma unroll
+    for (int i = 0; i < LP_VECS; ++i) q[i] = next[i];
   }
   if (extra == 0 || empty) return;
   __syncthreads();                                         // the named columns follow the CTA's others
@@ -663,7 +706,8 @@ cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
     attr.val.clusterDim = {(unsigned)parts, 1, 1};
     cfg.attrs = &attr;
     cfg.numAttrs = parts > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, log_probs_kernel<T, NW, kTop>, q, parts);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, log_probs_kernel<T, NW, kTop>, q, parts, Base<T>::type::scale(p.temperature),
+                                             (typename Acc<T>::type)(1.0 / p.temperature));
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -688,7 +732,11 @@ cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
 template <typename T, int NT>
 cudaError_t grad_launch(const LogProbsGradProblem& p, cudaStream_t stream) {
   constexpr long long kCols = (long long)NT * LP_VECS * Vec<T>::kN;
-  const int parts = (int)((p.cols + Vec<T>::kN - 1 + kCols - 1) / kCols);      // (a row may start inside a vector)
+  const long long all = (p.cols + Vec<T>::kN - 1 + kCols - 1) / kCols;         // (a row may start inside a vector)
+  // up to 4 chunks per CTA, which share the row's numbers, while there are CTAs for every SM's 4 places
+  int chunks = 1;
+  while (chunks < 4 && chunks < all && p.rows * ((all + 2 * chunks - 1) / (2 * chunks)) >= 148 * 8) chunks *= 2;
+  const int parts = (int)((all + chunks - 1) / chunks);
   const long long per = (1LL << 30) / parts;
   const size_t size = sizeof(typename Acc<T>::type);
   for (long long r = 0; r < p.rows; r += per) {
@@ -706,7 +754,8 @@ cudaError_t grad_launch(const LogProbsGradProblem& p, cudaStream_t stream) {
     q.d_entropy = at(p.d_entropy, r);
     q.d_lse = at(p.d_lse, r);
     q.d_top = at(p.d_top, r * p.top);
-    log_probs_grad_kernel<T, NT><<<(unsigned)(q.rows * parts), NT, 0, stream>>>(q, parts);
+    log_probs_grad_kernel<T, NT><<<(unsigned)(q.rows * parts), NT, 0, stream>>>(
+        q, parts, chunks, Base<T>::type::scale(p.temperature), (typename Acc<T>::type)(1.0 / p.temperature));
   }
   return cudaGetLastError();
 }

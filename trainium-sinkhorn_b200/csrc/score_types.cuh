@@ -52,6 +52,12 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return d;
 }
 
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // max that keeps a NaN
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -92,6 +98,31 @@ struct Vec {
     q = make_uint4(w[0], w[1], w[2], w[3]);
   }
 
+  // Scores i and i + 1 (i even), rounded.
+  __device__ __forceinline__ void set_pair(int i, typename Acc<T>::type a, typename Acc<T>::type b) {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t x = pair_of(a, b, (const T*)nullptr);
+      if (i == 0) q.x = x;
+      else if (i == 2) q.y = x;
+      else if (i == 4) q.z = x;
+      else q.w = x;
+    } else {
+      set(i, (T)a);
+      set(i + 1, (T)b);
+    }
+  }
+  __device__ __forceinline__ T stored(int i) const {
+    T r;
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    if constexpr (sizeof(T) == 2) {
+      const uint16_t b = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+      r = *reinterpret_cast<const T*>(&b);
+    } else {
+      r = (T)get(i);
+    }
+    return r;
+  }
+
   // The largest of the kN scores, NaN if one is; two 16-bit scores at a time.
   __device__ __forceinline__ typename Acc<T>::type peak() const {
     if constexpr (sizeof(T) == 2) {
@@ -105,6 +136,14 @@ struct Vec {
   }
 
  private:
+  static __device__ __forceinline__ uint32_t pair_of(float a, float b, const __nv_bfloat16*) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint32_t pair_of(float a, float b, const __half*) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
   static __device__ __forceinline__ float half_of(uint32_t x, int odd, const __nv_bfloat16*) {
     return __uint_as_float(odd ? x & 0xffff0000u : x << 16);
   }
