@@ -510,7 +510,7 @@ int trnopt_balance(int type, const void* scores, long long ld, int rows, int col
                    size_t ws_bytes, void* stream) {
   const int st = check_scores(type, scores, ld, rows, cols, false);
   if (st != TRNOPT_OK) return st;
-  if (rows < 1 || iters < 1 || !(eps >= 1e-30 && eps <= 1e30) || !f || !g) return TRNOPT_ERR_INVALID_ARGUMENT;
+  if (rows < 1 || iters < 1 || iters > (1 << 24) || !(eps >= 1e-30 && eps <= 1e30) || !f || !g) return TRNOPT_ERR_INVALID_ARGUMENT;
   if (cols > 1024) return TRNOPT_ERR_UNSUPPORTED;
   const int dev = current_device();
   if (!workspace || ws_bytes < balance_workspace_bytes(dev, rows, cols)) return TRNOPT_ERR_WORKSPACE;

@@ -21,6 +21,23 @@ __device__ __forceinline__ void narrow(float v, __half* p) { *p = __float2half_r
 __device__ __forceinline__ void narrow(float v, __nv_bfloat16* p) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void narrow(double v, double* p) { *p = v; }
 
+// Two neighbouring scores, on a boundary of both.
+__device__ __forceinline__ void load_pair(const float* p, float& a, float& b) {
+  const float2 v = __ldg(reinterpret_cast<const float2*>(p));
+  a = v.x;
+  b = v.y;
+}
+__device__ __forceinline__ void load_pair(const __half* p, float& a, float& b) {
+  const float2 v = __half22float2(__ldg(reinterpret_cast<const __half2*>(p)));
+  a = v.x;
+  b = v.y;
+}
+__device__ __forceinline__ void load_pair(const __nv_bfloat16* p, float& a, float& b) {
+  const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(p));
+  a = __uint_as_float(v << 16);
+  b = __uint_as_float(v & 0xffff0000u);
+}
+
 // Asynchronous 16-byte copies into shared memory, waited for by the thread that made them.
 __device__ __forceinline__ void copy_async16(void* to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
@@ -194,7 +211,7 @@ struct RowVectors {
   }
   static __device__ __forceinline__ Vec<T> read(const T* at) {
     Vec<T> r;
-    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
         : "=r"(r.q.x), "=r"(r.q.y), "=r"(r.q.z), "=r"(r.q.w)
         : "l"(at));
     return r;

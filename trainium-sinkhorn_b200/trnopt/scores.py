@@ -203,8 +203,8 @@ def balance(scores: torch.Tensor, *, eps: float = 0.05, iters: int = 20, a: torc
         raise ValueError("scores need between 1 and 2**31 - 1 rows")
     if not 1e-30 <= eps <= 1e30:
         raise ValueError("eps must be positive and finite (1e-30 .. 1e30)")
-    if iters < 1:
-        raise ValueError("iters must be at least 1")
+    if not 1 <= iters <= 1 << 24:
+        raise ValueError("iters must lie in 1 .. 2**24")
     a, b, g = _small(a, rows, "a", s), _small(b, cols, "b", s), _small(g, cols, "g", s)
     f = torch.empty(rows, dtype=torch.float32, device=s.device)
     g_out = torch.empty(cols, dtype=torch.float32, device=s.device)
