@@ -19,6 +19,8 @@
 // exponentials (16 per clock and SM) for many rows, by the barrier's latency for few.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "score_types.cuh"
@@ -94,31 +96,39 @@ __device__ __forceinline__ bool grid_barrier(unsigned* counter, unsigned target,
 
 struct BalanceWork {
   unsigned* counter;       // arrivals at the barrier, 0 at the start
-  float2* parts;           // (2, CTAs, cols): column sums (maximum and sum in the first iteration), by parity
+  float* parts;            // (2, 2, CTAs, cols rounded up to 4): by parity, the CTAs' column sums, and their maxima in the
+                           // first iteration
   int* error_word;
 };
 
 template <int C> struct BalanceShape {
   static constexpr int kThreads = C == 32 ? 256 : 512;
-  static constexpr int kRows = C <= 4 ? 4 : C == 8 ? 2 : 1;
+  static constexpr int kRows = C <= 8 ? 4 : C == 16 ? 2 : 1;
 };
 
-// C columns per lane, kPair: in neighbouring pairs (2 lane + 64 k), else lane + 32 k.
-template <typename T, int C, bool kPair>
+// Shared memory for the warps' column sums, and then for the slices of the sum over the CTAs (NT quads of float64).
+__host__ __device__ inline size_t exchange_bytes(int cols, int threads) {
+  const size_t warps = (size_t)(threads / 32) * cols * sizeof(float2), slices = (size_t)threads * 4 * sizeof(double);
+  return ((warps > slices ? warps : slices) + 15) & ~(size_t)15;
+}
+
+// C columns per lane, in runs of V neighbouring ones.
+template <typename T, int C, int V>
 __global__ void __launch_bounds__(BalanceShape<C>::kThreads, 1) balance_kernel(BalanceProblem p, BalanceWork wk) {
   constexpr int NT = BalanceShape<C>::kThreads, NW = NT / 32, kRows = BalanceShape<C>::kRows;
   extern __shared__ __align__(16) unsigned char smem[];
   // per-warp column sums, then the slices of the sum over the CTAs; the potentials u; whether a column has any term
   float2* red = reinterpret_cast<float2*>(smem);                    // (NW, cols)
-  double* us = reinterpret_cast<double*>(red + (size_t)NW * p.cols);
+  const int cols4 = (p.cols + 3) & ~3;
+  double* us = reinterpret_cast<double*>(smem + exchange_bytes(p.cols, NT));
   unsigned char* open = reinterpret_cast<unsigned char*>(us + p.cols);
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, cols = p.cols;
   const T* scores = static_cast<const T*>(p.scores);
-  const double per_eps = 1.4426950408889634 / p.eps;
+  const double per_eps = 1.4426950408889634 / p.eps, eps_per = p.eps * 0.6931471805599453;
   const float c = (float)per_eps;
   const long long r0 = (long long)blockIdx.x * p.rows / gridDim.x, r1 = (long long)(blockIdx.x + 1) * p.rows / gridDim.x;
-  auto column = [&](int k) { return kPair ? 2 * lane + 64 * (k / 2) + (k & 1) : lane + 32 * k; };
+  auto column = [&](int k) { return V * lane + 32 * V * (k / V) + k % V; };
 
   float b[C], u[C];
   bool closed = false;                                      // a column of mass 0 is there
@@ -146,75 +156,112 @@ __global__ void __launch_bounds__(BalanceShape<C>::kThreads, 1) balance_kernel(B
     float sum[C], peak[C];                                  // column sums; their maxima in the first iteration
 #pragma unroll
     for (int k = 0; k < C; ++k) { sum[k] = 0.f; peak[k] = -INFINITY; }
-    for (long long row = r0 + (long long)w * kRows; row < r1; row += NW * kRows) {
-      float z[kRows][C], m[kRows], l[kRows], a[kRows];
+    // the rows: kFirst with running maxima per column, kClosed where columns of mass 0 must not set a row's maximum
+    auto pass = [&](auto first_, auto closed_) {
+      constexpr bool kFirst = decltype(first_)::value, kClosed = decltype(closed_)::value;
+      const T* at = scores + (r0 + (long long)w * kRows) * p.ld + V * lane;
+      for (long long row = r0 + (long long)w * kRows; row < r1; row += NW * kRows, at += NW * kRows * p.ld) {
+        float z[kRows][C], m[kRows], l[kRows];
+        const bool whole = row + kRows <= r1;
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const bool there = row + r < r1;
-        const T* s = scores + (there ? row + r : row) * p.ld;
-        a[r] = there ? (p.a ? p.a[row + r] : 1.f) : 0.f;
+        for (int r = 0; r < kRows; ++r) {
+          const T* s = at + (whole || row + r < r1 ? r * p.ld : 0);
 #pragma unroll
-        for (int k = 0; k < C; k += kPair ? 2 : 1) {
-          const int j = column(k);
-          if constexpr (kPair) {
-            float x0 = -INFINITY, x1 = -INFINITY;
-            if (j < cols) load_pair(s + j, x0, x1);
-            z[r][k] = x0;
-            z[r][k + 1] = x1;
-          } else {
-            z[r][k] = j < cols ? widen(s[j]) : -INFINITY;
+          for (int k = 0; k < C; k += V) {
+            if (column(k) < cols) {
+              load_scores<V>(s + 32 * k, z[r] + k);
+            } else {
+#pragma unroll
+              for (int i = 0; i < V; ++i) z[r][k + i] = -INFINITY;
+            }
           }
         }
-      }
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        m[r] = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < C; ++k) {
-          z[r][k] = fmaf(z[r][k], c, u[k]);
-          m[r] = fmaxf(m[r], !closed || b[k] > 0.f ? z[r][k] : -INFINITY);
-        }
-        m[r] = warp_max(m[r]);
-        const float shown = m[r] == -INFINITY ? 0.f : m[r];
-        l[r] = 0.f;
-#pragma unroll
-        for (int k = 0; k < C; ++k) {
-          z[r][k] -= shown;
-          const float e = ex2_approx(z[r][k]);
-          l[r] = fmaf(b[k], b[k] > 0.f ? e : 0.f, l[r]);
-          if (!first) z[r][k] = e;
-        }
-      }
-      warp_sums<kRows>(l);
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const bool empty = l[r] == 0.f;                     // f = 0: terms 2^(S c + u) as they are, less the shift
-        if (last && lane == 0 && row + r < r1)
-          p.f[row + r] = empty ? 0.f : (float)(-((double)(m[r] == -INFINITY ? 0.f : m[r]) + (double)log2f(l[r]) + shift) / per_eps);
-        if (first) {
-          // x = S c + f c + log2 a, in the gauge of u - shift: z - u - log2 l + log2 a
-          const float off = (empty ? (float)shift : -log2f(l[r])) + log2f(a[r]);
+        for (int r = 0; r < kRows; ++r) {
+          float top = -INFINITY;
 #pragma unroll
           for (int k = 0; k < C; ++k) {
-            const float x = z[r][k] - u[k] + off;
-            if (column(k) < cols && x != -INFINITY) lse2_add(peak[k], sum[k], x, 1.f);
+            z[r][k] = fmaf(z[r][k], c, u[k]);
+            top = fmaxf(top, !kClosed || b[k] > 0.f ? z[r][k] : -INFINITY);
           }
-        } else {
-          const float weight = empty ? a[r] * exp2f((float)shift) : a[r] / l[r];
-          if (a[r] != 0.f)
+          top = warp_max(top);
+          m[r] = top == -INFINITY ? 0.f : top;
+          l[r] = 0.f;
+          if constexpr (C % 2 == 0 && !kClosed) {
+            uint64_t l2 = 0;
+            const uint64_t m2 = pack2(-m[r], -m[r]);
 #pragma unroll
-            for (int k = 0; k < C; ++k) sum[k] = fmaf(z[r][k], weight, sum[k]);
+            for (int k = 0; k < C; k += 2) {
+              float x, y;
+              unpack2(add2(pack2(z[r][k], z[r][k + 1]), m2), x, y);
+              const float ex = ex2_approx(x), ey = ex2_approx(y);
+              l2 = fma2(pack2(b[k], b[k + 1]), pack2(ex, ey), l2);
+              z[r][k] = kFirst ? x : ex;
+              z[r][k + 1] = kFirst ? y : ey;
+            }
+            float x, y;
+            unpack2(l2, x, y);
+            l[r] = x + y;
+          } else {
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+              z[r][k] -= m[r];
+              const float e = ex2_approx(z[r][k]);
+              l[r] = fmaf(b[k], !kClosed || b[k] > 0.f ? e : 0.f, l[r]);
+              if (!kFirst) z[r][k] = e;
+            }
+          }
+        }
+        warp_sums<kRows>(l);
+        if (last && lane < kRows && row + lane < r1) {
+          float lr = l[0], mr = m[0];
+#pragma unroll
+          for (int r = 1; r < kRows; ++r) {
+            lr = lane == r ? l[r] : lr;
+            mr = lane == r ? m[r] : mr;
+          }
+          p.f[row + lane] = lr == 0.f ? 0.f : (float)(-((double)mr + (double)log2f(lr) + shift) * eps_per);
+        }
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          const float a = !whole && row + r >= r1 ? 0.f : p.a ? __ldg(p.a + row + r) : 1.f;
+          const bool empty = l[r] == 0.f;                   // f = 0: terms 2^(S c + u) as they are, less the shift
+          if constexpr (kFirst) {
+            // x = S c + f c + log2 a, in the gauge of u - shift: z - u - log2 l + log2 a
+            const float off = (empty ? (float)shift : -log2f(l[r])) + log2f(a);
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+              const float x = z[r][k] - u[k] + off;
+              if (column(k) < cols && x != -INFINITY) lse2_add(peak[k], sum[k], x, 1.f);
+            }
+          } else if (a != 0.f) {
+            const float weight = empty ? a * exp2f((float)shift) : __fdividef(a, l[r]);
+            if constexpr (C % 2 == 0) {
+              const uint64_t w2 = pack2(weight, weight);
+#pragma unroll
+              for (int k = 0; k < C; k += 2)
+                unpack2(fma2(pack2(z[r][k], z[r][k + 1]), w2, pack2(sum[k], sum[k + 1])), sum[k], sum[k + 1]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < C; ++k) sum[k] = fmaf(z[r][k], weight, sum[k]);
+            }
+          }
         }
       }
-    }
+    };
+    if (first) pass(std::true_type{}, std::true_type{});
+    else if (closed) pass(std::false_type{}, std::true_type{});
+    else pass(std::false_type{}, std::false_type{});
 
-    // column sums of the CTA's warps, then of all CTAs (in the same order everywhere)
+    // column sums of the CTA's warps
     float2* mine = red + (size_t)w * cols;
 #pragma unroll
     for (int k = 0; k < C; ++k)
       if (column(k) < cols) mine[column(k)] = make_float2(peak[k], sum[k]);
     __syncthreads();
-    float2* parts = wk.parts + (size_t)(it & 1) * gridDim.x * cols;
+    const size_t plane = (size_t)gridDim.x * cols4;
+    float* sums = wk.parts + (size_t)(it & 1) * 2 * plane;
+    float* peaks = sums + plane;
     for (int j = tid; j < cols; j += NT) {
       float2 v = red[j];
       for (int k = 1; k < NW; ++k) {
@@ -222,7 +269,8 @@ __global__ void __launch_bounds__(BalanceShape<C>::kThreads, 1) balance_kernel(B
         if (first) lse2_add(v.x, v.y, o.x, o.y);
         else v.y += o.y;
       }
-      __stcg(parts + (size_t)blockIdx.x * cols + j, v);
+      __stcg(sums + (size_t)blockIdx.x * cols4 + j, v.y);
+      if (first) __stcg(peaks + (size_t)blockIdx.x * cols4 + j, v.x);
     }
     if (!grid_barrier(wk.counter, (unsigned)(it + 1) * gridDim.x, wk.error_word, &flag)) {
       // gave up: no potentials
@@ -231,20 +279,53 @@ __global__ void __launch_bounds__(BalanceShape<C>::kThreads, 1) balance_kernel(B
         for (int j = tid; j < cols; j += NT) p.g[j] = NAN;
       return;
     }
+    // of all CTAs, in the same order in each: four columns per thread, the CTAs in `slices` interleaved parts
+    const int quads = cols4 / 4, slices = NT / quads, slice = tid / quads, quad = tid - slice * quads;
+    double* part = reinterpret_cast<double*>(smem) + (size_t)slice * cols4 + 4 * quad;   // (`red` is free again)
+    if (slice < slices) {
+      if (first) {
+        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int k = slice; k < (int)gridDim.x; k += slices) {
+          const float4 om = __ldcg(reinterpret_cast<const float4*>(peaks + (size_t)k * cols4) + quad);
+          const float4 ol = __ldcg(reinterpret_cast<const float4*>(sums + (size_t)k * cols4) + quad);
+          lse2_add(m[0], l[0], om.x, ol.x);
+          lse2_add(m[1], l[1], om.y, ol.y);
+          lse2_add(m[2], l[2], om.z, ol.z);
+          lse2_add(m[3], l[3], om.w, ol.w);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(part + e) = make_float2(m[e], l[e]);
+      } else {
+        double v[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 16
+        for (int k = slice; k < (int)gridDim.x; k += slices) {
+          const float4 o = __ldcg(reinterpret_cast<const float4*>(sums + (size_t)k * cols4) + quad);
+          v[0] += (double)o.x;
+          v[1] += (double)o.y;
+          v[2] += (double)o.z;
+          v[3] += (double)o.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[e] = v[e];
+      }
+    }
+    __syncthreads();
     const double log_rows = p.a ? 0.0 : log2((double)p.rows);
     for (int j = tid; j < cols; j += NT) {
+      const double* at = reinterpret_cast<const double*>(smem) + j;
       double next;
       if (first) {
-        float2 v = __ldcg(parts + j);
-        for (int k = 1; k < (int)gridDim.x; ++k) {
-          const float2 o = __ldcg(parts + (size_t)k * cols + j);
+        float2 v = *reinterpret_cast<const float2*>(at);
+        for (int k = 1; k < slices; ++k) {
+          const float2 o = *reinterpret_cast<const float2*>(at + (size_t)k * cols4);
           lse2_add(v.x, v.y, o.x, o.y);
         }
         open[j] = v.y != 0.f;
         next = v.y == 0.f ? 0.0 : shift + log_rows - ((double)v.x + log2((double)v.y));
       } else {
         double k_j = 0.0;
-        for (int k = 0; k < (int)gridDim.x; ++k) k_j += (double)__ldcg(&parts[(size_t)k * cols + j].y);
+        for (int k = 0; k < slices; ++k) k_j += at[(size_t)k * cols4];
         // the same float32 potential that the sums were formed with
         const double before = (double)(float)(us[j] - shift) + shift;
         // (a sum that underflows, for masses beyond float32's range from one another, counts as 2^-126)
@@ -255,10 +336,10 @@ __global__ void __launch_bounds__(BalanceShape<C>::kThreads, 1) balance_kernel(B
     __syncthreads();
   }
   if (blockIdx.x == 0)
-    for (int j = tid; j < cols; j += NT) p.g[j] = (float)(us[j] / per_eps);
+    for (int j = tid; j < cols; j += NT) p.g[j] = (float)(us[j] * eps_per);
 }
 
-size_t smem_bytes(int cols, int threads) { return (size_t)(threads / 32) * cols * sizeof(float2) + cols * (sizeof(double) + 1); }
+size_t smem_bytes(int cols, int threads) { return exchange_bytes(cols, threads) + cols * (sizeof(double) + 1); }
 
 int columns_per_lane(int cols) {
   int c = 1;
@@ -283,11 +364,11 @@ int balance_grid(int device, int rows) {
   return want < most ? want : most;
 }
 
-template <typename T, int C, bool kPair>
+template <typename T, int C, int V>
 cudaError_t launch(int device, const BalanceProblem& p, const BalanceWork& wk, cudaStream_t stream) {
   const size_t bytes = smem_bytes(p.cols, BalanceShape<C>::kThreads);
   static std::atomic<int> done[kMaxDevices];
-  cudaError_t e = smem_attr_once(reinterpret_cast<const void*>(balance_kernel<T, C, kPair>), (int)bytes, done);
+  cudaError_t e = smem_attr_once(reinterpret_cast<const void*>(balance_kernel<T, C, V>), (int)bytes, done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)balance_grid(device, p.rows));
@@ -299,19 +380,27 @@ cudaError_t launch(int device, const BalanceProblem& p, const BalanceWork& wk, c
   attr.val.cooperative = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, balance_kernel<T, C, kPair>, p, wk);
+  return cudaLaunchKernelEx(&cfg, balance_kernel<T, C, V>, p, wk);
 }
 
 template <typename T>
 cudaError_t launch(int device, const BalanceProblem& p, const BalanceWork& wk, cudaStream_t stream) {
-  const bool pair = p.cols % 2 == 0 && p.ld % 2 == 0 && reinterpret_cast<uintptr_t>(p.scores) % (2 * sizeof(T)) == 0;
+  // the longest runs of columns per lane (up to 16 bytes) that the sizes and addresses allow
+  auto runs = [&](int v) {
+    return p.cols % v == 0 && p.ld % v == 0 && reinterpret_cast<uintptr_t>(p.scores) % (v * sizeof(T)) == 0;
+  };
+  constexpr int kLong = 16 / (int)sizeof(T);
   switch (columns_per_lane(p.cols)) {
-    case 1: return launch<T, 1, false>(device, p, wk, stream);
-    case 2: return pair ? launch<T, 2, true>(device, p, wk, stream) : launch<T, 2, false>(device, p, wk, stream);
-    case 4: return pair ? launch<T, 4, true>(device, p, wk, stream) : launch<T, 4, false>(device, p, wk, stream);
-    case 8: return pair ? launch<T, 8, true>(device, p, wk, stream) : launch<T, 8, false>(device, p, wk, stream);
-    case 16: return pair ? launch<T, 16, true>(device, p, wk, stream) : launch<T, 16, false>(device, p, wk, stream);
-    default: return pair ? launch<T, 32, true>(device, p, wk, stream) : launch<T, 32, false>(device, p, wk, stream);
+    case 1: return launch<T, 1, 1>(device, p, wk, stream);
+    case 2: return runs(2) ? launch<T, 2, 2>(device, p, wk, stream) : launch<T, 2, 1>(device, p, wk, stream);
+    case 4: return runs(4) ? launch<T, 4, 4>(device, p, wk, stream)
+                           : runs(2) ? launch<T, 4, 2>(device, p, wk, stream) : launch<T, 4, 1>(device, p, wk, stream);
+    case 8: return runs(kLong) ? launch<T, 8, kLong>(device, p, wk, stream)
+                               : runs(2) ? launch<T, 8, 2>(device, p, wk, stream) : launch<T, 8, 1>(device, p, wk, stream);
+    case 16: return runs(kLong) ? launch<T, 16, kLong>(device, p, wk, stream)
+                                : runs(2) ? launch<T, 16, 2>(device, p, wk, stream) : launch<T, 16, 1>(device, p, wk, stream);
+    default: return runs(kLong) ? launch<T, 32, kLong>(device, p, wk, stream)
+                                : runs(2) ? launch<T, 32, 2>(device, p, wk, stream) : launch<T, 32, 1>(device, p, wk, stream);
   }
 }
 
@@ -320,11 +409,11 @@ constexpr size_t kCounterBytes = 256;
 }  // namespace
 
 size_t balance_workspace_bytes(int device, int rows, int cols) {
-  return kCounterBytes + (size_t)2 * balance_grid(device, rows) * cols * sizeof(float2);
+  return kCounterBytes + (size_t)4 * balance_grid(device, rows) * ((cols + 3) & ~3) * sizeof(float);
 }
 
 cudaError_t balance_launch(int device, int type, const BalanceProblem& p, void* ws, cudaStream_t stream) {
-  BalanceWork wk{static_cast<unsigned*>(ws), reinterpret_cast<float2*>(static_cast<char*>(ws) + kCounterBytes),
+  BalanceWork wk{static_cast<unsigned*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes),
                  device_error_word()};
   const cudaError_t e = cudaMemsetAsync(ws, 0, sizeof(unsigned), stream);
   if (e != cudaSuccess) return e;

@@ -21,23 +21,6 @@ __device__ __forceinline__ void narrow(float v, __half* p) { *p = __float2half_r
 __device__ __forceinline__ void narrow(float v, __nv_bfloat16* p) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void narrow(double v, double* p) { *p = v; }
 
-// Two neighbouring scores, on a boundary of both.
-__device__ __forceinline__ void load_pair(const float* p, float& a, float& b) {
-  const float2 v = __ldg(reinterpret_cast<const float2*>(p));
-  a = v.x;
-  b = v.y;
-}
-__device__ __forceinline__ void load_pair(const __half* p, float& a, float& b) {
-  const float2 v = __half22float2(__ldg(reinterpret_cast<const __half2*>(p)));
-  a = v.x;
-  b = v.y;
-}
-__device__ __forceinline__ void load_pair(const __nv_bfloat16* p, float& a, float& b) {
-  const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(p));
-  a = __uint_as_float(v << 16);
-  b = __uint_as_float(v & 0xffff0000u);
-}
-
 // Asynchronous 16-byte copies into shared memory, waited for by the thread that made them.
 __device__ __forceinline__ void copy_async16(void* to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
@@ -230,5 +213,21 @@ struct RowVectors {
     return r;
   }
 };
+
+// V neighbouring scores (at most 16 bytes, on a boundary of V), through the read-only cache.
+template <int V, typename T>
+__device__ __forceinline__ void load_scores(const T* p, float* out) {
+  constexpr int kBytes = V * (int)sizeof(T);
+  if constexpr (V == 1) {
+    out[0] = widen(__ldg(p));
+  } else {
+    Vec<T> v;
+    if constexpr (kBytes == 16) v.q = __ldg(reinterpret_cast<const uint4*>(p));
+    else if constexpr (kBytes == 8) { const uint2 h = __ldg(reinterpret_cast<const uint2*>(p)); v.q.x = h.x; v.q.y = h.y; }
+    else v.q.x = __ldg(reinterpret_cast<const uint32_t*>(p));
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = v.get(i);
+  }
+}
 
 }  // namespace trnopt
