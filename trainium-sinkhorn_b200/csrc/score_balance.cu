@@ -10,13 +10,15 @@
 // f_i c = -(m_i + log2 l_i); the column sums k_j = sum_i a_i e_ij / l_i then give the next potentials,
 // u_j <- u_j - log2 k_j. After an iteration every column's k_j would be 1, so the next one's lies between the smallest
 // a_i / (row sum) and the largest, far from underflow; only the first iteration, from any g, keeps a running maximum per
-// column instead. Potentials are held in float64 (their float32 copies are taken relative to the largest, which a row's
-// maximum absorbs), the sums over rows in float32 per warp and float64 over the CTAs.
+// column instead. Potentials are float32 relative to a column's after the first iteration (the common part, in float64,
+// goes back at the end): they are differences of a few units, where the potentials themselves may be hundreds.
 //
-// One cooperative launch runs all iterations: a CTA owns a block of rows (which its L1 or the L2 holds after the first
-// pass) and a warp takes kRows of them at a time, C columns per lane. Per iteration the CTAs exchange their column sums
-// through global memory and one grid barrier, and each adds up all of them in the same order. Bound by the
-// exponentials (16 per clock and SM) for many rows, by the barrier's latency for few.
+// One cooperative launch runs all iterations. A CTA owns a block of rows and keeps as many of them as fit in shared
+// memory as they were read in the first pass (the rest come from L2 in every pass); a warp takes kRows of them at a
+// time, C columns per lane, and a lane meets the same scores in every pass. Per iteration the CTAs exchange their column
+// sums through global memory and one grid barrier, and each adds up all of them in the same order. Bound by the
+// exponentials (16 per clock and SM) for many rows, by the barrier's latency for few; problems of up to
+// 1024 rows of 32 columns (512 of 64, ...) stay in one CTA, without it.
 #include <math.h>
 
 #include <type_traits>
@@ -74,8 +76,7 @@ __device__ __forceinline__ void lse2_add(float& m, float& l, float om, float ol)
 __device__ __forceinline__ bool grid_barrier(unsigned* counter, unsigned target, int* error_word, int* flag) {
   __syncthreads();
   if (threadIdx.x == 0) {
-    __threadfence();
-    atomicAdd(counter, 1u);
+    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory");
     const unsigned long long t0 = globaltimer_ns();
     int ok = 1;
     unsigned seen;
@@ -106,27 +107,34 @@ template <int C> struct BalanceShape {
   static constexpr int kRows = C <= 8 ? 4 : C == 16 ? 2 : 1;
 };
 
-// Shared memory for the warps' column sums, and then for the slices of the sum over the CTAs (NT quads of float64).
+// Shared memory: the warps' column sums, later the slices of the sum over the CTAs (NT quads), and the potentials; after
+// it the rows that are kept.
 __host__ __device__ inline size_t exchange_bytes(int cols, int threads) {
-  const size_t warps = (size_t)(threads / 32) * cols * sizeof(float2), slices = (size_t)threads * 4 * sizeof(double);
+  const size_t warps = (size_t)(threads / 32) * cols * sizeof(float2), slices = (size_t)threads * 4 * sizeof(float2);
   return ((warps > slices ? warps : slices) + 15) & ~(size_t)15;
 }
+__host__ __device__ inline size_t fixed_bytes(int cols, int threads) {
+  return (exchange_bytes(cols, threads) + cols * (sizeof(float) + 1) + 15) & ~(size_t)15;
+}
+__host__ __device__ inline int row_bytes(int cols, int size) { return (cols * size + 15) & ~15; }
 
 // C columns per lane, in runs of V neighbouring ones.
 template <typename T, int C, int V>
-__global__ void __launch_bounds__(BalanceShape<C>::kThreads, 1) balance_kernel(BalanceProblem p, BalanceWork wk) {
+__global__ void __launch_bounds__(BalanceShape<C>::kThreads, 1) balance_kernel(BalanceProblem p, BalanceWork wk,
+                                                                           int kept_rows) {
   constexpr int NT = BalanceShape<C>::kThreads, NW = NT / 32, kRows = BalanceShape<C>::kRows;
   extern __shared__ __align__(16) unsigned char smem[];
-  // per-warp column sums, then the slices of the sum over the CTAs; the potentials u; whether a column has any term
+  // per-warp column sums, then the slices of the sum over the CTAs; the potentials; whether a column has any term; rows
   float2* red = reinterpret_cast<float2*>(smem);                    // (NW, cols)
-  const int cols4 = (p.cols + 3) & ~3;
-  double* us = reinterpret_cast<double*>(smem + exchange_bytes(p.cols, NT));
+  float* us = reinterpret_cast<float*>(smem + exchange_bytes(p.cols, NT));
   unsigned char* open = reinterpret_cast<unsigned char*>(us + p.cols);
+  T* kept = reinterpret_cast<T*>(smem + fixed_bytes(p.cols, NT));   // (kept_rows, pitch)
   __shared__ int flag;
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, cols = p.cols;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, cols = p.cols, cols4 = (cols + 3) & ~3;
+  const int pitch = row_bytes(cols, sizeof(T)) / (int)sizeof(T);
   const T* scores = static_cast<const T*>(p.scores);
   const double per_eps = 1.4426950408889634 / p.eps, eps_per = p.eps * 0.6931471805599453;
-  const float c = (float)per_eps;
+  const float c = (float)per_eps, per_rows = p.a ? 1.f : 1.f / (float)p.rows;
   const long long r0 = (long long)blockIdx.x * p.rows / gridDim.x, r1 = (long long)(blockIdx.x + 1) * p.rows / gridDim.x;
   auto column = [&](int k) { return V * lane + 32 * V * (k / V) + k % V; };
 
@@ -139,19 +147,15 @@ __global__ void __launch_bounds__(BalanceShape<C>::kThreads, 1) balance_kernel(B
     closed = closed || (j < cols && b[k] == 0.f);
   }
   closed = __any_sync(kAll, closed);
-  for (int j = tid; j < cols; j += NT) us[j] = p.g0 ? (double)p.g0[j] * per_eps : 0.0;
+  // what float32 potentials are relative to: 0, or the given potential of column 0; later its potential after one iteration
+  double shift = p.g0 && fabsf(p.g0[0]) < INFINITY ? (double)p.g0[0] * per_eps : 0.0;
+  for (int j = tid; j < cols; j += NT) us[j] = p.g0 ? (float)((double)p.g0[j] * per_eps - shift) : 0.f;
   __syncthreads();
 
   for (int it = 0; it < p.iters; ++it) {
     const bool first = it == 0, last = it == p.iters - 1;
-    // float32 potentials relative to the largest
-    double shift = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < C; ++k) shift = fmax(shift, column(k) < cols ? us[column(k)] : -INFINITY);
-    for (int o = 16; o > 0; o >>= 1) shift = fmax(shift, __shfl_xor_sync(kAll, shift, o));
-    if (!(fabs(shift) < INFINITY)) shift = 0.0;
-#pragma unroll
-    for (int k = 0; k < C; ++k) u[k] = column(k) < cols ? (float)(us[column(k)] - shift) : -INFINITY;
+    for (int k = 0; k < C; ++k) u[k] = column(k) < cols ? us[column(k)] : -INFINITY;
 
     float sum[C], peak[C];                                  // column sums; their maxima in the first iteration
 #pragma unroll
@@ -160,20 +164,39 @@ __global__ void __launch_bounds__(BalanceShape<C>::kThreads, 1) balance_kernel(B
     auto pass = [&](auto first_, auto closed_) {
       constexpr bool kFirst = decltype(first_)::value, kClosed = decltype(closed_)::value;
       const T* at = scores + (r0 + (long long)w * kRows) * p.ld + V * lane;
-      for (long long row = r0 + (long long)w * kRows; row < r1; row += NW * kRows, at += NW * kRows * p.ld) {
+      T* here = kept + (size_t)w * kRows * pitch + V * lane;
+      for (long long row = r0 + (long long)w * kRows; row < r1;
+           row += NW * kRows, at += NW * kRows * p.ld, here += NW * kRows * pitch) {
         float z[kRows][C], m[kRows], l[kRows];
-        const bool whole = row + kRows <= r1;
+        const bool whole = row + kRows <= r1, keep = row - r0 + kRows <= kept_rows;
+        if (!kFirst && keep) {
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          const T* s = at + (whole || row + r < r1 ? r * p.ld : 0);
+          for (int r = 0; r < kRows; ++r)
 #pragma unroll
-          for (int k = 0; k < C; k += V) {
-            if (column(k) < cols) {
-              load_scores<V>(s + 32 * k, z[r] + k);
-            } else {
+            for (int k = 0; k < C; k += V)
+              if (column(k) < cols) {
+                const Vec<T> v = read_any<V>(here + r * pitch + 32 * k);
 #pragma unroll
-              for (int i = 0; i < V; ++i) z[r][k + i] = -INFINITY;
-            }
+                for (int i = 0; i < V; ++i) z[r][k + i] = v.get(i);
+              } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) z[r][k + i] = -INFINITY;
+              }
+        } else {
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            const T* s = at + (whole || row + r < r1 ? r * p.ld : 0);
+#pragma unroll
+            for (int k = 0; k < C; k += V)
+              if (column(k) < cols) {
+                const Vec<T> v = read_global<V>(s + 32 * k);
+                if (kFirst && keep) write_any<V>(here + r * pitch + 32 * k, v);
+#pragma unroll
+                for (int i = 0; i < V; ++i) z[r][k + i] = v.get(i);
+              } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) z[r][k + i] = -INFINITY;
+              }
           }
         }
 #pragma unroll
@@ -225,7 +248,7 @@ __global__ void __launch_bounds__(BalanceShape<C>::kThreads, 1) balance_kernel(B
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
           const float a = !whole && row + r >= r1 ? 0.f : p.a ? __ldg(p.a + row + r) : 1.f;
-          const bool empty = l[r] == 0.f;                   // f = 0: terms 2^(S c + u) as they are, less the shift
+          const bool empty = l[r] == 0.f;                   // f = 0: the terms 2^(S c + u) as they are
           if constexpr (kFirst) {
             // x = S c + f c + log2 a, in the gauge of u - shift: z - u - log2 l + log2 a
             const float off = (empty ? (float)shift : -log2f(l[r])) + log2f(a);
@@ -234,8 +257,13 @@ __global__ void __launch_bounds__(BalanceShape<C>::kThreads, 1) balance_kernel(B
               const float x = z[r][k] - u[k] + off;
               if (column(k) < cols && x != -INFINITY) lse2_add(peak[k], sum[k], x, 1.f);
             }
+          } else if (empty) {
+            if (a != 0.f)
+#pragma unroll
+              for (int k = 0; k < C; ++k)
+                if (z[r][k] > 0.f) sum[k] += a * exp2f(log2f(z[r][k]) + (float)shift);
           } else if (a != 0.f) {
-            const float weight = empty ? a * exp2f((float)shift) : __fdividef(a, l[r]);
+            const float weight = __fdividef(a, l[r]);
             if constexpr (C % 2 == 0) {
               const uint64_t w2 = pack2(weight, weight);
 #pragma unroll
@@ -259,87 +287,95 @@ __global__ void __launch_bounds__(BalanceShape<C>::kThreads, 1) balance_kernel(B
     for (int k = 0; k < C; ++k)
       if (column(k) < cols) mine[column(k)] = make_float2(peak[k], sum[k]);
     __syncthreads();
+    const bool alone = gridDim.x == 1;
     const size_t plane = (size_t)gridDim.x * cols4;
     float* sums = wk.parts + (size_t)(it & 1) * 2 * plane;
     float* peaks = sums + plane;
     for (int j = tid; j < cols; j += NT) {
       float2 v = red[j];
-      for (int k = 1; k < NW; ++k) {
-        const float2 o = red[(size_t)k * cols + j];
-        if (first) lse2_add(v.x, v.y, o.x, o.y);
-        else v.y += o.y;
-      }
-      __stcg(sums + (size_t)blockIdx.x * cols4 + j, v.y);
-      if (first) __stcg(peaks + (size_t)blockIdx.x * cols4 + j, v.x);
-    }
-    if (!grid_barrier(wk.counter, (unsigned)(it + 1) * gridDim.x, wk.error_word, &flag)) {
-      // gave up: no potentials
-      for (long long i = r0 + tid; i < r1; i += NT) p.f[i] = NAN;
-      if (blockIdx.x == 0)
-        for (int j = tid; j < cols; j += NT) p.g[j] = NAN;
-      return;
-    }
-    // of all CTAs, in the same order in each: four columns per thread, the CTAs in `slices` interleaved parts
-    const int quads = cols4 / 4, slices = NT / quads, slice = tid / quads, quad = tid - slice * quads;
-    double* part = reinterpret_cast<double*>(smem) + (size_t)slice * cols4 + 4 * quad;   // (`red` is free again)
-    if (slice < slices) {
       if (first) {
-        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 1; k < NW; ++k) lse2_add(v.x, v.y, red[(size_t)k * cols + j].x, red[(size_t)k * cols + j].y);
+      } else {
+#pragma unroll
+        for (int k = 1; k < NW; ++k) v.y += red[(size_t)k * cols + j].y;
+      }
+      if (alone) {
+        red[j] = v;                                         // (row 0 of `red` is read by this thread alone)
+      } else {
+        __stcg(sums + (size_t)blockIdx.x * cols4 + j, v.y);
+        if (first) __stcg(peaks + (size_t)blockIdx.x * cols4 + j, v.x);
+      }
+    }
+    int slices = 1;
+    if (!alone) {
+      if (!grid_barrier(wk.counter, (unsigned)(it + 1) * gridDim.x, wk.error_word, &flag)) {
+        // gave up: no potentials
+        for (long long i = r0 + tid; i < r1; i += NT) p.f[i] = NAN;
+        if (blockIdx.x == 0)
+          for (int j = tid; j < cols; j += NT) p.g[j] = NAN;
+        return;
+      }
+      // of all CTAs, in the same order in each: four columns per thread, the CTAs in `slices` interleaved parts
+      const int quads = cols4 / 4, slice = tid / quads, quad = tid - slice * quads;
+      slices = NT / quads;
+      float2* part = red + (size_t)slice * cols4 + 4 * quad;            // (`red` is free again)
+      if (slice < slices) {
+        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (first) {
 #pragma unroll 4
-        for (int k = slice; k < (int)gridDim.x; k += slices) {
-          const float4 om = __ldcg(reinterpret_cast<const float4*>(peaks + (size_t)k * cols4) + quad);
-          const float4 ol = __ldcg(reinterpret_cast<const float4*>(sums + (size_t)k * cols4) + quad);
-          lse2_add(m[0], l[0], om.x, ol.x);
-          lse2_add(m[1], l[1], om.y, ol.y);
-          lse2_add(m[2], l[2], om.z, ol.z);
-          lse2_add(m[3], l[3], om.w, ol.w);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(part + e) = make_float2(m[e], l[e]);
-      } else {
-        double v[4] = {0.0, 0.0, 0.0, 0.0};
+          for (int k = slice; k < (int)gridDim.x; k += slices) {
+            const float4 om = __ldcg(reinterpret_cast<const float4*>(peaks + (size_t)k * cols4) + quad);
+            const float4 ol = __ldcg(reinterpret_cast<const float4*>(sums + (size_t)k * cols4) + quad);
+            lse2_add(m[0], v[0], om.x, ol.x);
+            lse2_add(m[1], v[1], om.y, ol.y);
+            lse2_add(m[2], v[2], om.z, ol.z);
+            lse2_add(m[3], v[3], om.w, ol.w);
+          }
+        } else {
 #pragma unroll 16
-        for (int k = slice; k < (int)gridDim.x; k += slices) {
-          const float4 o = __ldcg(reinterpret_cast<const float4*>(sums + (size_t)k * cols4) + quad);
-          v[0] += (double)o.x;
-          v[1] += (double)o.y;
-          v[2] += (double)o.z;
-          v[3] += (double)o.w;
+          for (int k = slice; k < (int)gridDim.x; k += slices) {
+            const float4 o = __ldcg(reinterpret_cast<const float4*>(sums + (size_t)k * cols4) + quad);
+            v[0] += o.x;
+            v[1] += o.y;
+            v[2] += o.z;
+            v[3] += o.w;
+          }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) part[e] = v[e];
+        for (int e = 0; e < 4; ++e) part[e] = make_float2(m[e], v[e]);
       }
+      __syncthreads();
     }
-    __syncthreads();
-    const double log_rows = p.a ? 0.0 : log2((double)p.rows);
     for (int j = tid; j < cols; j += NT) {
-      const double* at = reinterpret_cast<const double*>(smem) + j;
-      double next;
+      float2 v = red[j];
       if (first) {
-        float2 v = *reinterpret_cast<const float2*>(at);
-        for (int k = 1; k < slices; ++k) {
-          const float2 o = *reinterpret_cast<const float2*>(at + (size_t)k * cols4);
-          lse2_add(v.x, v.y, o.x, o.y);
-        }
+        for (int k = 1; k < slices; ++k) lse2_add(v.x, v.y, red[(size_t)k * cols4 + j].x, red[(size_t)k * cols4 + j].y);
+        // u after it, in float64 in the slices' place: the next float32 potentials are relative to column 0's
         open[j] = v.y != 0.f;
-        next = v.y == 0.f ? 0.0 : shift + log_rows - ((double)v.x + log2((double)v.y));
+        reinterpret_cast<double*>(red)[j] =
+            v.y == 0.f ? 0.0 : shift - ((double)v.x + (double)log2f(v.y * per_rows));
       } else {
-        double k_j = 0.0;
-        for (int k = 0; k < slices; ++k) k_j += at[(size_t)k * cols4];
-        // the same float32 potential that the sums were formed with
-        const double before = (double)(float)(us[j] - shift) + shift;
+        for (int k = 1; k < slices; ++k) v.y += red[(size_t)k * cols4 + j].y;
         // (a sum that underflows, for masses beyond float32's range from one another, counts as 2^-126)
-        next = open[j] ? before + log_rows - log2(k_j == 0.0 ? 0x1p-126 : k_j) : 0.0;
+        const float step = log2f(v.y == 0.f ? 1.17549435e-38f : v.y * per_rows);
+        // the last potentials are not rounded to float32 before the common part goes back
+        if (last && blockIdx.x == 0) p.g[j] = open[j] ? (float)(((double)us[j] - (double)step + shift) * eps_per) : 0.f;
+        if (open[j]) us[j] -= step;
       }
-      us[j] = next;
     }
     __syncthreads();
+    if (first) {
+      const double* full = reinterpret_cast<const double*>(red);
+      const double base = full[0];
+      shift = fabs(base) < INFINITY ? base : 0.0;
+      for (int j = tid; j < cols; j += NT) {
+        us[j] = (float)(full[j] - shift);
+        if (last && blockIdx.x == 0) p.g[j] = (float)(full[j] * eps_per);
+      }
+      __syncthreads();
+    }
   }
-  if (blockIdx.x == 0)
-    for (int j = tid; j < cols; j += NT) p.g[j] = (float)(us[j] * eps_per);
 }
-
-size_t smem_bytes(int cols, int threads) { return exchange_bytes(cols, threads) + cols * (sizeof(double) + 1); }
 
 int columns_per_lane(int cols) {
   int c = 1;
@@ -358,29 +394,38 @@ int sm_count(int device) {
   return n;
 }
 
-// CTAs: one per SM, each with at least 128 rows.
-int balance_grid(int device, int rows) {
-  const int most = sm_count(device), want = (rows + 127) / 128;
+// CTAs: one for problems of few rows, else one per SM with at least 64 rows each.
+int balance_grid(int device, int rows, int cols) {
+  if ((long long)rows * columns_per_lane(cols) <= 1024) return 1;
+  const int most = sm_count(device), want = (rows + 63) / 64;
   return want < most ? want : most;
 }
 
 template <typename T, int C, int V>
 cudaError_t launch(int device, const BalanceProblem& p, const BalanceWork& wk, cudaStream_t stream) {
-  const size_t bytes = smem_bytes(p.cols, BalanceShape<C>::kThreads);
+  using Shape = BalanceShape<C>;
+  const int grid = balance_grid(device, p.rows, p.cols);
+  // the rows a CTA keeps: all of them, or what shared memory holds (227 KB less what the launch itself takes)
+  const size_t fixed = fixed_bytes(p.cols, Shape::kThreads), most = 226 * 1024 - fixed;
+  int kept = ((p.rows + grid - 1) / grid + Shape::kRows - 1) / Shape::kRows * Shape::kRows;
+  const int fits = (int)(most / row_bytes(p.cols, sizeof(T))) / Shape::kRows * Shape::kRows;
+  if (kept > fits) kept = fits;
+  if (p.iters == 1) kept = 0;
+  const size_t bytes = fixed + (size_t)kept * row_bytes(p.cols, sizeof(T));
   static std::atomic<int> done[kMaxDevices];
   cudaError_t e = smem_attr_once(reinterpret_cast<const void*>(balance_kernel<T, C, V>), (int)bytes, done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)balance_grid(device, p.rows));
-  cfg.blockDim = dim3(BalanceShape<C>::kThreads);
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(Shape::kThreads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeCooperative;                // its CTAs wait for one another
   attr.val.cooperative = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, balance_kernel<T, C, V>, p, wk);
+  cfg.numAttrs = grid > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, balance_kernel<T, C, V>, p, wk, kept);
 }
 
 template <typename T>
@@ -409,14 +454,16 @@ constexpr size_t kCounterBytes = 256;
 }  // namespace
 
 size_t balance_workspace_bytes(int device, int rows, int cols) {
-  return kCounterBytes + (size_t)4 * balance_grid(device, rows) * ((cols + 3) & ~3) * sizeof(float);
+  return kCounterBytes + (size_t)4 * balance_grid(device, rows, cols) * ((cols + 3) & ~3) * sizeof(float);
 }
 
 cudaError_t balance_launch(int device, int type, const BalanceProblem& p, void* ws, cudaStream_t stream) {
   BalanceWork wk{static_cast<unsigned*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes),
                  device_error_word()};
-  const cudaError_t e = cudaMemsetAsync(ws, 0, sizeof(unsigned), stream);
-  if (e != cudaSuccess) return e;
+  if (balance_grid(device, p.rows, p.cols) > 1) {
+    const cudaError_t e = cudaMemsetAsync(ws, 0, sizeof(unsigned), stream);
+    if (e != cudaSuccess) return e;
+  }
   switch (type) {
     case TRNOPT_F32: return launch<float>(device, p, wk, stream);
     case TRNOPT_F16: return launch<__half>(device, p, wk, stream);
