@@ -1,0 +1,431 @@
+// Sinkhorn on a score matrix: the potentials of the entropic transport plan
+//     P_ij = a_i b_j exp((f_i + g_j + S_ij) / eps)
+// between rows of mass a and columns of mass b, by the half-steps of the reference (src/trnopt/sinkhorn.py:108-119,
+// with the cost -S held as a matrix):
+//     f_i = -eps LSE_j(log b_j + (g_j + S_ij) / eps),   g_j = -eps LSE_i(log a_i + (f_i + S_ij) / eps).
+// A row or column without mass to exchange (all its terms zero) takes potential 0.
+//
+// Both half-steps of an iteration come from one exponential per score. In base 2, with c = log2 e / eps and the column
+// potentials u_j = g_j c, a row's terms are e_j = 2^(S_ij c + u_j - m_i) and its sum l_i = sum_j b_j e_j, so
+// f_i c = -(m_i + log2 l_i); the column sums k_j = sum_i a_i e_ij / l_i then give the next potentials,
+// u_j <- u_j - log2 k_j. After an iteration every column's k_j would be 1, so the next one's lies between the smallest
+// a_i / (row sum) and the largest, far from underflow; only the first iteration, from any g, keeps a running maximum per
+// column instead. Potentials are float32 relative to a column's after the first iteration (the common part, in float64,
+// goes back at the end): they are differences of a few units, where the potentials themselves may be hundreds.
+//
+// One cooperative launch runs all iterations. A CTA owns a block of rows and keeps as many of them as fit in shared
+// memory as they were read in the first pass (the rest come from L2 in every pass). L neighbouring lanes share a row, up
+// to 32 columns each, so a row's maximum and sum take log2 L shuffles for the warp's 32 / L rows together, and a lane
+// sums its columns over its rows in registers. Per iteration the CTAs exchange their column sums through global memory
+// and one grid barrier, and each adds up all of them in the same order. Bound by the exponentials (16 per clock and SM)
+// for many rows, by the barrier's latency for few; what one CTA takes in two steps of its warps stays in one, without it.
+#pragma once
+
+#include <math.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "score_types.cuh"
+#include "scores.h"
+
+namespace trnopt {
+
+namespace {
+
+constexpr unsigned kAll = 0xffffffffu;
+
+__device__ __forceinline__ void lse2_add(float& m, float& l, float om, float ol) {
+  const float n = om != om ? om : fmaxf(m, om);      // a NaN stays
+  if (n == -INFINITY) return;
+  l = l * exp2f(m - n) + ol * exp2f(om - n);
+  m = n;
+}
+
+// Arrive at the grid's barrier and wait until `target` arrivals have been made; false (on every thread) if that takes
+// longer than the bound on waits.
+__device__ __forceinline__ bool grid_barrier(unsigned* counter, unsigned target, int* error_word, int* flag) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory");
+    const unsigned long long t0 = globaltimer_ns();
+    int ok = 1;
+    unsigned seen;
+    for (;;) {
+      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
+      if (seen >= target) break;
+      if (globaltimer_ns() - t0 > kWaitLimitNs) {
+        atomicOr(error_word, (int)kErrWaitTimeout);
+        ok = 0;
+        break;
+      }
+    }
+    *flag = ok;
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+constexpr int NT = kBalanceThreads, NW = NT / 32;
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+struct Plus {
+  __device__ __forceinline__ float operator()(float x, float y) const { return x + y; }
+};
+struct Larger {
+  __device__ __forceinline__ float operator()(float x, float y) const { return fmaxf(x, y); }
+};
+
+// Shared memory: the warps' column sums, later the slices of the sum over the CTAs (NT quads), and the potentials; after
+// it the rows that are kept.
+__host__ __device__ inline size_t exchange_bytes(int cols) {
+  const size_t warps = (size_t)NW * cols * sizeof(float), slices = (size_t)NT * 4 * sizeof(float2);
+  return ((warps > slices ? warps : slices) + 15) & ~(size_t)15;
+}
+__host__ __device__ inline size_t fixed_bytes(int cols) {
+  return (exchange_bytes(cols) + cols * (3 * sizeof(float) + 1) + 15) & ~(size_t)15;
+}
+// A kept row: an odd number of 16-byte units, so that lanes on neighbouring rows meet different banks.
+__host__ __device__ inline int row_bytes(int cols, int size) { return (((cols * size + 15) >> 4) | 1) << 4; }
+
+// L lanes per row, C columns per lane in runs of V neighbouring ones.
+template <typename T, int L, int C, int V>
+__global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, BalanceWork wk, int kept_rows) {
+  constexpr int G = 32 / L;                                 // rows a warp takes at a time
+  extern __shared__ __align__(16) unsigned char smem[];
+  // the warps' column sums, then the slices of the sum over the CTAs; u + log2 b; log2 b; the CTA's column maxima in the
+  // first iteration; whether a column has any term; the kept rows
+  float* red = reinterpret_cast<float*>(smem);                      // (NW, cols)
+  float2* slice_sums = reinterpret_cast<float2*>(smem);             // (slices, cols4)
+  float* us = reinterpret_cast<float*>(smem + exchange_bytes(p.cols));
+  float *lb = us + p.cols, *peaks_s = lb + p.cols;
+  unsigned char* open = reinterpret_cast<unsigned char*>(peaks_s + p.cols);
+  T* kept = reinterpret_cast<T*>(smem + fixed_bytes(p.cols));       // (kept_rows, pitch)
+  __shared__ int flag;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, q = lane & (L - 1), group = lane / L;
+  const int cols = p.cols, cols4 = (cols + 3) & ~3, pitch = row_bytes(cols, sizeof(T)) / (int)sizeof(T);
+  const double per_eps = 1.4426950408889634 / p.eps, eps_per = p.eps * 0.6931471805599453;
+  const float c = (float)per_eps, per_rows = p.a ? 1.f : 1.f / (float)p.rows;
+  const long long r0 = (long long)blockIdx.x * p.rows / gridDim.x, r1 = (long long)(blockIdx.x + 1) * p.rows / gridDim.x;
+  const T* scores = static_cast<const T*>(p.scores) + r0 * p.ld + q * V;
+  const float* masses = p.a ? p.a + r0 : nullptr;
+  const int n = (int)(r1 - r0);
+  auto column = [&](int k) { return (k / V) * (L * V) + q * V + k % V; };
+
+  // what float32 potentials are relative to: 0, or the given potential of column 0; later its potential after one iteration
+  double shift = p.g0 && fabsf(p.g0[0]) < INFINITY ? (double)p.g0[0] * per_eps : 0.0;
+  bool some_closed = false;                                 // columns of mass 0: out of the rows' sums, log2 b = 0
+  for (int j = tid; j < cols; j += NT) {
+    const float b = p.b ? p.b[j] : 1.f;                     // (1 / cols each: log2 cols in a row's sum instead)
+    some_closed = some_closed || b == 0.f;
+    lb[j] = b == 0.f ? 0.f : log2f(b);
+    us[j] = (p.g0 ? (float)((double)p.g0[j] * per_eps - shift) : 0.f) + lb[j];
+  }
+  some_closed = __syncthreads_or(some_closed);
+  const float log_cols = p.b ? 0.f : log2f((float)cols);
+  unsigned closed = 0;                                      // the lane's columns of mass 0
+#pragma unroll
+  for (int k = 0; k < C; ++k)
+    if (column(k) < cols && p.b && p.b[column(k)] == 0.f) closed |= 1u << k;
+
+  for (int it = 0; it < p.iters; ++it) {
+    const bool first = it == 0, last = it == p.iters - 1;
+    float acc[C];
+    // Modes: 0 column sums; in the first iteration 1 the columns' maxima and then 2 their sums relative to those.
+    auto pass = [&](auto mode_, auto closed_) {
+      constexpr int kMode = decltype(mode_)::value;
+      constexpr bool kClosed = decltype(closed_)::value;
+      uint64_t u2[C / 2], acc2[C / 2];                      // pairs of columns
+#pragma unroll
+      for (int k = 0; k < C; k += 2) {
+        u2[k / 2] = pack2(column(k) < cols ? us[column(k)] : -INFINITY, column(k + 1) < cols ? us[column(k + 1)] : -INFINITY);
+        acc2[k / 2] = kMode == 1 ? pack2(-INFINITY, -INFINITY) : 0;
+      }
+      const uint64_t c2 = pack2(c, c);
+      for (int base = w * G; base < n; base += NW * G) {
+        const int row = base + group;
+        const bool there = row < n, keep = base + G <= kept_rows;
+        const T* s = scores + (there ? row : n - 1) * p.ld;
+        T* here = kept + (keep ? row * pitch + q * V : 0);
+        uint64_t z2[C / 2];
+        float m = -INFINITY, l = 0.f;
+        Vec<T> v[C / V];
+#pragma unroll
+        for (int r = 0; r < C / V; ++r) {                   // columns past the last: 0, with u = -inf
+          const int at = r * L * V;
+          v[r].q = make_uint4(0, 0, 0, 0);
+          if (at < cols && (L == 1 || at + q * V < cols)) {
+            if (kMode != 1 && keep) v[r] = read_any<V>(here + at);
+            else v[r] = read_global<V>(s + at);
+            if (kMode == 1 && keep) write_any<V>(here + at, v[r]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < C; k += 2) {
+          z2[k / 2] = fma2(pack2(v[k / V].get(k % V), v[(k + 1) / V].get((k + 1) % V)), c2, u2[k / 2]);
+          float x, y;
+          unpack2(z2[k / 2], x, y);
+          if (kClosed) {
+            x = closed >> k & 1 ? -INFINITY : x;
+            y = closed >> (k + 1) & 1 ? -INFINITY : y;
+          }
+          m = max3(m, x, y);
+        }
+#pragma unroll
+        for (int o = 1; o < L; o *= 2) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
+        m = m == -INFINITY ? 0.f : m;
+        {
+          const uint64_t m2 = pack2(-m, -m);
+          uint64_t l2 = 0;
+#pragma unroll
+          for (int k = 0; k < C; k += 2) {
+            const uint64_t d2 = add2(z2[k / 2], m2);
+            float x, y;
+            unpack2(d2, x, y);
+            const float ex = ex2_approx(x), ey = ex2_approx(y);
+            const uint64_t e2 = pack2(ex, ey);
+            if (kClosed) l2 = add2(pack2(closed >> k & 1 ? 0.f : ex, closed >> (k + 1) & 1 ? 0.f : ey), l2);
+            else l2 = add2(e2, l2);
+            z2[k / 2] = kMode == 0 ? e2 : d2;
+          }
+          float x, y;
+          unpack2(l2, x, y);
+          l = x + y;
+        }
+#pragma unroll
+        for (int o = 1; o < L; o *= 2) l += __shfl_xor_sync(kAll, l, o);
+        const float a = !there ? 0.f : masses ? __ldg(masses + row) : 1.f;
+        const bool empty = l == 0.f;                        // f = 0: the terms 2^(S c + u) as they are
+        if (kMode != 1 && last && q == 0 && there)
+          p.f[r0 + row] = empty ? 0.f : (float)(((double)log_cols - ((double)m + (double)log2f(l) + shift)) * eps_per);
+        if constexpr (kMode == 0) {
+          if (!__any_sync(kAll, empty && a != 0.f)) {
+            const float weight = empty ? 0.f : __fdividef(a, l);
+            const uint64_t w2 = pack2(weight, weight);
+#pragma unroll
+            for (int k = 0; k < C / 2; ++k) acc2[k] = fma2(z2[k], w2, acc2[k]);
+          } else if (a != 0.f) {
+#pragma unroll
+            for (int k = 0; k < C; k += 2) {
+              float x, y;
+              unpack2(z2[k / 2], x, y);
+              auto term = [&](float e) {
+                return !empty ? e * __fdividef(a, l) : e > 0.f ? a * exp2f(log2f(e) + ((float)shift - log_cols)) : 0.f;
+              };
+              acc2[k / 2] = add2(acc2[k / 2], pack2(term(x), term(y)));
+            }
+          }
+        } else {
+          // x = S c + f c + log2 a, in the gauge of u - shift: z - u - log2 l + log2 a (and log2 cols, as in mode 0)
+          const float off = (empty ? (float)shift - log_cols : -log2f(l)) + log2f(a);
+#pragma unroll
+          for (int k = 0; k < C; k += 2) {
+            float zx, zy, ux, uy, ax, ay;
+            unpack2(z2[k / 2], zx, zy);
+            unpack2(u2[k / 2], ux, uy);
+            unpack2(acc2[k / 2], ax, ay);
+            auto term = [&](float z, float u, float acc, int j) {
+              if (j >= cols) return acc;
+              const float x = z - u + off;
+              return kMode == 1 ? fmaxf(acc, x) : acc + ex2_approx(x - peaks_s[j]);
+            };
+            acc2[k / 2] = pack2(term(zx, ux, ax, column(k)), term(zy, uy, ay, column(k + 1)));
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < C; k += 2) unpack2(acc2[k / 2], acc[k], acc[k + 1]);
+    };
+    // Over the warp's groups (a lane gives half of its columns away at each step, while it has several), then to `red`.
+    auto fold = [&](auto op) {
+      int from = 0, have = C;
+#pragma unroll
+      for (int o = L; o < 32; o *= 2) {
+        if (have > 1) {
+          const bool upper = lane & o;
+          have /= 2;
+#pragma unroll
+          for (int k = 0; k < C / 2; ++k)
+            if (k < have) {
+              const float give = upper ? acc[k] : acc[k + have], held = upper ? acc[k + have] : acc[k];
+              acc[k] = op(held, __shfl_xor_sync(kAll, give, o));
+            }
+          from += upper ? have : 0;
+        } else {
+          acc[0] = op(acc[0], __shfl_xor_sync(kAll, acc[0], o));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < C; ++k)
+        if (k < have && column(from + k) < cols) red[w * cols + column(from + k)] = acc[k];
+      __syncthreads();
+    };
+    if (first) {
+      pass(std::integral_constant<int, 1>{}, std::true_type{});
+      fold(Larger{});
+      for (int j = tid; j < cols; j += NT) {
+        float m = red[j];
+        for (int k = 1; k < NW; ++k) m = fmaxf(m, red[k * cols + j]);
+        peaks_s[j] = fabsf(m) < INFINITY ? m : 0.f;
+      }
+      __syncthreads();
+      pass(std::integral_constant<int, 2>{}, std::true_type{});
+    } else if (some_closed) {
+      pass(std::integral_constant<int, 0>{}, std::true_type{});
+    } else {
+      pass(std::integral_constant<int, 0>{}, std::false_type{});
+    }
+    fold(Plus{});
+
+    const bool alone = gridDim.x == 1;
+    const size_t plane = (size_t)gridDim.x * cols4;
+    float* sums = wk.parts + (size_t)(it & 1) * 2 * plane;
+    float* peaks = sums + plane;
+    for (int j = tid; j < cols; j += NT) {
+      float v = red[j];
+#pragma unroll
+      for (int k = 1; k < NW; ++k) v += red[k * cols + j];
+      if (alone) {
+        red[j] = v;                                         // (column j of `red` is this thread's alone)
+      } else {
+        __stcg(sums + (size_t)blockIdx.x * cols4 + j, v);
+        if (first) __stcg(peaks + (size_t)blockIdx.x * cols4 + j, v == 0.f ? -INFINITY : peaks_s[j]);
+      }
+    }
+    int slices = 1;
+    if (!alone) {
+      if (!grid_barrier(wk.counter, (unsigned)(it + 1) * gridDim.x, wk.error_word, &flag)) {
+        // gave up: no potentials
+        for (long long i = r0 + tid; i < r1; i += NT) p.f[i] = NAN;
+        if (blockIdx.x == 0)
+          for (int j = tid; j < cols; j += NT) p.g[j] = NAN;
+        return;
+      }
+      // of all CTAs, in the same order in each: four columns per thread, the CTAs in `slices` interleaved parts
+      const int quads = cols4 / 4, slice = tid / quads, quad = tid - slice * quads;
+      slices = NT / quads;
+      float2* part = slice_sums + (size_t)slice * cols4 + 4 * quad;     // (`red` is free again)
+      if (slice < slices) {
+        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (first) {
+#pragma unroll 4
+          for (int k = slice; k < (int)gridDim.x; k += slices) {
+            const float4 om = __ldcg(reinterpret_cast<const float4*>(peaks + (size_t)k * cols4) + quad);
+            const float4 ol = __ldcg(reinterpret_cast<const float4*>(sums + (size_t)k * cols4) + quad);
+            lse2_add(m[0], v[0], om.x, ol.x);
+            lse2_add(m[1], v[1], om.y, ol.y);
+            lse2_add(m[2], v[2], om.z, ol.z);
+            lse2_add(m[3], v[3], om.w, ol.w);
+          }
+        } else {
+#pragma unroll 16
+          for (int k = slice; k < (int)gridDim.x; k += slices) {
+            const float4 o = __ldcg(reinterpret_cast<const float4*>(sums + (size_t)k * cols4) + quad);
+            v[0] += o.x;
+            v[1] += o.y;
+            v[2] += o.z;
+            v[3] += o.w;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[e] = make_float2(m[e], v[e]);
+      }
+      __syncthreads();
+    }
+    double full[2];                                         // first iteration: u of the thread's columns (at most 2)
+    double* base = reinterpret_cast<double*>(&slice_sums[0]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int j = tid + i * NT;
+      if (j >= cols) break;
+      float2 v = alone ? make_float2(peaks_s[j], red[j]) : slice_sums[j];
+      if (first) {
+        for (int k = 1; k < slices; ++k) lse2_add(v.x, v.y, slice_sums[(size_t)k * cols4 + j].x, slice_sums[(size_t)k * cols4 + j].y);
+        open[j] = v.y != 0.f;
+        full[i] = v.y == 0.f ? 0.0 : shift - ((double)v.x + (double)log2f(v.y * per_rows) + (double)log_cols);
+      } else {
+        for (int k = 1; k < slices; ++k) v.y += slice_sums[(size_t)k * cols4 + j].y;
+        // k_j (a sum that underflows, for masses beyond float32's range from one another, counts as 2^-126)
+        const float step = log2f(v.y == 0.f ? 1.17549435e-38f : v.y * per_rows) - (lb[j] - log_cols);
+        // the last potentials are not rounded to float32 before the common part goes back
+        if (last && blockIdx.x == 0)
+          p.g[j] = open[j] ? (float)(((double)us[j] - (double)lb[j] - (double)step + shift) * eps_per) : 0.f;
+        if (open[j]) us[j] -= step;
+      }
+    }
+    if (first) {
+      __syncthreads();
+      if (tid == 0) base[0] = full[0];
+      __syncthreads();
+      shift = fabs(base[0]) < INFINITY ? base[0] : 0.0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int j = tid + i * NT;
+        if (j >= cols) break;
+        us[j] = (float)(full[i] - shift) + lb[j];
+        if (last && blockIdx.x == 0) p.g[j] = (float)(full[i] * eps_per);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int L, int C, int V>
+cudaError_t launch(int device, const BalanceProblem& p, const BalanceWork& wk, cudaStream_t stream) {
+  const int grid = balance_grid(device, p.rows, p.cols);
+  // the rows a CTA keeps: all of them, or what shared memory holds (227 KB less what the launch itself takes)
+  constexpr int G = 32 / L;
+  const size_t fixed = fixed_bytes(p.cols), most = 226 * 1024 - fixed;
+  long long kept = ((p.rows + grid - 1) / grid + G - 1) / G * (long long)G;
+  const long long fits = (long long)(most / row_bytes(p.cols, sizeof(T))) / G * G;
+  if (kept > fits) kept = fits;
+  const size_t bytes = fixed + (size_t)kept * row_bytes(p.cols, sizeof(T));
+  static std::atomic<int> done[kMaxDevices];
+  cudaError_t e = smem_attr_once(reinterpret_cast<const void*>(balance_kernel<T, L, C, V>), (int)bytes, done);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeCooperative;                // its CTAs wait for one another
+  attr.val.cooperative = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = grid > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, balance_kernel<T, L, C, V>, p, wk, (int)kept);
+}
+
+template <typename T, int L, int C>
+cudaError_t launch(int device, const BalanceProblem& p, const BalanceWork& wk, cudaStream_t stream) {
+  // the longest runs of columns per lane that the sizes and addresses allow: 16 bytes, 8, or single scores
+  auto runs = [&](int v) {
+    return p.cols % v == 0 && p.ld % v == 0 && reinterpret_cast<uintptr_t>(p.scores) % (v * sizeof(T)) == 0;
+  };
+  if constexpr (sizeof(T) == 2)
+    if (runs(8)) return launch<T, L, C, 8>(device, p, wk, stream);
+  return runs(4) ? launch<T, L, C, 4>(device, p, wk, stream) : launch<T, L, C, 1>(device, p, wk, stream);
+}
+
+template <typename T>
+cudaError_t launch(int device, const BalanceProblem& p, const BalanceWork& wk, cudaStream_t stream) {
+  switch (lanes_per_row(p.cols)) {
+    case 1: return p.cols <= 8 ? launch<T, 1, 8>(device, p, wk, stream)
+                               : p.cols <= 16 ? launch<T, 1, 16>(device, p, wk, stream) : launch<T, 1, 32>(device, p, wk, stream);
+    case 2: return launch<T, 2, 32>(device, p, wk, stream);
+    case 4: return launch<T, 4, 32>(device, p, wk, stream);
+    case 8: return launch<T, 8, 32>(device, p, wk, stream);
+    case 16: return launch<T, 16, 32>(device, p, wk, stream);
+    default: return launch<T, 32, 32>(device, p, wk, stream);
+  }
+}
+
+}  // namespace
+
+}  // namespace trnopt

@@ -45,6 +45,13 @@ struct BalanceProblem {
   float *f, *g;
 };
 
+struct BalanceWork {
+  unsigned* counter;       // arrivals at the barrier, 0 at the start
+  float* parts;            // (2, 2, CTAs, cols rounded up to 4): by parity, the CTAs' column sums, and their maxima in the
+                           // first iteration
+  int* error_word;
+};
+
 struct RouteProblem {
   const void* scores;
   long long ld, rows;
@@ -70,6 +77,17 @@ struct RouteGradProblem {
 
 cudaError_t log_probs_launch(int type, const LogProbsProblem& p, cudaStream_t stream);
 cudaError_t log_probs_grad_launch(int type, const LogProbsGradProblem& p, cudaStream_t stream);
+// balance, by the scores' type (score_balance_f32.cu, ...: one file each, for the compiler's time)
+cudaError_t balance_launch_f32(int device, const BalanceProblem& p, const BalanceWork& wk, cudaStream_t stream);
+cudaError_t balance_launch_f16(int device, const BalanceProblem& p, const BalanceWork& wk, cudaStream_t stream);
+cudaError_t balance_launch_bf16(int device, const BalanceProblem& p, const BalanceWork& wk, cudaStream_t stream);
+int balance_grid(int device, int rows, int cols);     // its CTAs
+constexpr int kBalanceThreads = 512;
+inline int lanes_per_row(int cols) {
+  int l = 1;
+  while (32 * l < cols) l *= 2;
+  return l;
+}
 size_t balance_workspace_bytes(int device, int rows, int cols);
 cudaError_t balance_launch(int device, int type, const BalanceProblem& p, void* ws, cudaStream_t stream);
 cudaError_t route_launch(int type, const RouteProblem& p, cudaStream_t stream);
