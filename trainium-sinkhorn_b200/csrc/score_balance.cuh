@@ -89,12 +89,14 @@ __host__ __device__ inline size_t exchange_bytes(int cols) {
   return ((warps > slices ? warps : slices) + 15) & ~(size_t)15;
 }
 __host__ __device__ inline size_t fixed_bytes(int cols) {
-  return (exchange_bytes(cols) + cols * (3 * sizeof(float) + 1) + 15) & ~(size_t)15;
+  const size_t pad = (size_t)lanes_per_row(cols) * 32;
+  return (exchange_bytes(cols) + 2 * pad * sizeof(float) + cols * (sizeof(float) + 1) + 15) & ~(size_t)15;
 }
 // A kept row: an odd number of 16-byte units, so that lanes on neighbouring rows meet different banks.
 __host__ __device__ inline int row_bytes(int cols, int size) { return (((cols * size + 15) >> 4) | 1) << 4; }
 
 // L lanes per row, C columns per lane in runs of V neighbouring ones.
+// (C is 32, or 8 or 16 where a row of few columns has a lane of its own; u has places for 32 either way.)
 template <typename T, int L, int C, int V>
 __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, BalanceWork wk, int kept_rows) {
   constexpr int G = 32 / L;                                 // rows a warp takes at a time
@@ -104,8 +106,8 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
   float* red = reinterpret_cast<float*>(smem);                      // (NW, cols)
   float2* slice_sums = reinterpret_cast<float2*>(smem);             // (slices, cols4)
   float* us = reinterpret_cast<float*>(smem + exchange_bytes(p.cols));
-  float *lb = us + p.cols, *peaks_s = lb + p.cols;
-  unsigned char* open = reinterpret_cast<unsigned char*>(peaks_s + p.cols);
+  float *peaks_s = us + L * 32, *lb = peaks_s + L * 32;             // (u and the maxima have L x 32 places: -inf, 0)
+  unsigned char* open = reinterpret_cast<unsigned char*>(lb + p.cols);
   T* kept = reinterpret_cast<T*>(smem + fixed_bytes(p.cols));       // (kept_rows, pitch)
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, q = lane & (L - 1), group = lane / L;
@@ -127,6 +129,10 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
     lb[j] = b == 0.f ? 0.f : log2f(b);
     us[j] = (p.g0 ? (float)((double)p.g0[j] * per_eps - shift) : 0.f) + lb[j];
   }
+  for (int j = tid; j < L * 32; j += NT) {
+    if (j >= cols) us[j] = -INFINITY;
+    peaks_s[j] = 0.f;
+  }
   some_closed = __syncthreads_or(some_closed);
   const float log_cols = p.b ? 0.f : log2f((float)cols);
   unsigned closed = 0;                                      // the lane's columns of mass 0
@@ -144,7 +150,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
       uint64_t u2[C / 2], acc2[C / 2];                      // pairs of columns
 #pragma unroll
       for (int k = 0; k < C; k += 2) {
-        u2[k / 2] = pack2(column(k) < cols ? us[column(k)] : -INFINITY, column(k + 1) < cols ? us[column(k + 1)] : -INFINITY);
+        u2[k / 2] = pack2(us[column(k)], us[column(k + 1)]);
         acc2[k / 2] = kMode == 1 ? pack2(-INFINITY, -INFINITY) : 0;
       }
       const uint64_t c2 = pack2(c, c);
@@ -231,8 +237,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
             unpack2(u2[k / 2], ux, uy);
             unpack2(acc2[k / 2], ax, ay);
             auto term = [&](float z, float u, float acc, int j) {
-              if (j >= cols) return acc;
-              const float x = z - u + off;
+              const float x = u == -INFINITY ? -INFINITY : z - u + off;      // (a column past the last, or closed by g)
               return kMode == 1 ? fmaxf(acc, x) : acc + ex2_approx(x - peaks_s[j]);
             };
             acc2[k / 2] = pack2(term(zx, ux, ax, column(k)), term(zy, uy, ay, column(k + 1)));
@@ -309,7 +314,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
       }
       // of all CTAs, in the same order in each: four columns per thread, the CTAs in `slices` interleaved parts
       const int quads = cols4 / 4, slice = tid / quads, quad = tid - slice * quads;
-      slices = NT / quads;
+      slices = min(NT / quads, 16);                         // (few enough for the columns' threads to join)
       float2* part = slice_sums + (size_t)slice * cols4 + 4 * quad;     // (`red` is free again)
       if (slice < slices) {
         float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -324,13 +329,22 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
             lse2_add(m[3], v[3], om.w, ol.w);
           }
         } else {
-#pragma unroll 16
-          for (int k = slice; k < (int)gridDim.x; k += slices) {
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(sums + (size_t)k * cols4) + quad);
-            v[0] += o.x;
-            v[1] += o.y;
-            v[2] += o.z;
-            v[3] += o.w;
+          constexpr int kBatch = 10;                        // loads in flight (148 CTAs in 16 slices: one round)
+          for (int k0 = slice; k0 < (int)gridDim.x; k0 += slices * kBatch) {
+            float4 o[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+              const int k = k0 + i * slices;
+              o[i] = k < (int)gridDim.x ? __ldcg(reinterpret_cast<const float4*>(sums + (size_t)k * cols4) + quad)
+                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+              v[0] += o[i].x;
+              v[1] += o[i].y;
+              v[2] += o[i].z;
+              v[3] += o[i].w;
+            }
           }
         }
 #pragma unroll
@@ -350,6 +364,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
         open[j] = v.y != 0.f;
         full[i] = v.y == 0.f ? 0.0 : shift - ((double)v.x + (double)log2f(v.y * per_rows) + (double)log_cols);
       } else {
+#pragma unroll 8
         for (int k = 1; k < slices; ++k) v.y += slice_sums[(size_t)k * cols4 + j].y;
         // k_j (a sum that underflows, for masses beyond float32's range from one another, counts as 2^-126)
         const float step = log2f(v.y == 0.f ? 1.17549435e-38f : v.y * per_rows) - (lb[j] - log_cols);

@@ -83,7 +83,7 @@ cudaError_t balance_launch_f16(int device, const BalanceProblem& p, const Balanc
 cudaError_t balance_launch_bf16(int device, const BalanceProblem& p, const BalanceWork& wk, cudaStream_t stream);
 int balance_grid(int device, int rows, int cols);     // its CTAs
 constexpr int kBalanceThreads = 512;
-inline int lanes_per_row(int cols) {
+__host__ __device__ inline int lanes_per_row(int cols) {
   int l = 1;
   while (32 * l < cols) l *= 2;
   return l;
