@@ -554,6 +554,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) log_probs_grad_kernel(LogProbsG
   const T* s = static_cast<const T*>(p.scores) + row * p.ld;
   T* out = static_cast<T*>(p.grad) + row * p.ld_grad;
   const RowVectors<T> rv(out, p.cols);
+  if (v0 >= rv.count) return;
   const long long v1 = min(rv.count, v0 + (long long)chunks * kChunk);
   const long long first = rv.column(v0), end = rv.column(v1);                   // the CTA's columns
   const bool vectors = (reinterpret_cast<uintptr_t>(s + first) & 15) == 0;     // the scores' vectors fall together
@@ -732,10 +733,12 @@ cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
 template <typename T, int NT>
 cudaError_t grad_launch(const LogProbsGradProblem& p, cudaStream_t stream) {
   constexpr long long kCols = (long long)NT * LP_VECS * Vec<T>::kN;
-  const long long all = (p.cols + Vec<T>::kN - 1 + kCols - 1) / kCols;         // (a row may start inside a vector)
-  // up to 4 chunks per CTA, which share the row's numbers, while there are CTAs for every SM's 4 places
+  // (a row may start inside a vector, and then reach into one more chunk)
+  const bool aligned = p.ld_grad % Vec<T>::kN == 0 && reinterpret_cast<uintptr_t>(p.grad) % 16 == 0;
+  const long long all = (p.cols + (aligned ? 0 : Vec<T>::kN - 1) + kCols - 1) / kCols;
+  // up to 4 chunks per CTA, which share the row's numbers, while there are CTAs for 6 rounds of the SMs' 4 places
   int chunks = 1;
-  while (chunks < 4 && chunks < all && p.rows * ((all + 2 * chunks - 1) / (2 * chunks)) >= 148 * 8) chunks *= 2;
+  while (chunks < 4 && chunks < all && p.rows * ((all + 2 * chunks - 1) / (2 * chunks)) >= 148 * 24) chunks *= 2;
   const int parts = (int)((all + chunks - 1) / chunks);
   const long long per = (1LL << 30) / parts;
   const size_t size = sizeof(typename Acc<T>::type);
