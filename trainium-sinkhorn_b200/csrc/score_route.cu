@@ -8,10 +8,18 @@
 //     weight = scale * share, or scale * share / sum of the chosen shares
 // Columns of score -inf or biased key -inf are closed. Slots that no open column fills hold index -1 and weight 0. A
 // row holding NaN or +inf chooses nothing: index -1, weight NaN.
-// The order of keys is a comparison of values that may be a few float32 steps apart, so keys are float64; the weights
-// are float32 from the logarithms of the shares (shares that underflow still give their ratio). One warp per row.
+// The order of keys is that of their 64-bit values. One warp per row holds float32 keys in registers, a run of columns
+// per lane within a group, and takes the best one `top` + 1 times (two warp reductions each). Where neighbours in that
+// order, or the last open and the first closed group, are closer than the float32 keys are exact, and not equal in score
+// and bias, the row is done again in float64 through shared memory (a few rows in a thousand). Keys that are the scores
+// themselves are exact. Weights are float32 from the logarithms of the shares (shares that underflow still give their
+// ratio). A persistent grid counts the load in shared memory. Bound by the selection's instructions.
 #include <math.h>
 
+#include <atomic>
+
+#include "common.cuh"
+#include "kernels.h"
 #include "score_types.cuh"
 #include "scores.h"
 
@@ -19,10 +27,14 @@ namespace trnopt {
 
 namespace {
 
-constexpr int RT_WARPS = 4;
-constexpr int RT_MAX_COLS = 1024;
+constexpr int RT_WARPS = 8;
 constexpr unsigned kAll = 0xffffffffu;
 
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "r"(kAll));
+  return r;
+}
 __device__ __forceinline__ double warp_max(double v) {
   for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(kAll, v, o));
   return v;
@@ -44,119 +56,291 @@ __device__ __forceinline__ void warp_best(double& v, int& j) {
 // log sigmoid(x), exact for large |x|
 __device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.f) - log1pf(expf(-fabsf(x))); }
 
+// Whole numbers in the order of the scores (-0 = +0); 0 is below every score's.
+__device__ __forceinline__ uint32_t order(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+
+// A row's choices by 64-bit keys in shared memory: lane k < top gets the k-th column, or -1.
 template <typename T>
-__global__ void __launch_bounds__(32 * RT_WARPS) route_kernel(RouteProblem p) {
-  __shared__ double keys[RT_WARPS][RT_MAX_COLS];
+__device__ __noinline__ int choose_exact(const RouteProblem& p, const T* s, double* key) {
+  const int lane = threadIdx.x & 31, size = p.cols / p.groups;
+  double m = -INFINITY, sum = 0.0;
+  for (int j = lane; j < p.cols; j += 32) m = fmax(m, (double)widen(s[j]));
+  m = warp_max(m);
+  if (p.kind == TRNOPT_ROUTE_SOFTMAX && m > -INFINITY) {
+    for (int j = lane; j < p.cols; j += 32) sum += exp((double)widen(s[j]) - m);
+    sum = warp_sum(sum);
+  }
+  const bool on_scores = p.bias && p.bias_on == TRNOPT_ROUTE_BIAS_SCORES;
+  auto share = [&](double x) { return p.kind == TRNOPT_ROUTE_SOFTMAX ? exp(x - m) / sum : 1.0 / (1.0 + exp(-x)); };
+  for (int j = lane; j < p.cols; j += 32) {
+    const double x = widen(s[j]);
+    double k = x;
+    if (x > -INFINITY) {
+      if (on_scores || (p.groups > 1 && !p.bias)) k = share(x);
+      if (p.bias) k += (double)p.bias[j];
+    }
+    key[j] = k;
+  }
+  __syncwarp();
+  if (p.groups > 1) {
+    // lane g scores group g, then ranks it among all
+    double top1 = -INFINITY, top2 = -INFINITY;
+    if (lane < p.groups)
+      for (int j = lane * size; j < (lane + 1) * size; ++j) {
+        const double k = key[j];
+        if (k > top1) { top2 = top1; top1 = k; }
+        else if (k > top2) top2 = k;
+      }
+    const bool alive = top1 > -INFINITY;
+    const double score = p.group_top == 2 && top2 > -INFINITY ? top1 + top2 : top1;
+    int rank = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const double other = __shfl_sync(kAll, score, g);
+      const bool other_alive = __shfl_sync(kAll, alive, g);
+      rank += other_alive && (other > score || (other == score && g < lane));
+    }
+    __syncwarp();
+    const unsigned open = __ballot_sync(kAll, lane < p.groups && alive && rank < p.top_groups);
+    for (int j = lane; j < p.cols; j += 32) {
+      if (!((open >> (j / size)) & 1)) key[j] = -INFINITY;
+      else if (!p.bias) key[j] = widen(s[j]);              // without a bias the columns go by their scores themselves
+    }
+    __syncwarp();
+  }
+  int mine = -1;
+  for (int k = 0; k < p.top; ++k) {
+    double v = -INFINITY;
+    int j = -1;
+    for (int c = lane; c < p.cols; c += 32)
+      if (key[c] > v) { v = key[c]; j = c; }
+    warp_best(v, j);
+    if (j < 0) break;
+    if (lane == k) mine = j;
+    if (lane == (j & 31)) key[j] = -INFINITY;
+    __syncwarp();
+  }
+  __syncwarp();
+  return mine;
+}
+
+// How the columns lie on the lanes: `lanes` (a power of two) for each group, `run` neighbouring columns on each.
+struct RouteLayout {
+  int lanes, run, size;
+  bool vectors;                // runs are whole 16-byte (or shorter) vectors on their boundaries
+  bool exact;                  // no such layout (or float64 asked for): every row by 64-bit keys
+};
+
+template <typename T, int C>
+__global__ void __launch_bounds__(32 * RT_WARPS) route_kernel(RouteProblem p, RouteLayout lay) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  double* keys = reinterpret_cast<double*>(smem);                  // (RT_WARPS, cols), for rows by 64-bit keys
+  int* counts = reinterpret_cast<int*>(keys + (size_t)RT_WARPS * p.cols);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int size = p.cols / p.groups;
-  double* key = keys[w];
+  const int group = lane / lay.lanes, in_group = (lane & (lay.lanes - 1)) * lay.run;
+  const int first = group * lay.size + in_group;                    // the lane's columns: first + k, k < mine_n
+  const int mine_n = group < p.groups ? max(0, min(lay.run, lay.size - in_group)) : 0;
+  const bool softmax = p.kind == TRNOPT_ROUTE_SOFTMAX, on_scores = p.bias && p.bias_on == TRNOPT_ROUTE_BIAS_SCORES;
+  const bool shares = on_scores || (p.groups > 1 && !p.bias);       // the choice looks at shares
+  if (p.load) {
+    for (int j = threadIdx.x; j < p.cols; j += 32 * RT_WARPS) counts[j] = 0;
+    __syncthreads();
+  }
+  float bias[C];
+  bool bad_bias = false;
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    bias[k] = p.bias && k < mine_n ? p.bias[first + k] : 0.f;
+    bad_bias = bad_bias || bias[k] != bias[k];
+  }
+  if (lay.exact && p.bias)
+    for (int j = lane; j < p.cols; j += 32) bad_bias = bad_bias || p.bias[j] != p.bias[j];
+  bad_bias = __any_sync(kAll, bad_bias);
+
   for (long long row = (long long)blockIdx.x * RT_WARPS + w; row < p.rows; row += (long long)gridDim.x * RT_WARPS) {
     const T* s = static_cast<const T*>(p.scores) + row * p.ld;
-    double m = -INFINITY, sum = 0.0;
-    bool bad = false;
-    for (int j = lane; j < p.cols; j += 32) {
-      const float x = widen(s[j]);
-      bad = bad || !(x < INFINITY) || (p.bias && p.bias[j] != p.bias[j]);
-      m = fmax(m, (double)x);
+    float x[C];
+    if (lay.vectors) {
+      constexpr int kV = C < Vec<T>::kN ? C : Vec<T>::kN;
+#pragma unroll
+      for (int k = 0; k < C; k += kV) {
+        if (mine_n > 0) {
+          const Vec<T> v = read_global<kV>(s + first + k);
+#pragma unroll
+          for (int i = 0; i < kV; ++i) x[k + i] = v.get(i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kV; ++i) x[k + i] = -INFINITY;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < C; ++k) x[k] = k < mine_n ? widen(s[first + k]) : -INFINITY;
     }
-    bad = __any_sync(kAll, bad);
+    float m = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      bad = bad || !(x[k] < INFINITY);
+      m = fmaxf(m, x[k]);
+    }
+    if (lay.exact)                                          // (the registers hold the first columns only)
+      for (int j = lane; j < p.cols; j += 32) {
+        const float v = widen(s[j]);
+        bad = bad || !(v < INFINITY);
+        m = fmaxf(m, v);
+      }
+    bad = __any_sync(kAll, bad) || bad_bias;
     m = warp_max(m);
-    if (p.kind == TRNOPT_ROUTE_SOFTMAX && m > -INFINITY) {
-      for (int j = lane; j < p.cols; j += 32) sum += exp((double)widen(s[j]) - m);
+    float sum = 0.f;
+    if (softmax && (shares || !p.renormalize)) {
+#pragma unroll
+      for (int k = 0; k < C; ++k) sum += x[k] > -INFINITY ? ex2_approx((x[k] - m) * kLog2e) : 0.f;
+      if (lay.exact) {
+        sum = 0.f;
+        for (int j = lane; j < p.cols; j += 32) sum += widen(s[j]) > -INFINITY ? ex2_approx((widen(s[j]) - m) * kLog2e) : 0.f;
+      }
       sum = warp_sum(sum);
     }
-    const bool on_scores = p.bias && p.bias_on == TRNOPT_ROUTE_BIAS_SCORES;
-    auto share = [&](double x) { return p.kind == TRNOPT_ROUTE_SOFTMAX ? exp(x - m) / sum : 1.0 / (1.0 + exp(-x)); };
-    if (!bad) {
-      for (int j = lane; j < p.cols; j += 32) {
-        const double x = widen(s[j]);
-        double k = x;
-        if (x > -INFINITY) {
-          if (on_scores || (p.groups > 1 && !p.bias)) k = share(x);
-          if (p.bias) k += (double)p.bias[j];
-        }
-        key[j] = k;
+
+    int mine = -1;                                          // lane k < top: the k-th choice
+    bool exact = lay.exact;
+    if (!bad && !exact) {
+      // keys, and how far two of them may be apart in float32 and still be in the other order in 64 bits: shares are off
+      // by 2^-21 of themselves (2^-20 for a softmax, with its sum), a sum with a bias by 2^-24 of itself
+      float key[C], tol = 0.f;
+      const float per_sum = softmax && shares ? 1.f / sum : 0.f;
+#pragma unroll
+      for (int k = 0; k < C; ++k) {
+        key[k] = x[k];
+        if (shares) key[k] = softmax ? ex2_approx((x[k] - m) * kLog2e) * per_sum : __fdividef(1.f, 1.f + ex2_approx(-x[k] * kLog2e));
+        if (p.bias) key[k] += bias[k];
+        if (x[k] == -INFINITY) key[k] = -INFINITY;
+        if (p.bias && key[k] > -INFINITY) tol = fmaxf(tol, fabsf(key[k]));
       }
-      __syncwarp();
+      if (shares || p.bias) tol = 2.4e-7f * warp_max(tol) + (shares ? 4e-6f * (softmax ? per_sum : 1.f) : 0.f);
       if (p.groups > 1) {
-        // lane g scores group g, then ranks it among all
-        double top1 = -INFINITY, top2 = -INFINITY;
-        if (lane < p.groups)
-          for (int j = lane * size; j < (lane + 1) * size; ++j) {
-            const double k = key[j];
-            if (k > top1) { top2 = top1; top1 = k; }
-            else if (k > top2) top2 = k;
-          }
-        const bool alive = top1 > -INFINITY;
-        const double score = p.group_top == 2 && top2 > -INFINITY ? top1 + top2 : top1;
+        float t1 = -INFINITY, t2 = -INFINITY;               // the group's two best, over its lanes
+#pragma unroll
+        for (int k = 0; k < C; ++k) {
+          t2 = fmaxf(t2, fminf(t1, key[k]));
+          t1 = fmaxf(t1, key[k]);
+        }
+        for (int o = 1; o < lay.lanes; o *= 2) {
+          const float o1 = __shfl_xor_sync(kAll, t1, o), o2 = __shfl_xor_sync(kAll, t2, o);
+          t2 = fmaxf(fminf(t1, o1), fmaxf(t2, o2));
+          t1 = fmaxf(t1, o1);
+        }
+        const bool alive = t1 > -INFINITY;
+        const float score = p.group_top == 2 && t2 > -INFINITY ? t1 + t2 : t1;
         int rank = 0;
         for (int g = 0; g < p.groups; ++g) {
-          const double other = __shfl_sync(kAll, score, g);
-          const bool other_alive = __shfl_sync(kAll, alive, g);
-          rank += other_alive && (other > score || (other == score && g < lane));
+          const float other = __shfl_sync(kAll, score, g * lay.lanes);        // (-inf: nothing open there)
+          rank += other > score || (other == score && g < group);
         }
-        __syncwarp();
-        const unsigned open = __ballot_sync(kAll, lane < p.groups && alive && rank < p.top_groups);
-        for (int j = lane; j < p.cols; j += 32) {
-          if (!((open >> (j / size)) & 1)) key[j] = -INFINITY;
-          else if (!p.bias) key[j] = widen(s[j]);        // without a bias the columns go by their scores themselves
+        const bool open = alive && rank < p.top_groups;
+        const float lowest = -warp_max(open ? -score : -INFINITY), highest = warp_max(open || !alive ? -INFINITY : score);
+        exact = lowest - highest <= 3.f * tol + 2.4e-7f * fabsf(lowest);
+#pragma unroll
+        for (int k = 0; k < C; ++k) key[k] = !open ? -INFINITY : p.bias ? key[k] : x[k];
+      }
+      const bool rounded = p.bias != nullptr;               // without a bias keys are scores from here on
+      float best = -INFINITY, mine_key = -INFINITY;
+      int best_j = 0x7fffffff;
+      auto lane_best = [&]() {
+        best = -INFINITY;
+        best_j = 0x7fffffff;
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+          if (key[k] > best) { best = key[k]; best_j = first + k; }
+      };
+      lane_best();
+      const int rounds = min(p.top + (rounded ? 1 : 0), 32);
+      for (int r = 0; r < rounds; ++r) {
+        const uint32_t k = best > -INFINITY ? order(best) : 0u, largest = __reduce_max_sync(kAll, k);
+        if (largest == 0) break;
+        const int j = __reduce_min_sync(kAll, k == largest ? best_j : 0x7fffffff);
+        if (lane == r) {
+          mine = j;
+          mine_key = __uint_as_float(largest ^ ((largest & 0x80000000u) ? 0x80000000u : 0xffffffffu));
         }
-        __syncwarp();
+        if (j == best_j) {
+#pragma unroll
+          for (int i = 0; i < C; ++i)
+            if (first + i == j) key[i] = -INFINITY;
+          lane_best();
+        }
+      }
+      if (rounded) {
+        // neighbours that float32 may have in the wrong order (equal scores and biases are in the right one, if it is
+        // clear that nothing else comes between)
+        const float xs = mine >= 0 ? widen(s[mine]) : 0.f, bs = mine >= 0 ? p.bias[mine] : 0.f;
+        const float next = __shfl_down_sync(kAll, mine_key, 1), nx = __shfl_down_sync(kAll, xs, 1), nb = __shfl_down_sync(kAll, bs, 1);
+        const bool near = lane < rounds - 1 && next > -INFINITY && mine_key - next <= tol;
+        const bool same = xs == nx && bs == nb && lane < p.top - 1;
+        exact = exact || __any_sync(kAll, near && !same) || (p.top == 32 && rounds == 32);
+        if (lane >= p.top) mine = -1;
       }
     }
-    int mine = -1;                                        // lane k < top holds the k-th choice
-    for (int k = 0; k < p.top && !bad; ++k) {
-      double v = -INFINITY;
-      int j = -1;
-      for (int c = lane; c < p.cols; c += 32)
-        if (key[c] > v) { v = key[c]; j = c; }
-      warp_best(v, j);
-      if (j < 0) break;
-      if (lane == k) mine = j;
-      if (lane == (j & 31)) key[j] = -INFINITY;
-      __syncwarp();
-    }
+    if (!bad && exact) mine = choose_exact(p, s, keys + (size_t)w * p.cols);
+
     float weight = 0.f;
-    const float x = mine >= 0 ? widen(s[mine]) : 0.f;
-    float lw = mine < 0 ? -INFINITY : p.kind == TRNOPT_ROUTE_SOFTMAX ? x - (float)m : log_sigmoid(x);
+    const float xm = mine >= 0 ? widen(s[mine]) : 0.f;
+    const float lw = mine < 0 ? -INFINITY : softmax ? xm - m : log_sigmoid(xm);
     if (p.renormalize) {
-      float peak = lw;
-      for (int o = 16; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor_sync(kAll, peak, o));
-      const float e = mine >= 0 ? expf(lw - peak) : 0.f, total = warp_sum(e);
+      const float peak = warp_max(lw), e = mine >= 0 ? expf(lw - peak) : 0.f, total = warp_sum(e);
       if (mine >= 0) weight = p.scale * (e / total);
     } else if (mine >= 0) {
-      weight = p.scale * (p.kind == TRNOPT_ROUTE_SOFTMAX ? expf(lw) / (float)sum : expf(lw));
+      weight = p.scale * (softmax ? expf(lw) / sum : expf(lw));
     }
     if (lane < p.top) {
       p.index[row * p.top + lane] = mine;
       p.weight[row * p.top + lane] = bad ? NAN : weight;
-      if (p.load && mine >= 0) atomicAdd(p.load + mine, 1);
+      if (p.load && mine >= 0) atomicAdd(counts + mine, 1);
     }
-    __syncwarp();
+  }
+  if (p.load) {
+    __syncthreads();
+    for (int j = threadIdx.x; j < p.cols; j += 32 * RT_WARPS) {
+      if (gridDim.x == 1) p.load[j] = counts[j];
+      else if (counts[j] != 0) atomicAdd(p.load + j, counts[j]);
+    }
   }
 }
 
+// Gradient: a chosen column's value is scale * share * (d - mean) (renormalised: parts of the chosen ones' sum; a sigmoid:
+// its own derivative), the others' 0, or for plain softmax weights -share * mean. One warp per row: the row's vectors, then
+// the chosen columns over them.
 template <typename T>
 __global__ void __launch_bounds__(32 * RT_WARPS) route_grad_kernel(RouteGradProblem p) {
+  constexpr int kN = Vec<T>::kN;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const bool softmax = p.kind == TRNOPT_ROUTE_SOFTMAX;
   for (long long row = (long long)blockIdx.x * RT_WARPS + w; row < p.rows; row += (long long)gridDim.x * RT_WARPS) {
     const T* s = static_cast<const T*>(p.scores) + row * p.ld;
     T* out = static_cast<T*>(p.grad) + row * p.ld_grad;
-    const int mine = lane < p.top ? (int)p.index[row * p.top + lane] : -1;
+    const RowVectors<T> rv(out, p.cols);
+    const long long index = lane < p.top ? p.index[row * p.top + lane] : -1;
+    const int mine = index >= 0 && index < p.cols ? (int)index : -1;
     const float d = mine >= 0 ? p.scale * p.d_weight[row * p.top + lane] : 0.f;
     const float x = mine >= 0 ? widen(s[mine]) : 0.f;
-    const bool softmax = p.kind == TRNOPT_ROUTE_SOFTMAX;
-    const bool any = __any_sync(kAll, mine >= 0);
     float grad = 0.f;
-    if (p.renormalize || !softmax || !any) {
-      for (int j = lane; j < p.cols; j += 32) narrow(0.f, out + j);
+    if (p.renormalize || !softmax || !__any_sync(kAll, mine >= 0)) {
+      for (int v = lane; v < (int)rv.count; v += 32) {
+        const int j = (int)rv.column(v);
+        if (rv.inside(v)) {
+          *reinterpret_cast<uint4*>(out + j) = make_uint4(0, 0, 0, 0);
+        } else {
+          for (int e = max(j, 0); e < min(j + kN, p.cols); ++e) narrow(0.f, out + e);
+        }
+      }
       const float other = softmax ? 1.f : 1.f / (1.f + expf(x));      // d log share / dS of a column by itself
       if (p.renormalize) {
         const float lw = mine < 0 ? -INFINITY : softmax ? x : log_sigmoid(x);
-        float peak = lw;
-        for (int o = 16; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor_sync(kAll, peak, o));
-        const float e = mine >= 0 ? expf(lw - peak) : 0.f;
-        const float part = e / warp_sum(e), mean = warp_sum(mine >= 0 ? part * d : 0.f);
+        const float peak = warp_max(lw), e = mine >= 0 ? expf(lw - peak) : 0.f;
+        const float total = warp_sum(e), part = mine >= 0 ? e / total : 0.f, mean = warp_sum(mine >= 0 ? part * d : 0.f);
         grad = part * (d - mean) * other;
       } else {
         grad = d * expf(log_sigmoid(x)) * other;
@@ -164,14 +348,29 @@ __global__ void __launch_bounds__(32 * RT_WARPS) route_grad_kernel(RouteGradProb
     } else {
       float m = -INFINITY, sum = 0.f;
       for (int j = lane; j < p.cols; j += 32) m = fmaxf(m, widen(s[j]));
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
-      for (int j = lane; j < p.cols; j += 32) sum += expf(widen(s[j]) - m);
+      m = warp_max(m);
+      for (int j = lane; j < p.cols; j += 32) sum += ex2_approx((widen(s[j]) - m) * kLog2e);
       sum = warp_sum(sum);
-      const float share = mine >= 0 ? expf(x - m) / sum : 0.f, mean = warp_sum(share * d);
-      for (int j = lane; j < p.cols; j += 32) narrow(-(expf(widen(s[j]) - m) / sum) * mean, out + j);
+      const float share = mine >= 0 ? expf(x - m) / sum : 0.f, mean = warp_sum(share * d), back = -mean / sum;
+      for (int v = lane; v < (int)rv.count; v += 32) {
+        const int j = (int)rv.column(v);
+        Vec<T> r;
+#pragma unroll
+        for (int e = 0; e < kN; e += 2) {
+          auto at = [&](int k) { return k >= 0 && k < p.cols ? ex2_approx((widen(s[k]) - m) * kLog2e) * back : 0.f; };
+          r.set_pair(e, at(j + e), at(j + e + 1));
+        }
+        if (rv.inside(v)) {
+          *reinterpret_cast<uint4*>(out + j) = r.q;
+        } else {
+#pragma unroll
+          for (int e = 0; e < kN; ++e)
+            if (j + e >= 0 && j + e < p.cols) out[j + e] = r.stored(e);
+        }
+      }
       grad = share * (d - mean);
     }
-    __syncwarp();                                        // a chosen column's value follows the row's dense one
+    __syncwarp();                                           // a chosen column's value follows the row's others
     if (mine >= 0) narrow(grad, out + mine);
   }
 }
@@ -181,21 +380,56 @@ unsigned route_grid(long long rows) {
   return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20));
 }
 
+template <typename T, int C>
+cudaError_t launch(const RouteProblem& p, const RouteLayout& lay, cudaStream_t stream) {
+  const size_t bytes = (size_t)RT_WARPS * p.cols * sizeof(double) + (size_t)p.cols * sizeof(int);
+  static std::atomic<int> done[kMaxDevices];
+  cudaError_t e = smem_attr_once(reinterpret_cast<const void*>(route_kernel<T, C>), (int)bytes, done);
+  if (e != cudaSuccess) return e;
+  // a persistent grid of 4 CTAs per SM (the load is counted once per CTA)
+  const long long blocks = (p.rows + RT_WARPS - 1) / RT_WARPS;
+  const unsigned grid = (unsigned)(blocks < 148 * 4 ? blocks : 148 * 4);
+  if (p.load && grid > 1) {
+    e = cudaMemsetAsync(p.load, 0, sizeof(int) * p.cols, stream);
+    if (e != cudaSuccess) return e;
+  }
+  route_kernel<T, C><<<grid, 32 * RT_WARPS, bytes, stream>>>(p, lay);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch(const RouteProblem& p, cudaStream_t stream) {
+  RouteLayout lay{};
+  lay.size = p.cols / p.groups;
+  lay.lanes = 32;
+  for (int g = 1; g < p.groups; g *= 2) lay.lanes /= 2;
+  lay.run = (lay.size + lay.lanes - 1) / lay.lanes;
+  lay.exact = lay.run > 32;                                 // (few groups of many columns, not a power of two of them)
+  if (lay.exact) { lay.lanes = 32; lay.run = 1; lay.size = p.cols < 32 ? p.cols : 32; }
+  int c = 1;
+  while (c < lay.run) c *= 2;
+  const int v = c < Vec<T>::kN ? c : Vec<T>::kN;
+  lay.vectors = !lay.exact && c == lay.run && lay.size % c == 0 && p.ld % v == 0 &&
+                reinterpret_cast<uintptr_t>(p.scores) % (v * sizeof(T)) == 0;
+  switch (c) {
+    case 1: return launch<T, 1>(p, lay, stream);
+    case 2: return launch<T, 2>(p, lay, stream);
+    case 4: return launch<T, 4>(p, lay, stream);
+    case 8: return launch<T, 8>(p, lay, stream);
+    case 16: return launch<T, 16>(p, lay, stream);
+    default: return launch<T, 32>(p, lay, stream);
+  }
+}
+
 }  // namespace
 
 cudaError_t route_launch(int type, const RouteProblem& p, cudaStream_t stream) {
-  if (p.load) {
-    const cudaError_t e = cudaMemsetAsync(p.load, 0, sizeof(int) * p.cols, stream);
-    if (e != cudaSuccess) return e;
-  }
-  if (p.rows == 0) return cudaSuccess;
-  const unsigned grid = route_grid(p.rows);
+  if (p.rows == 0) return p.load ? cudaMemsetAsync(p.load, 0, sizeof(int) * p.cols, stream) : cudaSuccess;
   switch (type) {
-    case TRNOPT_F32: route_kernel<float><<<grid, 32 * RT_WARPS, 0, stream>>>(p); break;
-    case TRNOPT_F16: route_kernel<__half><<<grid, 32 * RT_WARPS, 0, stream>>>(p); break;
-    default: route_kernel<__nv_bfloat16><<<grid, 32 * RT_WARPS, 0, stream>>>(p); break;
+    case TRNOPT_F32: return launch<float>(p, stream);
+    case TRNOPT_F16: return launch<__half>(p, stream);
+    default: return launch<__nv_bfloat16>(p, stream);
   }
-  return cudaGetLastError();
 }
 
 cudaError_t route_grad_launch(int type, const RouteGradProblem& p, cudaStream_t stream) {
