@@ -9,7 +9,8 @@
 // Columns of score -inf or biased key -inf are closed. Slots that no open column fills hold index -1 and weight 0. A
 // row holding NaN or +inf chooses nothing: index -1, weight NaN.
 // The order of keys is that of their 64-bit values. One warp per row holds float32 keys in registers, a run of columns
-// per lane within a group, and takes the best one `top` + 1 times (two warp reductions each). Where neighbours in that
+// per lane within a group; the keys that reach the (top + 1)-th largest of the lanes' best are a dozen or so, which are
+// ranked in shared memory. Where neighbours in that
 // order, or the last open and the first closed group, are closer than the float32 keys are exact, and not equal in score
 // and bias, the row is done again in float64 through shared memory (a few rows in a thousand). Keys that are the scores
 // themselves are exact. Weights are float32 from the logarithms of the shares (shares that underflow still give their
@@ -28,6 +29,11 @@ namespace trnopt {
 namespace {
 
 constexpr int RT_WARPS = 8;
+constexpr int RT_LIST = 64;          // candidates of a row that are ranked
+
+struct RouteSmem {
+  uint64_t list[RT_WARPS][RT_LIST], best[RT_WARPS][32];     // (key, column) as whole numbers in their order
+};
 constexpr unsigned kAll = 0xffffffffu;
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -60,6 +66,19 @@ __device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.f) - l
 __device__ __forceinline__ uint32_t order(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+
+// The k-th largest (1 .. 32) of the warp's values.
+__device__ __forceinline__ float kth_largest(float v, int k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int o = size / 2; o > 0; o /= 2) {
+      const float x = __shfl_xor_sync(kAll, v, o);
+      v = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(v, x) : fminf(v, x);
+    }
+  return __shfl_sync(kAll, v, k - 1);
 }
 
 // A row's choices by 64-bit keys in shared memory: lane k < top gets the k-th column, or -1.
@@ -134,8 +153,9 @@ struct RouteLayout {
 };
 
 template <typename T, int C>
-__global__ void __launch_bounds__(32 * RT_WARPS) route_kernel(RouteProblem p, RouteLayout lay) {
+__global__ void __launch_bounds__(32 * RT_WARPS, C <= 8 ? 4 : 2) route_kernel(RouteProblem p, RouteLayout lay) {
   extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ RouteSmem sh;
   double* keys = reinterpret_cast<double*>(smem);                  // (RT_WARPS, cols), for rows by 64-bit keys
   int* counts = reinterpret_cast<int*>(keys + (size_t)RT_WARPS * p.cols);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -180,19 +200,13 @@ __global__ void __launch_bounds__(32 * RT_WARPS) route_kernel(RouteProblem p, Ro
       for (int k = 0; k < C; ++k) x[k] = k < mine_n ? widen(s[first + k]) : -INFINITY;
     }
     float m = -INFINITY;
-    bool bad = false;
 #pragma unroll
-    for (int k = 0; k < C; ++k) {
-      bad = bad || !(x[k] < INFINITY);
-      m = fmaxf(m, x[k]);
-    }
+    for (int k = 0; k < C; ++k) m = max_nan(m, x[k]);
     if (lay.exact)                                          // (the registers hold the first columns only)
       for (int j = lane; j < p.cols; j += 32) {
-        const float v = widen(s[j]);
-        bad = bad || !(v < INFINITY);
-        m = fmaxf(m, v);
+        m = max_nan(m, widen(s[j]));
       }
-    bad = __any_sync(kAll, bad) || bad_bias;
+    const bool bad = __any_sync(kAll, !(m < INFINITY)) || bad_bias;
     m = warp_max(m);
     float sum = 0.f;
     if (softmax && (shares || !p.renormalize)) {
@@ -247,40 +261,69 @@ __global__ void __launch_bounds__(32 * RT_WARPS) route_kernel(RouteProblem p, Ro
         for (int k = 0; k < C; ++k) key[k] = !open ? -INFINITY : p.bias ? key[k] : x[k];
       }
       const bool rounded = p.bias != nullptr;               // without a bias keys are scores from here on
-      float best = -INFINITY, mine_key = -INFINITY;
-      int best_j = 0x7fffffff;
-      auto lane_best = [&]() {
-        best = -INFINITY;
-        best_j = 0x7fffffff;
+      const int wanted = min(p.top + (rounded ? 1 : 0), 32);
+      float mine_key = -INFINITY;
+      // at least `wanted` keys reach the wanted-th largest of the lanes' best ones: these go to shared memory
+      float best = key[0];
 #pragma unroll
-        for (int k = 0; k < C; ++k)
-          if (key[k] > best) { best = key[k]; best_j = first + k; }
-      };
-      lane_best();
-      const int rounds = min(p.top + (rounded ? 1 : 0), 32);
-      for (int r = 0; r < rounds; ++r) {
-        const uint32_t k = best > -INFINITY ? order(best) : 0u, largest = __reduce_max_sync(kAll, k);
-        if (largest == 0) break;
-        const int j = __reduce_min_sync(kAll, k == largest ? best_j : 0x7fffffff);
-        if (lane == r) {
-          mine = j;
-          mine_key = __uint_as_float(largest ^ ((largest & 0x80000000u) ? 0x80000000u : 0xffffffffu));
-        }
-        if (j == best_j) {
+      for (int k = 1; k < C; ++k) best = fmaxf(best, key[k]);
+      const float bound = kth_largest(best, wanted);
+      int n = 0;
 #pragma unroll
-          for (int i = 0; i < C; ++i)
-            if (first + i == j) key[i] = -INFINITY;
-          lane_best();
+      for (int k = 0; k < C; ++k) {
+        const bool in = key[k] >= bound && key[k] > -INFINITY;
+        const unsigned all = __ballot_sync(kAll, in);
+        const int at = n + __popc(all & ((1u << lane) - 1));
+        if (in && at < RT_LIST) sh.list[w][at] = (uint64_t)order(key[k]) << 32 | (0xffffffffu - (unsigned)(first + k));
+        n += __popc(all);
+      }
+      __syncwarp();
+      uint64_t taken = 0;                                   // lane r < wanted: the r-th of them, 0 where there is none
+      if (n <= RT_LIST) {
+        // ranked by counting, a candidate or two per lane
+        for (int e = lane; e < n; e += 32) {
+          const uint64_t c = sh.list[w][e];
+          int rank = 0;
+#pragma unroll 4
+          for (int o = 0; o < n; ++o) rank += sh.list[w][o] > c;
+          if (rank < 32) sh.best[w][rank] = c;
         }
+        __syncwarp();
+        if (lane < min(n, wanted)) taken = sh.best[w][lane];
+      } else {
+        // many equal keys: the best one `wanted` times
+        for (int r = 0; r < wanted; ++r) {
+          uint64_t c = 0;
+#pragma unroll
+          for (int k = 0; k < C; ++k) {
+            const uint64_t x = (uint64_t)order(key[k]) << 32 | (0xffffffffu - (unsigned)(first + k));
+            c = key[k] > -INFINITY && x > c ? x : c;
+          }
+          for (int o = 16; o > 0; o >>= 1) {
+            const uint64_t x = __shfl_xor_sync(kAll, c, o);
+            c = x > c ? x : c;
+          }
+          if (c == 0) break;
+          if (lane == r) taken = c;
+#pragma unroll
+          for (int k = 0; k < C; ++k)
+            if (first + k == (int)(0xffffffffu - (unsigned)c)) key[k] = -INFINITY;
+        }
+      }
+      __syncwarp();
+      if (taken != 0) {
+        const uint32_t k = (uint32_t)(taken >> 32);
+        mine = (int)(0xffffffffu - (unsigned)taken);
+        mine_key = __uint_as_float(k ^ ((k & 0x80000000u) ? 0x80000000u : 0xffffffffu));
       }
       if (rounded) {
         // neighbours that float32 may have in the wrong order (equal scores and biases are in the right one, if it is
         // clear that nothing else comes between)
         const float xs = mine >= 0 ? widen(s[mine]) : 0.f, bs = mine >= 0 ? p.bias[mine] : 0.f;
         const float next = __shfl_down_sync(kAll, mine_key, 1), nx = __shfl_down_sync(kAll, xs, 1), nb = __shfl_down_sync(kAll, bs, 1);
-        const bool near = lane < rounds - 1 && next > -INFINITY && mine_key - next <= tol;
+        const bool near = lane < wanted - 1 && next > -INFINITY && mine_key - next <= tol;
         const bool same = xs == nx && bs == nb && lane < p.top - 1;
-        exact = exact || __any_sync(kAll, near && !same) || (p.top == 32 && rounds == 32);
+        exact = exact || __any_sync(kAll, near && !same) || p.top == 32;
         if (lane >= p.top) mine = -1;
       }
     }
