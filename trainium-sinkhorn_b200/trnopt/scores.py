@@ -21,7 +21,7 @@ the device (an index out of range, NaN) never raise and show in the results as d
 
 from __future__ import annotations
 
-import ctypes
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
@@ -80,16 +80,21 @@ def _small(t: torch.Tensor | None, n: int, name: str, like: torch.Tensor) -> tor
     return t.detach().contiguous()
 
 
-def _call(name: str, like: torch.Tensor, *args) -> None:
-    """A C call on the device of `like`, on that device's current stream."""
-    index = like.device.index
+# The current stream's handle on a device, without making a Stream object for it where torch offers that.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(name: str, index: int, *args) -> None:
+    """A C call on device `index`, on that device's current stream."""
     fn = getattr(_capi.lib, name)
     if index == torch.cuda.current_device():
-        status = fn(*args, ctypes.c_void_p(torch.cuda.current_stream(index).cuda_stream))
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            status = fn(*args, ctypes.c_void_p(torch.cuda.current_stream(index).cuda_stream))
-    _capi.check(status, name)
+            status = fn(*args, _raw_stream(index))
+    if status != 0:
+        _capi.check(status, name)
 
 
 def _at(t: torch.Tensor | None):
@@ -98,44 +103,48 @@ def _at(t: torch.Tensor | None):
 
 # log_probs -----------------------------------------------------------------------------------------------------------
 
-def _log_probs_forward(s, targets, top, temperature, keep):
+def _log_probs_forward(s, lead, targets, n_targets, top, temperature, keep):
+    """The call's outputs, in the shapes the user sees, and the rows' (maximum, log sum) if they are to be kept."""
     rows, cols = s.shape
     wide = torch.float64 if s.dtype == torch.float64 else torch.float32
-    n_targets = 0 if targets is None else targets.shape[1]
-
-    def new(*shape, dtype=wide):
-        return torch.empty(shape, dtype=dtype, device=s.device)
-
-    log_prob, entropy, lse = new(rows, n_targets), new(rows), new(rows)
-    top_log_prob, top_index = new(rows, top), new(rows, top, dtype=torch.int64)
-    row_max, log_sum = (new(rows), new(rows)) if keep else (None, None)
-    _call("trnopt_log_probs", s, _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, temperature, _at(targets),
-          n_targets, top, _at(log_prob), _at(entropy), _at(lse), _at(top_log_prob), _at(top_index), _at(row_max),
-          _at(log_sum))
-    return log_prob, entropy, lse, top_log_prob, top_index, row_max, log_sum
+    new = s.new_empty
+    log_prob = None if targets is None else new(targets.shape, dtype=wide)
+    entropy, lse = new(lead, dtype=wide), new(lead, dtype=wide)
+    top_log_prob, top_index = (new((*lead, top), dtype=wide), new((*lead, top), dtype=torch.int64)) if top else (None,) * 2
+    kept = new((2, rows), dtype=wide) if keep else None
+    row_max = _at(kept)
+    log_sum = row_max + rows * wide.itemsize if keep else None
+    _call("trnopt_log_probs", s.get_device(), _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, temperature,
+          _at(targets), n_targets, top, _at(log_prob), entropy.data_ptr(), lse.data_ptr(), _at(top_log_prob),
+          _at(top_index), row_max, log_sum)
+    return log_prob, entropy, lse, top_log_prob, top_index, kept
 
 
 class _LogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, s, targets, top, temperature):
-        *out, row_max, log_sum = _log_probs_forward(s, targets, top, temperature, True)
-        ctx.save_for_backward(s, targets, out[4], row_max, log_sum, out[1])
-        ctx.top, ctx.temperature = top, temperature
-        ctx.mark_non_differentiable(out[4])
+    def forward(ctx, s, lead, targets, n_targets, top, temperature):
+        log_prob, entropy, lse, top_log_prob, top_index, kept = _log_probs_forward(s, lead, targets, n_targets, top,
+                                                                                   temperature, True)
+        ctx.save_for_backward(s, targets, top_index, kept, entropy)
+        ctx.call = (n_targets, top, temperature)
+        if top:
+            ctx.mark_non_differentiable(top_index)
         ctx.set_materialize_grads(False)
-        return tuple(out)
+        return log_prob, entropy, lse, top_log_prob, top_index
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_log_prob, d_entropy, d_lse, d_top, _):
-        s, targets, top_index, row_max, log_sum, entropy = ctx.saved_tensors
+        s, targets, top_index, kept, entropy = ctx.saved_tensors
+        n_targets, top, temperature = ctx.call
         rows, cols = s.shape
-        grad = torch.empty((rows, cols), dtype=s.dtype, device=s.device)
+        grad = s.new_empty((rows, cols))
         up = [None if d is None else d.contiguous() for d in (d_log_prob, d_entropy, d_lse, d_top)]
-        _call("trnopt_log_probs_grad", s, _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, ctx.temperature,
-              _at(targets), 0 if targets is None else targets.shape[1], _at(top_index), ctx.top, _at(row_max),
-              _at(log_sum), _at(entropy), *map(_at, up), _at(grad), cols)
-        return grad, None, None, None
+        row_max = kept.data_ptr()
+        _call("trnopt_log_probs_grad", s.get_device(), _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, temperature,
+              _at(targets), n_targets, _at(top_index), top, row_max, row_max + rows * kept.element_size(),
+              entropy.data_ptr(), *map(_at, up), grad.data_ptr(), cols)
+        return grad, None, None, None, None, None
 
 
 def log_probs(scores: torch.Tensor, targets: torch.Tensor | None = None, *, top: int = 0,
@@ -156,25 +165,24 @@ def log_probs(scores: torch.Tensor, targets: torch.Tensor | None = None, *, top:
         raise ValueError(f"top must lie in 0 .. {MAX_TOP}")
     if not 1e-30 <= temperature <= 1e30:
         raise ValueError("temperature must be positive and finite (1e-30 .. 1e30)")
-    lead = scores.shape[:-1]
-    t = None
+    lead, n_targets = scores.shape[:-1], 0
     if targets is not None:
         if not isinstance(targets, torch.Tensor) or targets.device != scores.device or \
                 targets.dtype not in (torch.int64, torch.int32):
             raise ValueError(f"targets must be an int64 or int32 tensor on {scores.device}")
-        if targets.shape != lead and targets.shape[:-1] != lead:
+        if targets.shape == lead:
+            n_targets = 1
+        elif targets.shape[:-1] == lead:
+            n_targets = targets.shape[-1]
+        else:
             raise ValueError(f"targets must have shape {tuple(lead)} or {tuple(lead)} + (T,)")
-        per_row = 1 if targets.shape == lead else targets.shape[-1]
-        if per_row > MAX_TARGETS:
+        if n_targets > MAX_TARGETS:
             raise ValueError(f"at most {MAX_TARGETS} targets a row")
-        t = targets.reshape(s.shape[0], per_row).to(torch.int64).contiguous()
+        if targets.dtype != torch.int64 or not targets.is_contiguous():
+            targets = targets.to(torch.int64).contiguous()
     if s.requires_grad and torch.is_grad_enabled():
-        log_prob, entropy, lse, top_log_prob, top_index = _LogProbs.apply(s, t, int(top), float(temperature))
-    else:
-        log_prob, entropy, lse, top_log_prob, top_index, _, _ = _log_probs_forward(s.detach(), t, int(top),
-                                                                                   float(temperature), False)
-    return LogProbs(None if t is None else log_prob.view(targets.shape), entropy.view(lead), lse.view(lead),
-                    top_log_prob.view(*lead, top) if top else None, top_index.view(*lead, top) if top else None)
+        return LogProbs(*_LogProbs.apply(s, lead, targets, n_targets, int(top), float(temperature)))
+    return LogProbs(*_log_probs_forward(s, lead, targets, n_targets, int(top), float(temperature), False)[:5])
 
 
 # balance -------------------------------------------------------------------------------------------------------------
@@ -195,7 +203,7 @@ def balance(scores: torch.Tensor, *, eps: float = 0.05, iters: int = 20, a: torc
     g        a starting potential, for instance the last step's
     A row or column whose terms are all zero (scores -inf, masses 0) has potential 0. The potentials are constants to
     autograd."""
-    s = _matrix(scores, False).detach()
+    s = _matrix(scores, False)
     rows, cols = s.shape
     if cols > MAX_COLUMNS:
         raise ValueError(f"at most {MAX_COLUMNS} columns")
@@ -206,48 +214,56 @@ def balance(scores: torch.Tensor, *, eps: float = 0.05, iters: int = 20, a: torc
     if not 1 <= iters <= 1 << 24:
         raise ValueError("iters must lie in 1 .. 2**24")
     a, b, g = _small(a, rows, "a", s), _small(b, cols, "b", s), _small(g, cols, "g", s)
-    f = torch.empty(rows, dtype=torch.float32, device=s.device)
-    g_out = torch.empty(cols, dtype=torch.float32, device=s.device)
-    with torch.cuda.device(s.device):
-        nbytes = int(_capi.lib.trnopt_balance_workspace_size(rows, cols))
-    ws = torch.empty(max(256, nbytes), dtype=torch.uint8, device=s.device)
-    _call("trnopt_balance", s, _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, float(eps), int(iters), _at(a),
-          _at(b), _at(g), _at(f), _at(g_out), _at(ws), ws.numel())
-    return Balance(f.view(scores.shape[:-1]), g_out)
+    index = s.get_device()
+    f = s.new_empty(scores.shape[:-1], dtype=torch.float32)
+    g_out = s.new_empty((cols,), dtype=torch.float32)
+    ws = s.new_empty((_balance_workspace(index, rows, cols),), dtype=torch.uint8)
+    _call("trnopt_balance", index, _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, float(eps), int(iters), _at(a),
+          _at(b), _at(g), f.data_ptr(), g_out.data_ptr(), ws.data_ptr(), ws.numel())
+    return Balance(f, g_out)
+
+
+@lru_cache(maxsize=256)
+def _balance_workspace(index: int, rows: int, cols: int) -> int:
+    with torch.cuda.device(index):
+        return max(256, int(_capi.lib.trnopt_balance_workspace_size(rows, cols)))
 
 
 # route ---------------------------------------------------------------------------------------------------------------
 
-def _route_forward(s, top, kind, bias, bias_on, groups, top_groups, group_top, renormalize, scale, load):
+def _route_forward(s, lead, top, kind, bias, bias_on, groups, top_groups, group_top, renormalize, scale, load):
     rows, cols = s.shape
-    index = torch.empty((rows, top), dtype=torch.int64, device=s.device)
-    weight = torch.empty((rows, top), dtype=torch.float32, device=s.device)
-    counts = torch.empty(cols, dtype=torch.int32, device=s.device) if load else None
-    _call("trnopt_route", s, _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, top, kind, _at(bias), bias_on,
-          groups, top_groups, group_top, renormalize, scale, _at(index), _at(weight), _at(counts))
-    return weight, index, counts
+    shape = (*lead, top)
+    index, weight = s.new_empty(shape, dtype=torch.int64), s.new_empty(shape, dtype=torch.float32)
+    counts = s.new_empty((cols,), dtype=torch.int32) if load else None
+    _call("trnopt_route", s.get_device(), _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, top, kind, _at(bias),
+          bias_on, groups, top_groups, group_top, renormalize, scale, index.data_ptr(), weight.data_ptr(), _at(counts))
+    return index, weight, counts
 
 
 class _Route(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, s, top, kind, bias, bias_on, groups, top_groups, group_top, renormalize, scale, load):
-        weight, index, counts = _route_forward(s, top, kind, bias, bias_on, groups, top_groups, group_top,
+    def forward(ctx, s, lead, top, kind, bias, bias_on, groups, top_groups, group_top, renormalize, scale, load):
+        index, weight, counts = _route_forward(s, lead, top, kind, bias, bias_on, groups, top_groups, group_top,
                                                renormalize, scale, load)
         ctx.save_for_backward(s, index)
         ctx.call = (top, kind, renormalize, scale)
         ctx.mark_non_differentiable(*((index,) if counts is None else (index, counts)))
-        return weight, index, counts
+        ctx.set_materialize_grads(False)
+        return index, weight, counts
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, d_weight, *_):
+    def backward(ctx, _, d_weight, *__):
+        if d_weight is None:
+            return (None,) * 12
         s, index = ctx.saved_tensors
         rows, cols = s.shape
-        grad = torch.empty((rows, cols), dtype=s.dtype, device=s.device)
+        grad = s.new_empty((rows, cols))
         d_weight = d_weight.contiguous()
-        _call("trnopt_route_grad", s, _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, *ctx.call, _at(index),
-              _at(d_weight), _at(grad), cols)
-        return (grad,) + (None,) * 10
+        _call("trnopt_route_grad", s.get_device(), _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, *ctx.call,
+              index.data_ptr(), d_weight.data_ptr(), grad.data_ptr(), cols)
+        return (grad,) + (None,) * 11
 
 
 def route(scores: torch.Tensor, top: int, *, kind: str = "softmax", bias: torch.Tensor | None = None,
@@ -289,11 +305,6 @@ def route(scores: torch.Tensor, top: int, *, kind: str = "softmax", bias: torch.
     if not abs(scale) < 1e30:
         raise ValueError("scale must be finite")
     bias = _small(bias, cols, "bias", s)
-    args = (int(top), _KIND[kind], bias, _BIAS_ON[bias_on], int(groups), int(top_groups), int(group_top),
-            int(bool(renormalize)), float(scale), bool(load))
-    if s.requires_grad and torch.is_grad_enabled():
-        weight, index, counts = _Route.apply(s, *args)
-    else:
-        weight, index, counts = _route_forward(s.detach(), *args)
-    lead = scores.shape[:-1]
-    return Routing(index.view(*lead, top), weight.view(*lead, top), counts)
+    forward = _Route.apply if s.requires_grad and torch.is_grad_enabled() else _route_forward
+    return Routing(*forward(s, scores.shape[:-1], int(top), _KIND[kind], bias, _BIAS_ON[bias_on], int(groups),
+                            int(top_groups), int(group_top), int(bool(renormalize)), float(scale), bool(load)))
