@@ -1,4 +1,6 @@
 // Launch shape and workspace of balance (the kernel is in score_balance.cuh, compiled per type of score).
+#include <math.h>
+
 #include <atomic>
 
 #include "kernels.h"
@@ -37,7 +39,8 @@ size_t balance_workspace_bytes(int device, int rows, int cols) {
 
 cudaError_t balance_launch(int device, int type, const BalanceProblem& p, void* ws, cudaStream_t stream) {
   const BalanceWork wk{static_cast<unsigned*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes),
-                       device_error_word()};
+                       device_error_word(), p.b ? 0.0 : log2((double)p.cols),
+                       (p.b ? 1.0 : (double)p.cols) / (p.a ? 1.0 : (double)p.rows)};
   if (balance_grid(device, p.rows, p.cols) > 1) {
     const cudaError_t e = cudaMemsetAsync(ws, 0, sizeof(unsigned), stream);
     if (e != cudaSuccess) return e;

@@ -75,6 +75,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// log2 k, to float32's relative accuracy also where k is close to 1: what converged potentials still move by is a
+// difference that would otherwise be rounded the same way in every iteration.
+__device__ __forceinline__ float log2_near_1(double k) {
+  const double t = k - 1.0;
+  if (!(fabs(t) < 0.015625)) return log2f((float)k);
+  return (float)(1.4426950408889634 * (t * (1.0 - t * (0.5 - t * (1.0 / 3.0 - t * (0.25 - t * 0.2))))));
+}
+
 struct Plus {
   __device__ __forceinline__ float operator()(float x, float y) const { return x + y; }
 };
@@ -90,7 +98,7 @@ __host__ __device__ inline size_t exchange_bytes(int cols) {
 }
 __host__ __device__ inline size_t fixed_bytes(int cols) {
   const size_t pad = (size_t)lanes_per_row(cols) * 32;
-  return (exchange_bytes(cols) + 2 * pad * sizeof(float) + cols * (sizeof(float) + 1) + 15) & ~(size_t)15;
+  return (exchange_bytes(cols) + 2 * pad * sizeof(float) + cols * (2 * sizeof(double) + 1) + 15) & ~(size_t)15;
 }
 // A kept row: an odd number of 16-byte units, so that lanes on neighbouring rows meet different banks.
 __host__ __device__ inline int row_bytes(int cols, int size) { return (((cols * size + 15) >> 4) | 1) << 4; }
@@ -106,14 +114,16 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
   float* red = reinterpret_cast<float*>(smem);                      // (NW, cols)
   float2* slice_sums = reinterpret_cast<float2*>(smem);             // (slices, cols4)
   float* us = reinterpret_cast<float*>(smem + exchange_bytes(p.cols));
-  float *peaks_s = us + L * 32, *lb = peaks_s + L * 32;             // (u and the maxima have L x 32 places: -inf, 0)
+  float* peaks_s = us + L * 32;                                     // (u and the maxima have L x 32 places: -inf, 0)
+  double* per_b = reinterpret_cast<double*>(peaks_s + L * 32);      // 1 / b, with the rows' and columns' counts in it
+  double* lb = per_b + p.cols;
   unsigned char* open = reinterpret_cast<unsigned char*>(lb + p.cols);
   T* kept = reinterpret_cast<T*>(smem + fixed_bytes(p.cols));       // (kept_rows, pitch)
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, q = lane & (L - 1), group = lane / L;
   const int cols = p.cols, cols4 = (cols + 3) & ~3, pitch = row_bytes(cols, sizeof(T)) / (int)sizeof(T);
   const double per_eps = 1.4426950408889634 / p.eps, eps_per = p.eps * 0.6931471805599453;
-  const float c = (float)per_eps, per_rows = p.a ? 1.f : 1.f / (float)p.rows;
+  const float c = (float)per_eps, log_cols = (float)wk.log_cols;
   const long long r0 = (long long)blockIdx.x * p.rows / gridDim.x, r1 = (long long)(blockIdx.x + 1) * p.rows / gridDim.x;
   const T* scores = static_cast<const T*>(p.scores) + r0 * p.ld + q * V;
   const float* masses = p.a ? p.a + r0 : nullptr;
@@ -126,15 +136,15 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
   for (int j = tid; j < cols; j += NT) {
     const float b = p.b ? p.b[j] : 1.f;                     // (1 / cols each: log2 cols in a row's sum instead)
     some_closed = some_closed || b == 0.f;
-    lb[j] = b == 0.f ? 0.f : log2f(b);
-    us[j] = (p.g0 ? (float)((double)p.g0[j] * per_eps - shift) : 0.f) + lb[j];
+    lb[j] = b == 0.f || b == 1.f ? 0.0 : log2((double)b);
+    per_b[j] = b == 0.f ? wk.k_scale : wk.k_scale / (double)b;
+    us[j] = (float)((p.g0 ? (double)p.g0[j] * per_eps - shift : 0.0) + lb[j]);
   }
   for (int j = tid; j < L * 32; j += NT) {
     if (j >= cols) us[j] = -INFINITY;
     peaks_s[j] = 0.f;
   }
   some_closed = __syncthreads_or(some_closed);
-  const float log_cols = p.b ? 0.f : log2f((float)cols);
   unsigned closed = 0;                                      // the lane's columns of mass 0
 #pragma unroll
   for (int k = 0; k < C; ++k)
@@ -209,10 +219,10 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
         const float a = !there ? 0.f : masses ? __ldg(masses + row) : 1.f;
         const bool empty = l == 0.f;                        // f = 0: the terms 2^(S c + u) as they are
         if (kMode != 1 && last && q == 0 && there)
-          p.f[r0 + row] = empty ? 0.f : (float)(((double)log_cols - ((double)m + (double)log2f(l) + shift)) * eps_per);
+          p.f[r0 + row] = empty ? 0.f : (float)((wk.log_cols - ((double)m + (double)log2f(l) + shift)) * eps_per);
         if constexpr (kMode == 0) {
           if (!__any_sync(kAll, empty && a != 0.f)) {
-            const float weight = empty ? 0.f : __fdividef(a, l);
+            const float weight = empty ? 0.f : a / l;
             const uint64_t w2 = pack2(weight, weight);
 #pragma unroll
             for (int k = 0; k < C / 2; ++k) acc2[k] = fma2(z2[k], w2, acc2[k]);
@@ -222,7 +232,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
               float x, y;
               unpack2(z2[k / 2], x, y);
               auto term = [&](float e) {
-                return !empty ? e * __fdividef(a, l) : e > 0.f ? a * exp2f(log2f(e) + ((float)shift - log_cols)) : 0.f;
+                return !empty ? e * (a / l) : e > 0.f ? a * exp2f(log2f(e) + ((float)shift - log_cols)) : 0.f;
               };
               acc2[k / 2] = add2(acc2[k / 2], pack2(term(x), term(y)));
             }
@@ -362,15 +372,15 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
       if (first) {
         for (int k = 1; k < slices; ++k) lse2_add(v.x, v.y, slice_sums[(size_t)k * cols4 + j].x, slice_sums[(size_t)k * cols4 + j].y);
         open[j] = v.y != 0.f;
-        full[i] = v.y == 0.f ? 0.0 : shift - ((double)v.x + (double)log2f(v.y * per_rows) + (double)log_cols);
+        full[i] = v.y == 0.f ? 0.0 : shift - ((double)v.x + log2((double)v.y * wk.k_scale));
       } else {
 #pragma unroll 8
         for (int k = 1; k < slices; ++k) v.y += slice_sums[(size_t)k * cols4 + j].y;
         // k_j (a sum that underflows, for masses beyond float32's range from one another, counts as 2^-126)
-        const float step = log2f(v.y == 0.f ? 1.17549435e-38f : v.y * per_rows) - (lb[j] - log_cols);
+        const float step = log2_near_1(v.y == 0.f ? 0x1p-126 : (double)v.y * per_b[j]);
         // the last potentials are not rounded to float32 before the common part goes back
         if (last && blockIdx.x == 0)
-          p.g[j] = open[j] ? (float)(((double)us[j] - (double)lb[j] - (double)step + shift) * eps_per) : 0.f;
+          p.g[j] = open[j] ? (float)(((double)us[j] - lb[j] - (double)step + shift) * eps_per) : 0.f;
         if (open[j]) us[j] -= step;
       }
     }
@@ -383,7 +393,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
       for (int i = 0; i < 2; ++i) {
         const int j = tid + i * NT;
         if (j >= cols) break;
-        us[j] = (float)(full[i] - shift) + lb[j];
+        us[j] = (float)(full[i] - shift + lb[j]);
         if (last && blockIdx.x == 0) p.g[j] = (float)(full[i] * eps_per);
       }
     }

@@ -50,6 +50,8 @@ struct BalanceWork {
   float* parts;            // (2, 2, CTAs, cols rounded up to 4): by parity, the CTAs' column sums, and their maxima in the
                            // first iteration
   int* error_word;
+  double log_cols, k_scale;  // log2 cols and cols / rows for uniform masses, where rows are summed without 1 / cols and
+                           // columns without 1 / rows
 };
 
 struct RouteProblem {
