@@ -103,11 +103,12 @@ __host__ __device__ inline size_t fixed_bytes(int cols) {
 // A kept row: an odd number of 16-byte units, so that lanes on neighbouring rows meet different banks.
 __host__ __device__ inline int row_bytes(int cols, int size) { return (((cols * size + 15) >> 4) | 1) << 4; }
 
-// L lanes per row, C columns per lane in runs of V neighbouring ones.
+// L lanes per row, C columns per lane in runs of 16 bytes (a kept row has whole runs, wherever it lies in global memory;
+// `vectors`: it can be read there by runs, too).
 // (C is 32, or 8 or 16 where a row of few columns has a lane of its own; u has places for 32 either way.)
-template <typename T, int L, int C, int V>
-__global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, BalanceWork wk, int kept_rows) {
-  constexpr int G = 32 / L;                                 // rows a warp takes at a time
+template <typename T, int L, int C>
+__global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, BalanceWork wk, int kept_rows, bool vectors) {
+  constexpr int V = Vec<T>::kN, G = 32 / L;                                 // rows a warp takes at a time
   extern __shared__ __align__(16) unsigned char smem[];
   // the warps' column sums, then the slices of the sum over the CTAs; u + log2 b; log2 b; the CTA's column maxima in the
   // first iteration; whether a column has any term; the kept rows
@@ -172,14 +173,31 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
         uint64_t z2[C / 2];
         float m = -INFINITY, l = 0.f;
         Vec<T> v[C / V];
+        // (columns past the last: 0, with u = -inf)
+        auto runs = [&](auto&& read) {
 #pragma unroll
-        for (int r = 0; r < C / V; ++r) {                   // columns past the last: 0, with u = -inf
-          const int at = r * L * V;
-          v[r].q = make_uint4(0, 0, 0, 0);
-          if (at < cols && (L == 1 || at + q * V < cols)) {
-            if (kMode != 1 && keep) v[r] = read_any<V>(here + at);
-            else v[r] = read_global<V>(s + at);
-            if (kMode == 1 && keep) write_any<V>(here + at, v[r]);
+          for (int r = 0; r < C / V; ++r) {
+            const int at = r * L * V;
+            v[r].q = make_uint4(0, 0, 0, 0);
+            if (at < cols && (L == 1 || at + q * V < cols)) read(v[r], at);
+          }
+        };
+        if (kMode != 1 && keep) {
+          runs([&](Vec<T>& x, int at) { x = read_any<V>(here + at); });
+        } else {
+          if (vectors) {
+            runs([&](Vec<T>& x, int at) { x = read_global<V>(s + at); });
+          } else {
+            runs([&](Vec<T>& x, int at) {
+#pragma unroll
+              for (int i = 0; i < V; ++i)
+                if (at + q * V + i < cols) x.set(i, s[at + i]);
+            });
+          }
+          if (kMode == 1 && keep) {
+#pragma unroll
+            for (int r = 0; r < C / V; ++r)
+              if (r * L * V + q * V < cols) write_any<V>(here + r * L * V, v[r]);
           }
         }
 #pragma unroll
@@ -401,7 +419,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
   }
 }
 
-template <typename T, int L, int C, int V>
+template <typename T, int L, int C>
 cudaError_t launch(int device, const BalanceProblem& p, const BalanceWork& wk, cudaStream_t stream) {
   const int grid = balance_grid(device, p.rows, p.cols);
   // the rows a CTA keeps: all of them, or what shared memory holds (227 KB less what the launch itself takes)
@@ -412,7 +430,7 @@ cudaError_t launch(int device, const BalanceProblem& p, const BalanceWork& wk, c
   if (kept > fits) kept = fits;
   const size_t bytes = fixed + (size_t)kept * row_bytes(p.cols, sizeof(T));
   static std::atomic<int> done[kMaxDevices];
-  cudaError_t e = smem_attr_once(reinterpret_cast<const void*>(balance_kernel<T, L, C, V>), (int)bytes, done);
+  cudaError_t e = smem_attr_once(reinterpret_cast<const void*>(balance_kernel<T, L, C>), (int)bytes, done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)grid);
@@ -424,18 +442,8 @@ cudaError_t launch(int device, const BalanceProblem& p, const BalanceWork& wk, c
   attr.val.cooperative = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = grid > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, balance_kernel<T, L, C, V>, p, wk, (int)kept);
-}
-
-template <typename T, int L, int C>
-cudaError_t launch(int device, const BalanceProblem& p, const BalanceWork& wk, cudaStream_t stream) {
-  // the longest runs of columns per lane that the sizes and addresses allow: 16 bytes, 8, or single scores
-  auto runs = [&](int v) {
-    return p.cols % v == 0 && p.ld % v == 0 && reinterpret_cast<uintptr_t>(p.scores) % (v * sizeof(T)) == 0;
-  };
-  if constexpr (sizeof(T) == 2)
-    if (runs(8)) return launch<T, L, C, 8>(device, p, wk, stream);
-  return runs(4) ? launch<T, L, C, 4>(device, p, wk, stream) : launch<T, L, C, 1>(device, p, wk, stream);
+  const bool vectors = p.cols % Vec<T>::kN == 0 && p.ld % Vec<T>::kN == 0 && reinterpret_cast<uintptr_t>(p.scores) % 16 == 0;
+  return cudaLaunchKernelEx(&cfg, balance_kernel<T, L, C>, p, wk, (int)kept, vectors);
 }
 
 template <typename T>
