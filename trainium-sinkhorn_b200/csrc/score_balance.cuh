@@ -98,7 +98,7 @@ __host__ __device__ inline size_t exchange_bytes(int cols) {
 }
 __host__ __device__ inline size_t fixed_bytes(int cols) {
   const size_t pad = (size_t)lanes_per_row(cols) * 32;
-  return (exchange_bytes(cols) + 2 * pad * sizeof(float) + cols * (2 * sizeof(double) + 1) + 15) & ~(size_t)15;
+  return (exchange_bytes(cols) + 3 * pad * sizeof(float) + cols * (2 * sizeof(double) + 1) + 15) & ~(size_t)15;
 }
 // A kept row: an odd number of 16-byte units, so that lanes on neighbouring rows meet different banks.
 __host__ __device__ inline int row_bytes(int cols, int size) { return (((cols * size + 15) >> 4) | 1) << 4; }
@@ -116,7 +116,8 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
   float2* slice_sums = reinterpret_cast<float2*>(smem);             // (slices, cols4)
   float* us = reinterpret_cast<float*>(smem + exchange_bytes(p.cols));
   float* peaks_s = us + L * 32;                                     // (u and the maxima have L x 32 places: -inf, 0)
-  double* per_b = reinterpret_cast<double*>(peaks_s + L * 32);      // 1 / b, with the rows' and columns' counts in it
+  float* off_s = peaks_s + L * 32;
+  double* per_b = reinterpret_cast<double*>(off_s + L * 32);      // 1 / b, with the rows' and columns' counts in it
   double* lb = per_b + p.cols;
   unsigned char* open = reinterpret_cast<unsigned char*>(lb + p.cols);
   T* kept = reinterpret_cast<T*>(smem + fixed_bytes(p.cols));       // (kept_rows, pitch)
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
   }
   for (int j = tid; j < L * 32; j += NT) {
     if (j >= cols) us[j] = -INFINITY;
-    peaks_s[j] = 0.f;
+    peaks_s[j] = off_s[j] = 0.f;
   }
   some_closed = __syncthreads_or(some_closed);
   unsigned closed = 0;                                      // the lane's columns of mass 0
@@ -256,19 +257,24 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
             }
           }
         } else {
-          // x = S c + f c + log2 a, in the gauge of u - shift: z - u - log2 l + log2 a (and log2 cols, as in mode 0)
+          // x = S c + f c + log2 a, in the gauge of u - shift: z - u - log2 l + log2 a (and log2 cols, as in mode 0); mode 2
+          // takes it relative to the column's maximum, off_s = -u - maximum. (Columns with u = -inf: no number, passed over
+          // by the maximum; z = -inf in the sums.)
           const float off = (empty ? (float)shift - log_cols : -log2f(l)) + log2f(a);
+          const uint64_t o2 = pack2(off, off);
 #pragma unroll
           for (int k = 0; k < C; k += 2) {
-            float zx, zy, ux, uy, ax, ay;
-            unpack2(z2[k / 2], zx, zy);
-            unpack2(u2[k / 2], ux, uy);
-            unpack2(acc2[k / 2], ax, ay);
-            auto term = [&](float z, float u, float acc, int j) {
-              const float x = u == -INFINITY ? -INFINITY : z - u + off;      // (a column past the last, or closed by g)
-              return kMode == 1 ? fmaxf(acc, x) : acc + ex2_approx(x - peaks_s[j]);
-            };
-            acc2[k / 2] = pack2(term(zx, ux, ax, column(k)), term(zy, uy, ay, column(k + 1)));
+            float x, y, ax, ay;
+            if constexpr (kMode == 1) {
+              float ux, uy;
+              unpack2(u2[k / 2], ux, uy);
+              unpack2(add2(add2(z2[k / 2], pack2(-ux, -uy)), o2), x, y);
+              unpack2(acc2[k / 2], ax, ay);
+              acc2[k / 2] = pack2(fmaxf(ax, x), fmaxf(ay, y));
+            } else {
+              unpack2(add2(add2(z2[k / 2], pack2(off_s[column(k)], off_s[column(k + 1)])), o2), x, y);
+              acc2[k / 2] = add2(acc2[k / 2], pack2(ex2_approx(x), ex2_approx(y)));
+            }
           }
         }
       }
@@ -300,15 +306,19 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
       __syncthreads();
     };
     if (first) {
-      pass(std::integral_constant<int, 1>{}, std::true_type{});
+      if (some_closed) pass(std::integral_constant<int, 1>{}, std::true_type{});
+      else pass(std::integral_constant<int, 1>{}, std::false_type{});
       fold(Larger{});
       for (int j = tid; j < cols; j += NT) {
         float m = red[j];
         for (int k = 1; k < NW; ++k) m = fmaxf(m, red[k * cols + j]);
-        peaks_s[j] = fabsf(m) < INFINITY ? m : 0.f;
+        m = fabsf(m) < INFINITY ? m : 0.f;
+        peaks_s[j] = m;
+        off_s[j] = us[j] == -INFINITY ? 0.f : -us[j] - m;
       }
       __syncthreads();
-      pass(std::integral_constant<int, 2>{}, std::true_type{});
+      if (some_closed) pass(std::integral_constant<int, 2>{}, std::true_type{});
+      else pass(std::integral_constant<int, 2>{}, std::false_type{});
     } else if (some_closed) {
       pass(std::integral_constant<int, 0>{}, std::true_type{});
     } else {
