@@ -9,12 +9,11 @@
 // Columns of score -inf or biased key -inf are closed. Slots that no open column fills hold index -1 and weight 0. A
 // row holding NaN or +inf chooses nothing: index -1, weight NaN.
 // The order of keys is that of their 64-bit values. One warp per row holds float32 keys in registers, a run of columns
-// per lane within a group; the keys that reach the (top + 1)-th largest of the lanes' best are a dozen or so, which are
-// ranked in shared memory. Where neighbours in that
-// order, or the last open and the first closed group, are closer than the float32 keys are exact, and not equal in score
-// and bias, the row is done again in float64 through shared memory (a few rows in a thousand). Keys that are the scores
-// themselves are exact. Weights are float32 from the logarithms of the shares (shares that underflow still give their
-// ratio). A persistent grid counts the load in shared memory. Bound by the selection's instructions.
+// per lane within a group; the keys that reach the (top + 1)-th largest of the lanes' best are a dozen or two, which are
+// ranked in shared memory. Where neighbours in that order, or the last open and the first closed group, are closer than
+// the float32 keys are exact, the candidates' (or the groups') keys are formed in float64 and ranked again. Keys that are
+// the scores themselves are exact. Weights are float32 from the logarithms of the shares (shares that underflow still
+// give their ratio). A persistent grid counts the load in shared memory. Bound by the selection's instructions.
 #include <math.h>
 
 #include <atomic>
@@ -33,6 +32,7 @@ constexpr int RT_LIST = 64;          // candidates of a row that are ranked
 
 struct RouteSmem {
   uint64_t list[RT_WARPS][RT_LIST], best[RT_WARPS][32];     // (key, column) as whole numbers in their order
+  double exact[RT_WARPS][RT_LIST];                          // their keys in float64, where they are needed
 };
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -68,41 +68,97 @@ __device__ __forceinline__ uint32_t order(float x) {
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 
-// The k-th largest (1 .. 32) of the warp's values.
+// The key of a (key, column) pair; of 0, -inf.
+__device__ __forceinline__ float key_of(uint64_t pair) {
+  const uint32_t k = (uint32_t)(pair >> 32);
+  return pair == 0 ? -INFINITY : __uint_as_float(k ^ ((k & 0x80000000u) ? 0x80000000u : 0xffffffffu));
+}
+
+// A value that the k largest of the warp's values reach: the k-th largest different one.
 __device__ __forceinline__ float kth_largest(float v, int k) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int size = 2; size <= 32; size *= 2)
-#pragma unroll
-    for (int o = size / 2; o > 0; o /= 2) {
-      const float x = __shfl_xor_sync(kAll, v, o);
-      v = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(v, x) : fminf(v, x);
+  float found = warp_max(v);
+  for (int r = 1; r < k; ++r) {
+    v = v == found ? -INFINITY : v;
+    found = warp_max(v);
+  }
+  return found;
+}
+
+// A row's keys in float64: its share's constants, by the whole warp, then any column's key.
+template <typename T>
+struct ExactKeys {
+  double m, sum;
+  bool softmax, on_scores;
+  __device__ __forceinline__ ExactKeys(const RouteProblem& p, const T* s) : m(-INFINITY), sum(0.0) {
+    const int lane = threadIdx.x & 31;
+    softmax = p.kind == TRNOPT_ROUTE_SOFTMAX;
+    on_scores = p.bias && p.bias_on == TRNOPT_ROUTE_BIAS_SCORES;
+    if (softmax && (on_scores || !p.bias)) {
+      for (int j = lane; j < p.cols; j += 32) m = fmax(m, (double)widen(s[j]));
+      m = warp_max(m);
+      if (m > -INFINITY)
+        for (int j = lane; j < p.cols; j += 32) sum += exp((double)widen(s[j]) - m);
+      sum = warp_sum(sum);
     }
-  return __shfl_sync(kAll, v, k - 1);
+  }
+  // `shares`: without a bias, the share (for the groups' scores) and not the score itself
+  __device__ __forceinline__ double key(const RouteProblem& p, const T* s, int j, bool shares) const {
+    const double x = widen(s[j]);
+    if (!(x > -INFINITY)) return -INFINITY;
+    double k = x;
+    if (on_scores || (shares && !p.bias)) k = softmax ? exp(x - m) / sum : 1.0 / (1.0 + exp(-x));
+    return p.bias ? k + (double)p.bias[j] : k;
+  }
+};
+
+// Candidates list[0 .. n) ranked by their float64 keys, then by column, into best.
+template <typename T>
+__device__ __noinline__ void rank_exact(const RouteProblem& p, const T* s, const uint64_t* list, double* exact, int n,
+                                        uint64_t* best) {
+  const int lane = threadIdx.x & 31;
+  const ExactKeys<T> keys(p, s);
+  for (int e = lane; e < n; e += 32) exact[e] = keys.key(p, s, (int)(0xffffffffu - (unsigned)list[e]), false);
+  __syncwarp();
+  for (int e = lane; e < n; e += 32) {
+    const double k = exact[e];
+    int rank = 0;
+    for (int o = 0; o < n; ++o) rank += exact[o] > k || (exact[o] == k && (unsigned)list[o] > (unsigned)list[e]);
+    if (rank < 32) best[rank] = list[e];
+  }
+  __syncwarp();
+}
+
+// Whether the lane's group stays open, by float64 scores; the lane's columns are first + k, k < n.
+template <typename T>
+__device__ __noinline__ bool open_exact(const RouteProblem& p, const T* s, int lanes, int first, int n) {
+  const int group = (threadIdx.x & 31) / lanes;
+  const ExactKeys<T> keys(p, s);
+  double t1 = -INFINITY, t2 = -INFINITY;
+  for (int k = 0; k < n; ++k) {
+    const double x = keys.key(p, s, first + k, true);
+    t2 = fmax(t2, fmin(t1, x));
+    t1 = fmax(t1, x);
+  }
+  for (int o = 1; o < lanes; o *= 2) {
+    const double o1 = __shfl_xor_sync(kAll, t1, o), o2 = __shfl_xor_sync(kAll, t2, o);
+    t2 = fmax(fmin(t1, o1), fmax(t2, o2));
+    t1 = fmax(t1, o1);
+  }
+  const double score = p.group_top == 2 && t2 > -INFINITY ? t1 + t2 : t1;
+  int rank = 0;
+  for (int g = 0; g < p.groups; ++g) {
+    const double other = __shfl_sync(kAll, score, g * lanes);
+    rank += other > score || (other == score && g < group);
+  }
+  return t1 > -INFINITY && rank < p.top_groups;
 }
 
 // A row's choices by 64-bit keys in shared memory: lane k < top gets the k-th column, or -1.
 template <typename T>
 __device__ __noinline__ int choose_exact(const RouteProblem& p, const T* s, double* key) {
   const int lane = threadIdx.x & 31, size = p.cols / p.groups;
-  double m = -INFINITY, sum = 0.0;
-  for (int j = lane; j < p.cols; j += 32) m = fmax(m, (double)widen(s[j]));
-  m = warp_max(m);
-  if (p.kind == TRNOPT_ROUTE_SOFTMAX && m > -INFINITY) {
-    for (int j = lane; j < p.cols; j += 32) sum += exp((double)widen(s[j]) - m);
-    sum = warp_sum(sum);
-  }
-  const bool on_scores = p.bias && p.bias_on == TRNOPT_ROUTE_BIAS_SCORES;
-  auto share = [&](double x) { return p.kind == TRNOPT_ROUTE_SOFTMAX ? exp(x - m) / sum : 1.0 / (1.0 + exp(-x)); };
-  for (int j = lane; j < p.cols; j += 32) {
-    const double x = widen(s[j]);
-    double k = x;
-    if (x > -INFINITY) {
-      if (on_scores || (p.groups > 1 && !p.bias)) k = share(x);
-      if (p.bias) k += (double)p.bias[j];
-    }
-    key[j] = k;
-  }
+  const ExactKeys<T> keys(p, s);
+  for (int j = lane; j < p.cols; j += 32) key[j] = keys.key(p, s, j, p.groups > 1);
   __syncwarp();
   if (p.groups > 1) {
     // lane g scores group g, then ranks it among all
@@ -225,16 +281,32 @@ __global__ void __launch_bounds__(32 * RT_WARPS, C <= 8 ? 4 : 2) route_kernel(Ro
       // keys, and how far two of them may be apart in float32 and still be in the other order in 64 bits: shares are off
       // by 2^-21 of themselves (2^-20 for a softmax, with its sum), a sum with a bias by 2^-24 of itself
       float key[C], tol = 0.f;
-      const float per_sum = softmax && shares ? 1.f / sum : 0.f;
+      if (!shares) {
 #pragma unroll
-      for (int k = 0; k < C; ++k) {
-        key[k] = x[k];
-        if (shares) key[k] = softmax ? ex2_approx((x[k] - m) * kLog2e) * per_sum : __fdividef(1.f, 1.f + ex2_approx(-x[k] * kLog2e));
-        if (p.bias) key[k] += bias[k];
-        if (x[k] == -INFINITY) key[k] = -INFINITY;
-        if (p.bias && key[k] > -INFINITY) tol = fmaxf(tol, fabsf(key[k]));
+        for (int k = 0; k < C; ++k) key[k] = x[k];
+      } else if (softmax) {
+        const float per_sum = 1.f / sum;
+        tol = 4e-6f * per_sum;
+#pragma unroll
+        for (int k = 0; k < C; ++k) key[k] = ex2_approx((x[k] - m) * kLog2e) * per_sum;
+      } else {
+        tol = 4e-6f;
+#pragma unroll
+        for (int k = 0; k < C; ++k) key[k] = __fdividef(1.f, 1.f + ex2_approx(-x[k] * kLog2e));
       }
-      if (shares || p.bias) tol = 2.4e-7f * warp_max(tol) + (shares ? 4e-6f * (softmax ? per_sum : 1.f) : 0.f);
+      if (p.bias) {
+        float size = 0.f;
+#pragma unroll
+        for (int k = 0; k < C; ++k) {
+          key[k] += bias[k];
+          size = fmaxf(size, key[k] > -INFINITY ? fabsf(key[k]) : 0.f);
+        }
+        tol += 2.4e-7f * warp_max(size);
+      }
+      if (shares) {
+#pragma unroll
+        for (int k = 0; k < C; ++k) key[k] = x[k] == -INFINITY ? -INFINITY : key[k];
+      }
       if (p.groups > 1) {
         float t1 = -INFINITY, t2 = -INFINITY;               // the group's two best, over its lanes
 #pragma unroll
@@ -254,24 +326,24 @@ __global__ void __launch_bounds__(32 * RT_WARPS, C <= 8 ? 4 : 2) route_kernel(Ro
           const float other = __shfl_sync(kAll, score, g * lay.lanes);        // (-inf: nothing open there)
           rank += other > score || (other == score && g < group);
         }
-        const bool open = alive && rank < p.top_groups;
+        bool open = alive && rank < p.top_groups;
         const float lowest = -warp_max(open ? -score : -INFINITY), highest = warp_max(open || !alive ? -INFINITY : score);
-        exact = lowest - highest <= 3.f * tol + 2.4e-7f * fabsf(lowest);
+        if (lowest - highest <= 3.f * tol + 2.4e-7f * fabsf(lowest)) open = open_exact(p, s, lay.lanes, first, mine_n);
 #pragma unroll
         for (int k = 0; k < C; ++k) key[k] = !open ? -INFINITY : p.bias ? key[k] : x[k];
       }
       const bool rounded = p.bias != nullptr;               // without a bias keys are scores from here on
       const int wanted = min(p.top + (rounded ? 1 : 0), 32);
-      float mine_key = -INFINITY;
       // at least `wanted` keys reach the wanted-th largest of the lanes' best ones: these go to shared memory
       float best = key[0];
 #pragma unroll
       for (int k = 1; k < C; ++k) best = fmaxf(best, key[k]);
-      const float bound = kth_largest(best, wanted);
+      // (closed columns are -inf; keys that rounding may have put below the bound are candidates, too)
+      const float bound = fmaxf(kth_largest(best, wanted) - 2.f * tol, -3.4028235e38f);
       int n = 0;
 #pragma unroll
       for (int k = 0; k < C; ++k) {
-        const bool in = key[k] >= bound && key[k] > -INFINITY;
+        const bool in = key[k] >= bound;
         const unsigned all = __ballot_sync(kAll, in);
         const int at = n + __popc(all & ((1u << lane) - 1));
         if (in && at < RT_LIST) sh.list[w][at] = (uint64_t)order(key[k]) << 32 | (0xffffffffu - (unsigned)(first + k));
@@ -290,6 +362,17 @@ __global__ void __launch_bounds__(32 * RT_WARPS, C <= 8 ? 4 : 2) route_kernel(Ro
         }
         __syncwarp();
         if (lane < min(n, wanted)) taken = sh.best[w][lane];
+        if (rounded) {
+          // neighbours that float32 may have in the wrong order
+          const float mine_key = key_of(taken), next = __shfl_down_sync(kAll, mine_key, 1);
+          if (__any_sync(kAll, lane < wanted - 1 && next > -INFINITY && mine_key - next <= tol) || p.top == 32) {
+            __syncwarp();
+            rank_exact(p, s, sh.list[w], sh.exact[w], n, sh.best[w]);
+            taken = lane < min(n, p.top) ? sh.best[w][lane] : 0;
+          }
+        }
+      } else if (rounded) {
+        exact = true;                                       // more candidates than places
       } else {
         // many equal keys: the best one `wanted` times
         for (int r = 0; r < wanted; ++r) {
@@ -311,21 +394,7 @@ __global__ void __launch_bounds__(32 * RT_WARPS, C <= 8 ? 4 : 2) route_kernel(Ro
         }
       }
       __syncwarp();
-      if (taken != 0) {
-        const uint32_t k = (uint32_t)(taken >> 32);
-        mine = (int)(0xffffffffu - (unsigned)taken);
-        mine_key = __uint_as_float(k ^ ((k & 0x80000000u) ? 0x80000000u : 0xffffffffu));
-      }
-      if (rounded) {
-        // neighbours that float32 may have in the wrong order (equal scores and biases are in the right one, if it is
-        // clear that nothing else comes between)
-        const float xs = mine >= 0 ? widen(s[mine]) : 0.f, bs = mine >= 0 ? p.bias[mine] : 0.f;
-        const float next = __shfl_down_sync(kAll, mine_key, 1), nx = __shfl_down_sync(kAll, xs, 1), nb = __shfl_down_sync(kAll, bs, 1);
-        const bool near = lane < wanted - 1 && next > -INFINITY && mine_key - next <= tol;
-        const bool same = xs == nx && bs == nb && lane < p.top - 1;
-        exact = exact || __any_sync(kAll, near && !same) || p.top == 32;
-        if (lane >= p.top) mine = -1;
-      }
+      if (taken != 0 && lane < p.top) mine = (int)(0xffffffffu - (unsigned)taken);
     }
     if (!bad && exact) mine = choose_exact(p, s, keys + (size_t)w * p.cols);
 
