@@ -139,6 +139,38 @@ def test_log_probs_patterns(cols, dtype):
     check_log_probs(s, t.long().cuda(), min(20, cols), 1.0)
 
 
+@pytest.mark.parametrize("repeats", [1, 40, 100, 250])      # few rows on many warps each, to many rows on one warp each
+@pytest.mark.parametrize("dtype,cols,top", [("bf16", 5003, 64), ("f32", 5000, 30), ("f16", 2600, 7), ("f64", 1500, 64)])
+def test_log_probs_patterns_in_many_rows(dtype, cols, top, repeats):
+    s = patterns(cols, TYPES[dtype]).repeat(repeats, 1)
+    s = s[torch.randperm(len(s), generator=gen(1), device="cuda")]
+    check_log_probs(s, torch.randint(cols, (len(s), 1), generator=gen(2), device="cuda"), top, 1.0)
+
+
+def test_log_probs_entropy_is_not_negative():
+    s = make(3000, 500, torch.float32, scale=30.0)
+    s[:, 7] += 200.0
+    for temperature in (1.0, 0.013):
+        assert (scores.log_probs(s, temperature=temperature).entropy >= 0).all()
+
+
+def test_log_probs_extreme_scores_and_temperatures():
+    """Scaled scores beyond float32's range: the differences to the row's maximum decide."""
+    t = torch.randint(2000, (6, 1), generator=gen(2), device="cuda")
+    for scale, temperature in ((1e31, 1e30), (1e37, 1.0), (1e37, 1e5)):
+        s = make(6, 2000, torch.float32, scale=scale)
+        s[1] = make(1, 2000, torch.float32, seed=3)[0] - 3e38
+        r = scores.log_probs(s, t, top=4, temperature=temperature)
+        w = lp_reference(s, t, 4, temperature)
+        assert torch.equal(r.top_index, w["top_i"])
+        close(r.log_prob, w["lp"], 1e-5 * (1 + w["lp"].abs()), "log_prob")
+        close(r.entropy, w["h"], 2e-5 * (1 + w["h"]), "entropy")
+    r = scores.log_probs(s[1:2], t[1:2], top=4)
+    assert torch.isfinite(r.log_prob).all() and torch.isfinite(r.entropy).all()
+    tiny = scores.log_probs(make(1, 2000, torch.float32), top=2, temperature=1e-30)      # one column has everything
+    assert tiny.entropy.item() == 0 and tiny.top_log_prob[0, 0].item() == 0
+
+
 @pytest.mark.parametrize("cols", [33, 20000])
 def test_log_probs_infinite_and_nan_rows(cols):
     for dtype in TYPES.values():
@@ -363,6 +395,23 @@ def test_balance_masses_and_masks():
     check_balance(torch.full((5, 4), -INF, device="cuda"), 0.2, 2)
 
 
+def test_balance_rows_without_open_columns():
+    """Rows whose only scores are on columns of mass 0: potential 0, and their terms still reach those columns."""
+    s = make(70, 9, torch.float32, scale=1.0)
+    b = torch.full((9,), 1 / 7, device="cuda")
+    b[[2, 6]] = 0
+    s[10, [0, 1, 3, 4, 5, 7, 8]] = -INF
+    s[11] = -INF
+    g = 0.5 * make(1, 9, torch.float32, seed=2)[0]
+    for iters in (1, 2, 7):
+        check_balance(s, 0.4, iters, None, b, g)
+
+
+def test_balance_more_rows_than_shared_memory_holds():
+    check_balance(make(70001, 40, torch.float32, scale=1.0), 0.3, 3)
+    check_balance(make(40000, 301, torch.bfloat16, scale=1.0), 0.3, 3)
+
+
 def test_balance_marginals_agree_with_sinkhorn():
     """Converged potentials on S = -C are sinkhorn()'s up to its constant shift, and the plan's columns sum to b."""
     from trnopt import Backend, SinkhornOptions, sinkhorn
@@ -493,6 +542,42 @@ def test_route_ties():
             for groups, top_groups in ((1, 1), (8, 3)):
                 check_route(s, 7, "sigmoid", bias, "scores", groups, top_groups)
                 check_route(s, 7, "softmax", bias, "logits", groups, top_groups)
+
+
+def test_route_many_equal_keys():
+    """More equal keys than a row's candidates have places."""
+    for dtype in (torch.float32, torch.bfloat16):
+        s = torch.zeros(20, 256, dtype=dtype, device="cuda")
+        s[1, 100:] = 1.0
+        s[2, ::2] = -3.0
+        s[3, :250] = -INF
+        for bias in (None, torch.zeros(256, device="cuda")):
+            for groups, top_groups in ((1, 1), (8, 3)):
+                check_route(s, 9, "softmax", bias, "scores", groups, top_groups)
+                check_route(s, 9, "sigmoid", bias, "logits", groups, top_groups)
+
+
+@pytest.mark.parametrize("cols,groups,top_groups,top", [(1020, 5, 2, 9), (1023, 3, 2, 4), (96, 3, 2, 5), (60, 6, 4, 7),
+                                                       (84, 12, 5, 6), (25, 5, 3, 12), (32, 32, 9, 9), (14, 7, 7, 14),
+                                                       (512, 1, 1, 32), (1024, 32, 8, 32)])
+def test_route_group_layouts(cols, groups, top_groups, top):
+    """Groups that are no power of two, of odd sizes, and of more columns than a lane's 32; the most choices."""
+    for dtype in (torch.float32, torch.bfloat16):
+        s = make(150, cols, dtype, seed=cols, scale=1.5)
+        bias = 0.1 * make(1, cols, torch.float32, seed=1)[0]
+        check_route(s, top, "sigmoid", bias, "scores", groups, top_groups)
+        check_route(s, top, "softmax", bias, "logits", groups, top_groups, 1, False)
+        check_route(s, top, "softmax", None, "scores", groups, top_groups)
+
+
+def test_route_infinite_bias():
+    """+inf puts a column first (several: by index), -inf closes it."""
+    s = make(30, 40, torch.float32)
+    bias = 0.1 * make(1, 40, torch.float32, seed=1)[0]
+    bias[[9, 30]], bias[[3, 17]] = INF, -INF
+    for bias_on in ("scores", "logits"):
+        r = check_route(s, 5, "sigmoid", bias, bias_on)
+        assert (r.index[:, 0] == 9).all() and (r.index[:, 1] == 30).all()
 
 
 def test_route_keys_closer_than_float32():

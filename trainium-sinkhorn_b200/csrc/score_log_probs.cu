@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_
   auto log_p = [&](A x) { return empty ? -inf : (x - a.m) * inv_t - log_s; };
   if (tid == 0) {
     static_cast<A*>(p.lse)[row] = empty ? -inf : a.m * inv_t + log_s;
-    static_cast<A*>(p.entropy)[row] = empty ? (A)0 : (B::log(a.s) - a.t / a.s) * B::unit();
+    static_cast<A*>(p.entropy)[row] = empty ? (A)0 : max_nan((A)0, (B::log(a.s) - a.t / a.s) * B::unit());
     if (p.row_max) {
       static_cast<A*>(p.row_max)[row] = a.m;
       static_cast<A*>(p.log_sum)[row] = log_s;

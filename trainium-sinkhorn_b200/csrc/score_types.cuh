@@ -64,7 +64,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ double max_nan(double a, double b) { return (a != a || a > b) ? a : b; }
+__device__ __forceinline__ double max_nan(double a, double b) { return (a != a || a > b) ? a : b; }   // (b NaN: b)
 
 // Sixteen bytes of a row: kN scores.
 template <typename T>
