@@ -171,8 +171,9 @@ struct Candidate<float> {
   __device__ __forceinline__ bool before(const Candidate& o) const { return k > o.k; }
 };
 
-// Shared memory of a CTA of NW warps. The ring holds kStages chunks; after the scores it serves as `kept`: the listed
-// vectors, then the scores of the K best vectors, or the best columns of each of a cluster's 8 CTAs. Where there are
+// Shared memory of a CTA of NW warps. The ring holds kStages chunks; after the scores it serves as `best` (the
+// listed vectors, later the best columns) and `kept` (the scores of the K best vectors, or the best columns of each of a
+// cluster's 8 CTAs). Where there are
 // more than kRanked vectors, they are ranked and cut to K first.
 template <typename T, int NW, bool kTop>
 struct LogProbsSmem {
@@ -181,17 +182,18 @@ struct LogProbsSmem {
   static constexpr int kRanked = 64, kScores = kRanked * Vec<T>::kN;
   static constexpr int kBest = NW == 8 ? 8 * LP_TOP : LP_TOP;
   static constexpr int kKept = (kScores > kBest ? kScores : kBest) * (int)sizeof(Candidate<A>);
+  static constexpr int kChosen = (NW * LP_LIST > kRanked ? NW * LP_LIST : kRanked) * (int)sizeof(Candidate<A>);
   union {
     uint4 ring[kRing / 16];
-    unsigned char kept_bytes[kTop ? (kRing > kKept ? kRing : kKept) : 16];
+    unsigned char after[kTop ? (kRing > kKept + kChosen ? kRing : kKept + kChosen) : 16];
   };
   Candidate<A> list[kTop ? NW * LP_LIST : 1];
-  Candidate<A> best[kTop ? (NW * LP_LIST > kRanked ? NW * LP_LIST : kRanked) : 1];
   volatile A bound[NW];
   int count[NW], kept_count, best_count;
   A m[NW], s[NW], t[NW];
   Sums<A, typename Base<T>::type> part[8];                   // of a cluster's CTAs (in the first one's)
-  __device__ __forceinline__ Candidate<A>* kept() { return reinterpret_cast<Candidate<A>*>(kept_bytes); }
+  __device__ __forceinline__ Candidate<A>* kept() { return reinterpret_cast<Candidate<A>*>(after); }
+  __device__ __forceinline__ Candidate<A>* best() { return reinterpret_cast<Candidate<A>*>(after + (kTop ? kKept : 0)); }
 };
 
 template <typename A>
@@ -441,13 +443,13 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_
     shared_bound();
     for (int e = lane; e < listed; e += 32) {
       const Candidate<A> cand = sh.list[w * LP_LIST + e];
-      if (cand.score() >= bound) sh.best[atomicAdd(&sh.best_count, 1)] = cand;
+      if (cand.score() >= bound) sh.best()[atomicAdd(&sh.best_count, 1)] = cand;
     }
     __syncthreads();
     int n = sh.best_count;
-    const Candidate<A>* vectors = sh.best;
+    const Candidate<A>* vectors = sh.best();
     if (n > Smem::kRanked) {
-      rank_into(sh.best, n, p.top, NT, sh.list);
+      rank_into(sh.best(), n, p.top, NT, sh.list);
       vectors = sh.list;
       n = p.top;
       __syncthreads();
@@ -461,13 +463,13 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_
     }
     __syncthreads();
     n_best = min(sh.kept_count, p.top);
-    rank_into(sh.kept(), sh.kept_count, p.top, NT, sh.best);
+    rank_into(sh.kept(), sh.kept_count, p.top, NT, sh.best());
     __syncthreads();
   }
   a = {sh.m[0], sh.s[0], sh.t[0]};
 #pragma unroll
   for (int k = 1; k < NW; ++k) a.add({sh.m[k], sh.s[k], sh.t[k]}, c);
-  const Candidate<A>* best = sh.best;
+  const Candidate<A>* best = sh.best();
   if (parts > 1) {
     // the cluster's CTAs bring their sums and best columns into the first one's shared memory
     cg::cluster_group cluster = cg::this_cluster();
@@ -483,7 +485,7 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_
     if (part != 0) return;
     for (int k = 1; k < parts; ++k) a.add(sh.part[k], c);
     if (kTop) {
-      rank_into(sh.kept(), parts * p.top, p.top, NT, sh.best);
+      rank_into(sh.kept(), parts * p.top, p.top, NT, sh.best());
       __syncthreads();
       n_best = p.top;
     }
@@ -663,13 +665,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) log_probs_grad_kernel(LogProbsG
   }
 }
 
-// CTAs per row: a cluster where the rows alone leave SMs empty, as long as each CTA has a chunk of its own.
+// CTAs per row: a cluster where the rows alone leave places empty (4 CTAs of 8 warps per SM), as long as each CTA has a
+// chunk of its own.
 template <typename T, int NW>
 int row_parts(const LogProbsProblem& p) {
   const long long chunk = 32LL * NW * LP_VECS * Vec<T>::kN;
   int parts = 1;
   if (NW == 8)
-    while (parts < 8 && p.rows * parts < 148 * 2 && (long long)p.cols > chunk * parts) parts *= 2;
+    while (parts < 8 && 2 * p.rows * parts <= 148 * 4 && (long long)p.cols > chunk * parts) parts *= 2;
   return parts;
 }
 
