@@ -9,16 +9,19 @@
 // potentials u_j = g_j c, a row's terms are e_j = 2^(S_ij c + u_j - m_i) and its sum l_i = sum_j b_j e_j, so
 // f_i c = -(m_i + log2 l_i); the column sums k_j = sum_i a_i e_ij / l_i then give the next potentials,
 // u_j <- u_j - log2 k_j. After an iteration every column's k_j would be 1, so the next one's lies between the smallest
-// a_i / (row sum) and the largest, far from underflow; only the first iteration, from any g, keeps a running maximum per
-// column instead. Potentials are float32 relative to a column's after the first iteration (the common part, in float64,
+// a_i / (row sum) and the largest, far from underflow; only the first iteration, from any g, finds each column's maximum
+// before its sum. Potentials are float32 relative to a column's after the first iteration (the common part, in float64,
 // goes back at the end): they are differences of a few units, where the potentials themselves may be hundreds.
 //
 // One cooperative launch runs all iterations. A CTA owns a block of rows and keeps as many of them as fit in shared
 // memory as they were read in the first pass (the rest come from L2 in every pass). L neighbouring lanes share a row, up
 // to 32 columns each, so a row's maximum and sum take log2 L shuffles for the warp's 32 / L rows together, and a lane
 // sums its columns over its rows in registers. Per iteration the CTAs exchange their column sums through global memory
-// and one grid barrier, and each adds up all of them in the same order. Bound by the exponentials (16 per clock and SM)
-// for many rows, by the barrier's latency for few; what one CTA takes in two steps of its warps stays in one, without it.
+// and one grid barrier, and each adds up all of them in the same order; what one CTA takes in two steps of its warps stays
+// in one, without the barrier. Bound by the pass's instructions for many rows, by the exchange's latency for few. Measured
+// per iteration: 65536 x 256 bfloat16 12.2 us (7 us the pass, of which 3.7 us are exponentials at 16 per clock and SM, the
+// rest the exchange), 65536 x 16 3.8 us, 8192 x 64 4.4 us, 509 x 24 in one CTA 2.2 us; a call of one iteration, which
+// passes twice and reads the scores from DRAM, 39 us for 65536 x 256.
 #pragma once
 
 #include <math.h>
@@ -184,7 +187,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
           }
         };
         if (kMode != 1 && keep) {
-          runs([&](Vec<T>& x, int at) { x = read_any<V>(here + at); });
+          runs([&](Vec<T>& x, int at) { x = *reinterpret_cast<const Vec<T>*>(here + at); });
         } else {
           if (vectors) {
             runs([&](Vec<T>& x, int at) { x = read_global<V>(s + at); });
@@ -198,7 +201,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
           if (kMode == 1 && keep) {
 #pragma unroll
             for (int r = 0; r < C / V; ++r)
-              if (r * L * V + q * V < cols) write_any<V>(here + r * L * V, v[r]);
+              if (r * L * V + q * V < cols) *reinterpret_cast<Vec<T>*>(here + r * L * V) = v[r];
           }
         }
 #pragma unroll

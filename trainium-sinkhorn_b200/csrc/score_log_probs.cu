@@ -20,7 +20,8 @@
 // the K best vectors by (largest score, position): each of these holds a better score than any other vector does. So
 // where ties or ascending scores overflow a list, the warp cuts it to its K best vectors by bisection, and at the end
 // the vectors that still reach the bound are read again (from L2), and their scores ranked. Nothing but the first bound
-// makes warps wait for one another.
+// makes warps wait for one another. Bound by DRAM for many rows: 4096 x 131072 bfloat16 (1.07 GB) 174-198 us without best
+// columns, 188-208 us with 5, by the scores, against 164 us at the copy rate of 6.55 TB/s; 1 x 131072 with 20, 12 us.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -542,7 +543,7 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_
 // chunk on its way while one is worked on. With the row's m and log s a score needs no sum: p (A + B log p), with
 // A = -(g + g_H H) / T, B = -g_H / T and g the sum of the upstream gradients of the row's given and best columns (less
 // that of lse). Those columns are written once more, by the first entry that names them, with the entries that repeat it
-// added in order. Bound by the two matrices' bytes.
+// added in order. Bound by the two matrices' bytes: 8192 x 32768 bfloat16 (2 x 0.54 GB) about 175 us, 164 us at the copy rate.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) log_probs_grad_kernel(LogProbsGradProblem p, int parts, int chunks,
                                                                        typename Acc<T>::type c,
@@ -721,9 +722,9 @@ template <typename T>
 cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
   // The fewest warps per row that fill half of the SMs' 32 warp slots, and no more than the row has chunks for: what a
   // row costs besides its scores (ranking, joining sums) grows with its warps. Measured at 8 / 4 / 2 / 1 warps, bfloat16,
-  // 5 best columns: 8192 x 32768 224 / 160 / 136 / 121 us, 8192 x 1000 139 / 66 / 35 / 21 us, 600 x 5000
-  // 16 / 12 / 10 / 12 us, 300 x 131072 33 / 37 / 52 / 70 us. A warp vouches for 24 best columns at most (of its 32
-  // lanes' maxima the 32nd is a poor bound): 2048 x 32000 with 64 best columns, 130 us with 2 warps, 91 us with 8.
+  // 5 best columns: 8192 x 32768 166 / 129 / 109 / 104 us, 8192 x 1000 115 / 59 / 33 / 18 us, 600 x 5000
+  // 15 / 12 / 10 / 12 us, 300 x 131072 29 / 35 / 47 / 68 us. A warp vouches for 24 best columns at most (of its 32
+  // lanes' maxima the 32nd is a poor bound): 2048 x 32000 with 64 best columns 72 / 76 / 126 / 237 us.
   const long long warp_cols = 32LL * LP_VECS * Vec<T>::kN;
   int nw = 1;
   while (nw < 8 && (p.rows * nw < 148 * 16 || p.top > 24 * nw) && (long long)p.cols > nw * warp_cols) nw *= 2;

@@ -13,7 +13,9 @@
 // ranked in shared memory. Where neighbours in that order, or the last open and the first closed group, are closer than
 // the float32 keys are exact, the candidates' (or the groups') keys are formed in float64 and ranked again. Keys that are
 // the scores themselves are exact. Weights are float32 from the logarithms of the shares (shares that underflow still
-// give their ratio). A persistent grid counts the load in shared memory. Bound by the selection's instructions.
+// give their ratio). A persistent grid counts the load in shared memory. Bound by the selection's instructions: 32768 x 256 float32
+// with 4 of 8 groups, a bias and 8 choices 50 us (958 instructions a row; 5.6 us the scores at the copy rate), plain softmax
+// 31 us; 32768 x 64 bfloat16, 2 choices, 23 us.
 #include <math.h>
 
 #include <atomic>

@@ -214,8 +214,8 @@ struct RowVectors {
   }
 };
 
-// V neighbouring scores (at most 16 bytes, on a boundary of V) in the first places of a vector: from global memory
-// through the read-only cache, or from (and to) any memory.
+// V neighbouring scores (at most 16 bytes, on a boundary of V) in the first places of a vector, through the read-only
+// cache.
 template <int V, typename T>
 __device__ __forceinline__ Vec<T> read_global(const T* p) {
   constexpr int kBytes = V * (int)sizeof(T);
@@ -226,23 +226,4 @@ __device__ __forceinline__ Vec<T> read_global(const T* p) {
   else v.q.x = __ldg(reinterpret_cast<const uint16_t*>(p));
   return v;
 }
-template <int V, typename T>
-__device__ __forceinline__ Vec<T> read_any(const T* p) {
-  constexpr int kBytes = V * (int)sizeof(T);
-  Vec<T> v;
-  if constexpr (kBytes == 16) v.q = *reinterpret_cast<const uint4*>(p);
-  else if constexpr (kBytes == 8) { const uint2 h = *reinterpret_cast<const uint2*>(p); v.q.x = h.x; v.q.y = h.y; }
-  else if constexpr (kBytes == 4) v.q.x = *reinterpret_cast<const uint32_t*>(p);
-  else v.q.x = *reinterpret_cast<const uint16_t*>(p);
-  return v;
-}
-template <int V, typename T>
-__device__ __forceinline__ void write_any(T* p, const Vec<T>& v) {
-  constexpr int kBytes = V * (int)sizeof(T);
-  if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(p) = v.q;
-  else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(p) = make_uint2(v.q.x, v.q.y);
-  else if constexpr (kBytes == 4) *reinterpret_cast<uint32_t*>(p) = v.q.x;
-  else *reinterpret_cast<uint16_t*>(p) = (uint16_t)v.q.x;
-}
-
 }  // namespace trnopt
