@@ -665,6 +665,62 @@ def test_route_gradient_by_differences_of_its_weights():
 
 # together, streams, graphs -------------------------------------------------------------------------------------------
 
+def test_inputs_are_left_as_they_were_and_outputs_stay_inside():
+    """Guard values around every output buffer of the C calls: odd sizes, a gradient with a pitch."""
+    from trnopt import _capi
+    rows, cols, top = 7, 301, 5
+    s = make(rows, cols, torch.bfloat16, seed=1)
+    before = s.clone()
+    t = torch.randint(cols, (rows, 2), generator=gen(1), device="cuda")
+
+    def guarded(*shape, dtype=torch.float32, fill=77):
+        n = math.prod(shape)
+        whole = torch.full((n + 64,), fill, dtype=dtype, device="cuda")
+        return whole, whole[32:32 + n]
+
+    def intact(whole, fill=77):
+        return bool((whole[:32] == fill).all() and (whole[-32:] == fill).all())
+
+    st = torch.cuda.current_stream().cuda_stream
+    bufs = {k: guarded(*shape, dtype=d) for k, shape, d in (
+        ("lp", (rows, 2), torch.float32), ("h", (rows,), torch.float32), ("lse", (rows,), torch.float32),
+        ("tl", (rows, top), torch.float32), ("ti", (rows, top), torch.int64), ("m", (rows,), torch.float32),
+        ("ls", (rows,), torch.float32), ("f", (rows,), torch.float32), ("g", (cols,), torch.float32),
+        ("ri", (rows, 3), torch.int64), ("rw", (rows, 3), torch.float32), ("ld", (cols,), torch.int32))}
+    at = {k: v[1].data_ptr() for k, v in bufs.items()}
+    _capi.check(_capi.lib.trnopt_log_probs(2, s.data_ptr(), cols, rows, cols, 1.0, t.data_ptr(), 2, top, at["lp"], at["h"],
+                                           at["lse"], at["tl"], at["ti"], at["m"], at["ls"], st), "log_probs")
+    pitch = 309
+    grad, inner = guarded(rows, pitch, dtype=torch.bfloat16)
+    _capi.check(_capi.lib.trnopt_log_probs_grad(2, s.data_ptr(), cols, rows, cols, 1.0, t.data_ptr(), 2, at["ti"], top,
+                                                at["m"], at["ls"], at["h"], at["lp"], at["h"], None, None,
+                                                inner.data_ptr(), pitch, st), "log_probs_grad")
+    assert intact(grad) and (inner.view(rows, pitch)[:, cols:] == 77).all()
+    ws = torch.full((_capi.lib.trnopt_balance_workspace_size(rows, cols) + 256,), 7, dtype=torch.uint8, device="cuda")
+    _capi.check(_capi.lib.trnopt_balance(2, s.data_ptr(), cols, rows, cols, 0.5, 3, None, None, None, at["f"], at["g"],
+                                         ws.data_ptr(), ws.numel() - 256, st), "balance")
+    assert (ws[-256:] == 7).all()
+    _capi.check(_capi.lib.trnopt_route(2, s.data_ptr(), cols, rows, cols, 3, 1, None, 0, 1, 1, 2, 1, 1.0, at["ri"], at["rw"],
+                                       at["ld"], st), "route")
+    grad, inner = guarded(rows, pitch, dtype=torch.bfloat16)
+    _capi.check(_capi.lib.trnopt_route_grad(2, s.data_ptr(), cols, rows, cols, 3, 1, 1, 1.0, at["ri"], at["rw"],
+                                            inner.data_ptr(), pitch, st), "route_grad")
+    assert intact(grad) and (inner.view(rows, pitch)[:, cols:] == 77).all()
+    assert all(intact(whole) for whole, _ in bufs.values()) and torch.equal(s, before)
+    assert not any((v == 77).any() for k, (_, v) in bufs.items() if k not in ("ti", "ri", "ld"))
+
+
+def test_workspace_too_small_is_refused():
+    from trnopt import _capi
+    s, f, g = make(4000, 64, torch.float32), torch.empty(4000, device="cuda"), torch.empty(64, device="cuda")
+    need = _capi.lib.trnopt_balance_workspace_size(4000, 64)
+    ws = torch.empty(need + 256, dtype=torch.uint8, device="cuda")
+    call = lambda at, n: _capi.lib.trnopt_balance(0, s.data_ptr(), 64, 4000, 64, 0.5, 3, None, None, None, f.data_ptr(),
+                                                  g.data_ptr(), at, n, torch.cuda.current_stream().cuda_stream)
+    assert call(ws.data_ptr(), need - 1) == -3 and call(None, need) == -3 and call(ws.data_ptr() + 16, need) == -2
+    assert call(ws.data_ptr(), need) == 0
+
+
 def test_balanced_router_step():
     """The three operators as a router's step uses them: potentials, a balanced choice, its weights' gradient, entropy."""
     s = (make(2048, 16, torch.float32, scale=1.0) + torch.linspace(2, -2, 16, device="cuda")).requires_grad_()
@@ -796,6 +852,8 @@ def test_descendants(monkeypatch):
     some = plan.descendants(x, y, r, rows=[5, -1], targets=[1, -1], top=0, a=a, b=b)
     assert some.log_prob[0] == pytest.approx(np.log(cond[5, 1]), abs=1e-11) and some.log_prob[1] == 0
     assert some.top_index.shape == (2, 0)
+    none = plan.descendants(x, y, r, rows=[], top=3, a=a, b=b)
+    assert none.entropy.shape == (0,) and none.top_index.shape == (0, 3) and none.log_prob is None
     for bad in (dict(rows=[n]), dict(rows=[0], targets=[m])):
         with pytest.raises(IndexError):
             plan.descendants(x, y, r, a=a, b=b, **bad)

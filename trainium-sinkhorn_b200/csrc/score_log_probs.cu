@@ -2,18 +2,16 @@
 // each row, and the gradient. For row S, temperature T, m = max S, d_j = (S_j - m) / T:
 //     s = sum_j exp(d_j),  log p_j = d_j - log s,  H = log s - sum_j exp(d_j) d_j / s,  lse = m / T + log s
 //     dS_j = (1 / T) [ sum_t g_t (1[j = t] - p_j) + g_lse p_j - g_H p_j (log p_j + H) ]
-// The difference S - m is taken before the scaling, so rows whose scores are all the type's lowest value are uniform
-// rows and not overflow. Both terms of H are >= 0. A column of score -inf has p = 0 and adds nothing; a row without
-// any other column has lse = log p = -inf, H = 0 and gradient 0; NaN or +inf in a row makes its values NaN.
-// Sums in float32 (float64 for float64 scores).
+// Both terms of H are >= 0. A column of score -inf has p = 0 and adds nothing; a row without any other column has
+// lse = log p = -inf, H = 0 and gradient 0; NaN or +inf in a row makes its values NaN. Rows whose scores are all the
+// type's lowest value are uniform rows. Sums in float32 (float64 for float64 scores).
 //
-// Forward: one pass over the scores. A row belongs to one CTA, or to the CTAs of a cluster when there are few rows;
-// each thread works on 64 bytes of scores at a time, which it brings through shared memory itself (asynchronous copies,
-// two more chunks in flight, no barrier), and keeps its own state: the largest score
-// m, and with M = m c rounded (c = log2 e / T, or 1 / T in float64) the sums s = sum exp(x c - M) and
-// t = sum exp(x c - M) (x c - M), both rescaled when m rises. M is a shift like any other, so its rounding cancels. Rows
-// whose M would not be an ordinary number (scores near the type's lowest value throughout) are summed again by the
-// differences x - m.
+// Forward: one pass over the scores. A row belongs to one CTA of 1 to 8 warps, or to the CTAs of a cluster when there are
+// few rows; each thread works on 64 bytes of scores at a time, which it brings through shared memory itself (asynchronous
+// copies, one or two more chunks in flight, no barrier), and keeps its own state: the largest score m, and with M = m c
+// rounded (c = log2 e / T, or 1 / T in float64) the sums s = sum exp(x c - M) and t = sum exp(x c - M) (x c - M), both
+// rescaled when m rises. M is a shift like any other, so its rounding cancels. Rows whose M would not be an ordinary
+// number (scores near the type's lowest value throughout) are summed again by the differences x - m.
 // The best columns come out of the same pass: a bound below the K-th largest score is kept from the threads' running
 // maxima (the K / warps-th largest of each warp's 32: at least K scores reach the smallest of these), raised after 1, 2,
 // 4, 8, ... chunks, and each warp lists the few 16-byte vectors whose largest score reaches it. The K best scores lie in
@@ -313,8 +311,8 @@ __device__ __forceinline__ void chunk_sums(const Vec<T> (&q)[LP_VECS], A c, A M,
 }
 
 template <typename T, int NW, bool kTop>
-__global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_probs_kernel(LogProbsProblem p, int parts, typename Acc<T>::type c,
-                                                                                 typename Acc<T>::type inv_t) {
+__global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW)
+    log_probs_kernel(LogProbsProblem p, int parts, typename Acc<T>::type c, typename Acc<T>::type inv_t) {
   using A = typename Acc<T>::type;
   using B = typename Base<T>::type;
   using Smem = LogProbsSmem<T, NW, kTop>;
@@ -417,7 +415,8 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW) log_
         __syncwarp();
         const int n = *(volatile int*)&sh.count[w];
         if (n > LP_LIST) {
-          const Cut<A> r = cut_list<T, A>(from, NT, (int)(v + tid), &sh.list[w * LP_LIST], &sh.count[w], listed, own, p.top);
+          const Cut<A> r = cut_list<T, A>(from, NT, (int)(v + tid), &sh.list[w * LP_LIST], &sh.count[w], listed, own,
+                                          p.top);
           listed = r.n;
           own = r.own;
         } else {
