@@ -860,3 +860,12 @@ def test_descendants(monkeypatch):
     for bad in (dict(top=65), dict(rows=[0], targets=[0.5]), dict(rows=[0], targets=[0, 1])):
         with pytest.raises(ValueError):
             plan.descendants(x, y, r, a=a, b=b, **bad)
+
+
+def test_gradients_are_differentiable_once():
+    """A second derivative is refused when it is asked for; a graph of the first alone is fine."""
+    s = make(3, 20, torch.float32).requires_grad_()
+    for out in (scores.log_probs(s).entropy.sum(), scores.route(s, 2).weight[:, 0].sum()):
+        g, = torch.autograd.grad(out, s, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), s)

@@ -101,6 +101,12 @@ def _at(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+def _once(backward):
+    """A backward pass that cannot be differentiated itself: torch's guard, entered only where a graph of it is wanted."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+    return staticmethod(lambda ctx, *up: (guarded if torch.is_grad_enabled() else backward)(ctx, *up))
+
+
 # log_probs -----------------------------------------------------------------------------------------------------------
 
 def _log_probs_forward(s, lead, targets, n_targets, top, temperature, keep):
@@ -122,21 +128,21 @@ def _log_probs_forward(s, lead, targets, n_targets, top, temperature, keep):
 
 class _LogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, s, lead, targets, n_targets, top, temperature):
+    def forward(ctx, s, targets, call):
+        lead, n_targets, top, temperature = call
         log_prob, entropy, lse, top_log_prob, top_index, kept = _log_probs_forward(s, lead, targets, n_targets, top,
                                                                                    temperature, True)
         ctx.save_for_backward(s, targets, top_index, kept, entropy)
-        ctx.call = (n_targets, top, temperature)
+        ctx.call = call
         if top:
             ctx.mark_non_differentiable(top_index)
         ctx.set_materialize_grads(False)
         return log_prob, entropy, lse, top_log_prob, top_index
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, d_log_prob, d_entropy, d_lse, d_top, _):
         s, targets, top_index, kept, entropy = ctx.saved_tensors
-        n_targets, top, temperature = ctx.call
+        _, n_targets, top, temperature = ctx.call
         rows, cols = s.shape
         grad = s.new_empty((rows, cols))
         up = [None if d is None else d.contiguous() for d in (d_log_prob, d_entropy, d_lse, d_top)]
@@ -144,7 +150,7 @@ class _LogProbs(torch.autograd.Function):
         _call("trnopt_log_probs_grad", s.get_device(), _TYPE[s.dtype], s.data_ptr(), s.stride(0), rows, cols, temperature,
               _at(targets), n_targets, _at(top_index), top, row_max, row_max + rows * kept.element_size(),
               entropy.data_ptr(), *map(_at, up), grad.data_ptr(), cols)
-        return grad, None, None, None, None, None
+        return grad, None, None
 
 
 def log_probs(scores: torch.Tensor, targets: torch.Tensor | None = None, *, top: int = 0,
@@ -181,7 +187,7 @@ def log_probs(scores: torch.Tensor, targets: torch.Tensor | None = None, *, top:
         if targets.dtype != torch.int64 or not targets.is_contiguous():
             targets = targets.to(torch.int64).contiguous()
     if s.requires_grad and torch.is_grad_enabled():
-        return LogProbs(*_LogProbs.apply(s, lead, targets, n_targets, int(top), float(temperature)))
+        return LogProbs(*_LogProbs.apply(s, targets, (lead, n_targets, int(top), float(temperature))))
     return LogProbs(*_log_probs_forward(s, lead, targets, n_targets, int(top), float(temperature), False)[:5])
 
 
@@ -243,17 +249,16 @@ def _route_forward(s, lead, top, kind, bias, bias_on, groups, top_groups, group_
 
 class _Route(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, s, lead, top, kind, bias, bias_on, groups, top_groups, group_top, renormalize, scale, load):
-        index, weight, counts = _route_forward(s, lead, top, kind, bias, bias_on, groups, top_groups, group_top,
-                                               renormalize, scale, load)
+    def forward(ctx, s, *call):
+        index, weight, counts = _route_forward(s, *call)
+        _, top, kind, *_, renormalize, scale, _ = call
         ctx.save_for_backward(s, index)
         ctx.call = (top, kind, renormalize, scale)
         ctx.mark_non_differentiable(*((index,) if counts is None else (index, counts)))
         ctx.set_materialize_grads(False)
         return index, weight, counts
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, _, d_weight, *__):
         if d_weight is None:
             return (None,) * 12
