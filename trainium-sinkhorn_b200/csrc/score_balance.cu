@@ -25,7 +25,8 @@ constexpr size_t kCounterBytes = 256;
 
 }  // namespace
 
-// CTAs: one for problems that it takes in two steps, else up to one per SM with a step's rows each.
+// CTAs: one for problems that it takes in two steps, else up to one per SM with a step's rows each. Per iteration, one CTA
+// against several: 1024 x 24 (two steps) 3.5 / 4.2 us, 512 x 64 3.6 / 4.4 us, 2000 x 24 (four steps) 5.5 / 4.3 us.
 int balance_grid(int device, int rows, int cols) {
   const long long steps = ((long long)rows * lanes_per_row(cols) + kBalanceThreads - 1) / kBalanceThreads;
   if (steps <= 2) return 1;

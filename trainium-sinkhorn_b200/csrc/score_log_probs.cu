@@ -538,19 +538,19 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW)
     }
 }
 
-// Gradient: a CTA takes `chunks` x NT x LP_VECS vectors of one row, placed on the gradient's 16-byte boundaries, the next
-// chunk on its way while one is worked on. With the row's m and log s a score needs no sum: p (A + B log p), with
+// Gradient: a CTA of one warp takes `chunks` x 32 x LP_VECS vectors of one row, placed on the gradient's 16-byte
+// boundaries, the next chunk on its way while one is worked on. With the row's m and log s a score needs no sum: p (A + B log p), with
 // A = -(g + g_H H) / T, B = -g_H / T and g the sum of the upstream gradients of the row's given and best columns (less
 // that of lse). Those columns are written once more, by the first entry that names them, with the entries that repeat it
-// added in order. Bound by the two matrices' bytes: 8192 x 32768 bfloat16 (2 x 0.54 GB) about 175 us, 164 us at the copy rate.
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) log_probs_grad_kernel(LogProbsGradProblem p, int parts, int chunks,
-                                                                       typename Acc<T>::type c,
-                                                                       typename Acc<T>::type inv_t) {
+// added in order. Bound by the two matrices' bytes: 8192 x 32768 bfloat16 (2 x 0.54 GB) 171 us, 164 us at the copy
+// rate. (CTAs of 256 threads: 174 us, but 8192 x 1000 70 us against 12 us.)
+template <typename T>
+__global__ void __launch_bounds__(32, 32) log_probs_grad_kernel(LogProbsGradProblem p, int parts, int chunks,
+                                                               typename Acc<T>::type c, typename Acc<T>::type inv_t) {
   using A = typename Acc<T>::type;
   using B = typename Base<T>::type;
-  constexpr int kN = Vec<T>::kN, kChunk = NT * LP_VECS;
-  const int tid = threadIdx.x, lane = tid & 31;
+  constexpr int NT = 32, kN = Vec<T>::kN, kChunk = NT * LP_VECS;
+  const int lane = threadIdx.x;
   const long long row = blockIdx.x / (unsigned)parts;
   const long long v0 = (long long)(blockIdx.x - (unsigned)row * (unsigned)parts) * chunks * kChunk;
   const T* s = static_cast<const T*>(p.scores) + row * p.ld;
@@ -562,13 +562,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) log_probs_grad_kernel(LogProbsG
   const bool vectors = (reinterpret_cast<uintptr_t>(s + first) & 15) == 0;     // the scores' vectors fall together
   auto fetch = [&](Vec<T>(&q)[LP_VECS], long long v) {
     if (vectors && v + kChunk <= v1 && rv.inside(v, kChunk)) {
-      const T* at = s + rv.column(v + tid);
+      const T* at = s + rv.column(v + lane);
 #pragma unroll
       for (int i = 0; i < LP_VECS; ++i) q[i] = RowVectors<T>::read(at + i * NT * kN);
     } else {
 #pragma unroll
       for (int i = 0; i < LP_VECS; ++i) {
-        const long long at = v + i * NT + tid, j = rv.column(at);
+        const long long at = v + i * NT + lane, j = rv.column(at);
         if (vectors && at < v1 && rv.inside(at)) {
           q[i] = RowVectors<T>::read(s + j);
         } else {
@@ -630,13 +630,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) log_probs_grad_kernel(LogProbsG
       if (empty) q[i].q = make_uint4(0, 0, 0, 0);
     }
     if (v + kChunk <= v1 && rv.inside(v, kChunk)) {
-      T* at = out + rv.column(v + tid);
+      T* at = out + rv.column(v + lane);
 #pragma unroll
       for (int i = 0; i < LP_VECS; ++i) *reinterpret_cast<uint4*>(at + i * NT * kN) = q[i].q;
     } else {
 #pragma unroll
       for (int i = 0; i < LP_VECS; ++i) {
-        const long long at = v + i * NT + tid, j = rv.column(at);
+        const long long at = v + i * NT + lane, j = rv.column(at);
         if (at >= v1) continue;
         if (rv.inside(at)) {
           *reinterpret_cast<uint4*>(out + j) = q[i].q;
@@ -651,8 +651,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) log_probs_grad_kernel(LogProbsG
     for (int i = 0; i < LP_VECS; ++i) q[i] = next[i];
   }
   if (extra == 0 || empty) return;
-  __syncthreads();                                         // the named columns follow the CTA's others
-  for (int k = tid; k < extra; k += NT) {
+  __syncwarp();                                            // the named columns follow the CTA's others
+  for (int k = lane; k < extra; k += NT) {
     const long long j = column(k);
     if (j < 0 || j >= p.cols || j < first || j >= end) continue;
     bool again = false;
@@ -665,14 +665,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) log_probs_grad_kernel(LogProbsG
   }
 }
 
-// CTAs per row: a cluster where the rows alone leave places empty (4 CTAs of 8 warps per SM), as long as each CTA has a
-// chunk of its own.
+// CTAs per row: a cluster where the rows alone leave SMs empty, up to two CTAs per SM and as long as each CTA has a chunk of
+// its own. Measured with 1 / 2 / 4 / 8 CTAs per row, 131072 columns, 20 best: 1 row 21 / 16 / 12 / 12 us, 16 rows
+// 21 / 16 / 14 / 13 us, 64 rows 22 / 16 / 15 / 19 us.
 template <typename T, int NW>
 int row_parts(const LogProbsProblem& p) {
   const long long chunk = 32LL * NW * LP_VECS * Vec<T>::kN;
   int parts = 1;
   if (NW == 8)
-    while (parts < 8 && 2 * p.rows * parts <= 148 * 4 && (long long)p.cols > chunk * parts) parts *= 2;
+    while (parts < 8 && 2 * p.rows * parts <= 148 * 2 && (long long)p.cols > chunk * parts) parts *= 2;
   return parts;
 }
 
@@ -733,15 +734,16 @@ cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
   return p.top > 0 ? launch<T, 8, true>(p, stream) : launch<T, 8, false>(p, stream);
 }
 
-template <typename T, int NT>
+template <typename T>
 cudaError_t grad_launch(const LogProbsGradProblem& p, cudaStream_t stream) {
-  constexpr long long kCols = (long long)NT * LP_VECS * Vec<T>::kN;
+  constexpr long long kCols = 32LL * LP_VECS * Vec<T>::kN;
   // (a row may start inside a vector, and then reach into one more chunk)
   const bool aligned = p.ld_grad % Vec<T>::kN == 0 && reinterpret_cast<uintptr_t>(p.grad) % 16 == 0;
   const long long all = (p.cols + (aligned ? 0 : Vec<T>::kN - 1) + kCols - 1) / kCols;
-  // up to 4 chunks per CTA, which share the row's numbers, while there are CTAs for 6 rounds of the SMs' 4 places
+  // up to 4 chunks per CTA, which share the row's numbers, while that leaves 8 CTAs per SM: 8192 x 32768 with 1 / 4 / 16
+  // chunks 241 / 171 / 177 us, 100 x 50000 8 / 8 / 12 us
   int chunks = 1;
-  while (chunks < 4 && chunks < all && p.rows * ((all + 2 * chunks - 1) / (2 * chunks)) >= 148 * 24) chunks *= 2;
+  while (chunks < 4 && chunks < all && p.rows * ((all + 2 * chunks - 1) / (2 * chunks)) >= 148 * 8) chunks *= 2;
   const int parts = (int)((all + chunks - 1) / chunks);
   const long long per = (1LL << 30) / parts;
   const size_t size = sizeof(typename Acc<T>::type);
@@ -760,15 +762,10 @@ cudaError_t grad_launch(const LogProbsGradProblem& p, cudaStream_t stream) {
     q.d_entropy = at(p.d_entropy, r);
     q.d_lse = at(p.d_lse, r);
     q.d_top = at(p.d_top, r * p.top);
-    log_probs_grad_kernel<T, NT><<<(unsigned)(q.rows * parts), NT, 0, stream>>>(
+    log_probs_grad_kernel<T><<<(unsigned)(q.rows * parts), 32, 0, stream>>>(
         q, parts, chunks, Base<T>::type::scale(p.temperature), (typename Acc<T>::type)(1.0 / p.temperature));
   }
   return cudaGetLastError();
-}
-
-template <typename T>
-cudaError_t grad_launch(const LogProbsGradProblem& p, cudaStream_t stream) {
-  return p.cols <= 64 * LP_VECS * Vec<T>::kN ? grad_launch<T, 64>(p, stream) : grad_launch<T, 256>(p, stream);
 }
 
 }  // namespace
