@@ -802,6 +802,26 @@ def test_calls_on_two_streams_at_once():
             assert torch.equal(x, y)
 
 
+def test_large_balances_on_several_streams():
+    """Grids that fill the GPU each and wait within themselves, queued on three streams beside other work."""
+    from trnopt import _capi
+    s = [make(65536, 256, torch.bfloat16, seed=k, scale=1.0) for k in range(3)]
+    want = [scores.balance(x, eps=0.1, iters=4) for x in s]
+    m, other = make(4096, 4096, torch.bfloat16), torch.cuda.Stream()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        with torch.cuda.stream(other):
+            m @ m
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got.append((k, scores.balance(s[k], eps=0.1, iters=4)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(r.f, want[k].f) and torch.equal(r.g, want[k].g) for k, r in got)
+    assert _capi.device_error_flags() == 0
+
+
 def test_refusals():
     s = make(4, 10, torch.float32)
     t = torch.zeros(4, dtype=torch.int64, device="cuda")
