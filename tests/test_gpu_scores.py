@@ -223,6 +223,41 @@ def test_log_probs_offsets_past_32_bits():
     check_gradient(s, t, 2, 1.0)
 
 
+def test_log_probs_longest_row():
+    """2^31 - 1 columns, off a 16-byte boundary, with the gradient. A lane adds its scores in 32,768 chunks of 32 and the
+    lanes' sums are joined, so sums are off by GAMMA = 33,000 roundings at most (relative to sums of magnitudes)."""
+    cols, step = 2 ** 31 - 1, 1 << 26
+    buf = torch.randn(cols + 1, generator=gen(3), device="cuda", dtype=torch.bfloat16)
+    s = buf[1:].view(1, cols)
+    named = [cols - 1, 2 ** 30 + 3, 7]
+    s[0, named] = torch.tensor([20.0, 19.0, 18.0], dtype=torch.bfloat16, device="cuda")
+    s.requires_grad_()
+    targets = torch.tensor([[7, cols - 1, 2 ** 30 + 5, -1]], device="cuda")
+    r = scores.log_probs(s, targets, top=3)
+    total = weighted = 0.0
+    for j in range(0, cols, step):
+        d = s.detach()[0, j:j + step].double() - 20
+        e = d.exp()
+        total += float(e.sum())
+        weighted += float((e * d).sum())
+    lse, far = 20 + math.log(total), -weighted / total
+    sums = 33_000 * U
+    assert r.top_index.tolist() == [named]
+    assert abs(r.lse.item() - lse) <= sums + 64 * U
+    assert abs(r.entropy.item() - (math.log(total) + far)) <= 2 * sums * (1 + far)
+    log_p = s.detach()[0, [7, cols - 1, 2 ** 30 + 5]].double() - lse
+    assert (r.log_prob[0, :3].double() - log_p).abs().max() <= sums + 64 * U and r.log_prob[0, 3] == 0
+
+    up = torch.tensor([[0.25, 0.5, 0.125, 9.0]], device="cuda")         # the last one's target is padding
+    grad, = torch.autograd.grad((r.log_prob * up).sum() + r.lse.sum(), s)
+    for j in range(0, cols, step):
+        want = (s.detach()[0, j:j + step].double() - lse).exp() * (1 - 0.875)
+        for t, g in zip(targets[0, :3].tolist(), up[0].tolist()):
+            if j <= t < j + step:
+                want[t - j] += g
+        assert ((grad[0, j:j + step].double() - want).abs() <= want * (2.0 ** -8 + 2 * sums)).all()
+
+
 # gradient -------------------------------------------------------------------------------------------------------------
 
 def upstream(rows, n, dtype, seed):

@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW)
     // M is not an ordinary number: s and t once more, by the differences x - m
     past = 0;
     A s = 0, t = 0;
-    for (int j = tid; j < p.cols; j += NT) {
+    for (long long j = tid; j < p.cols; j += NT) {
       const A d = floored((widen(scores[j]) - a.m) * c), x = B::exp(d);
       s += x;
       t += x * d;
@@ -739,7 +739,7 @@ cudaError_t grad_launch(const LogProbsGradProblem& p, cudaStream_t stream) {
   constexpr long long kCols = 32LL * LP_VECS * Vec<T>::kN;
   // (a row may start inside a vector, and then reach into one more chunk)
   const bool aligned = p.ld_grad % Vec<T>::kN == 0 && reinterpret_cast<uintptr_t>(p.grad) % 16 == 0;
-  const long long all = (p.cols + (aligned ? 0 : Vec<T>::kN - 1) + kCols - 1) / kCols;
+  const long long all = ((long long)p.cols + (aligned ? 0 : Vec<T>::kN - 1) + kCols - 1) / kCols;
   // up to 4 chunks per CTA, which share the row's numbers, while that leaves 8 CTAs per SM: 8192 x 32768 with 1 / 4 / 16
   // chunks 241 / 171 / 177 us, 100 x 50000 8 / 8 / 12 us
   int chunks = 1;
