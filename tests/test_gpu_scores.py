@@ -447,6 +447,19 @@ def test_balance_more_rows_than_shared_memory_holds():
     check_balance(make(40000, 301, torch.bfloat16, scale=1.0), 0.3, 3)
 
 
+def test_balance_most_rows():
+    """2^31 - 1 rows of one column: f = -S and g = 0. Column sums are of 28,341 terms a lane, then of 512 lanes in 148
+    CTAs: N = 28,341 + 200 roundings at most, which move g by eps N u; f besides by three roundings of |S| log2(e) / eps."""
+    rows, eps = 2 ** 31 - 1, 0.5
+    s = torch.randn(rows, generator=gen(5), device="cuda", dtype=torch.bfloat16).view(rows, 1)
+    r = scores.balance(s, eps=eps, iters=3)
+    off = eps * 28_541 * U
+    assert r.g.abs().item() <= off
+    for i in range(0, rows, 1 << 28):
+        x = s[i:i + (1 << 28), 0].float()
+        assert ((r.f[i:i + (1 << 28)] + x).abs() <= off + 4 * U * x.abs()).all()
+
+
 def test_balance_marginals_agree_with_sinkhorn():
     """Converged potentials on S = -C are sinkhorn()'s up to its constant shift, and the plan's columns sum to b."""
     from trnopt import Backend, SinkhornOptions, sinkhorn

@@ -438,7 +438,7 @@ cudaError_t launch(int device, const BalanceProblem& p, const BalanceWork& wk, c
   // the rows a CTA keeps: all of them, or what shared memory holds (227 KB less what the launch itself takes)
   constexpr int G = 32 / L;
   const size_t fixed = fixed_bytes(p.cols), most = 226 * 1024 - fixed;
-  long long kept = ((p.rows + grid - 1) / grid + G - 1) / G * (long long)G;
+  long long kept = (((long long)p.rows + grid - 1) / grid + G - 1) / G * G;
   const long long fits = (long long)(most / row_bytes(p.cols, sizeof(T))) / G * G;
   if (kept > fits) kept = fits;
   const size_t bytes = fixed + (size_t)kept * row_bytes(p.cols, sizeof(T));
