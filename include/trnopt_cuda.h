@@ -339,6 +339,7 @@ int trnopt_balance(int type, const void* scores, long long ld, int rows, int col
  *               2) largest biased shares (bias on the logits: biased scores) stay open
  *   weight      scale * share, or with `renormalize` scale * share / (sum of the row's chosen shares)
  *   index, weight (rows, top), best first, equal keys by lower index; load (cols,) or NULL: rows that chose a column
+ *               (rows < 2^31)
  * Columns of score -inf are closed. Slots that no open column fills hold index -1, weight 0; a row with NaN or +inf (or
  * a NaN bias) chooses nothing: index -1, weight NaN. The order is that of the keys in 64 bits. Deterministic.
  * cols <= 1024, top <= 32, groups <= 32, types F32, F16, BF16. */

@@ -896,6 +896,14 @@ def test_refusals():
 
 # the plan's rows -----------------------------------------------------------------------------------------------------
 
+def test_refusals_of_too_many_rows():
+    s = torch.zeros(1, 8, device="cuda").expand(2 ** 31, 8)
+    with pytest.raises(ValueError, match="rows"):
+        scores.route(s, 1, load=True)
+    with pytest.raises(ValueError, match="rows"):
+        scores.balance(s)
+
+
 def test_descendants(monkeypatch):
     import numpy as np
     from oracle import trnopt_oracle as O

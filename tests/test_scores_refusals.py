@@ -108,3 +108,7 @@ def test_cpu_tensors_are_refused():
             call()
     with pytest.raises(ValueError):
         scores.log_probs([1.0, 2.0])
+
+
+def test_route_load_counts_in_32_bits():
+    assert route(rows=1 << 31, load=A) == INVALID

@@ -531,7 +531,7 @@ int trnopt_route(int type, const void* scores, long long ld, long long rows, int
       top > top_groups * (cols / groups) || group_top < 1 || group_top > 2 || !isfinite(scale) ||
       (kind != TRNOPT_ROUTE_SOFTMAX && kind != TRNOPT_ROUTE_SIGMOID) ||
       (bias_on != TRNOPT_ROUTE_BIAS_SCORES && bias_on != TRNOPT_ROUTE_BIAS_LOGITS) ||
-      (rows > 0 && (!index || !weight)))
+      (rows > 0 && (!index || !weight)) || (load && rows >= 1LL << 31))
     return TRNOPT_ERR_INVALID_ARGUMENT;
   if (!aligned(bias, 4) || !aligned(index, 8) || !aligned(weight, 4) || !aligned(load, 4)) return TRNOPT_ERR_ALIGNMENT;
   const RouteProblem p{scores, ld, rows, cols, top, kind, bias, bias_on, groups, top_groups, group_top, renormalize,

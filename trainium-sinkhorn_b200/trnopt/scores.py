@@ -15,8 +15,9 @@ log_probs(S) tells how decided the rows are. trnopt.plan.descendants applies log
 
 Scores are CUDA tensors of any leading shape and row pitch (a last dimension that is not contiguous is copied first).
 The calls queue on the scores' device, on that device's current stream, return without waiting, and can be captured into
-a CUDA graph. There is no CPU path. What a call rejects it rejects before anything is queued, with ValueError; values on
-the device (an index out of range, NaN) never raise and show in the results as described.
+a CUDA graph (backward() as torch asks for it: on a side stream, with no eager graph of the same leaves alive). There is
+no CPU path. What a call rejects it rejects before anything is queued, with ValueError; values on the device (an index
+out of range, NaN) never raise and show in the results as described.
 """
 
 from __future__ import annotations
@@ -283,7 +284,7 @@ def route(scores: torch.Tensor, top: int, *, kind: str = "softmax", bias: torch.
     groups       columns form `groups` equal runs; the `top_groups` (None: all) runs with the largest sum of their
                  `group_top` (1 or 2) largest biased shares (bias on the logits: biased scores) stay open
     weight       scale * share, or with renormalize scale * share / (sum of the row's chosen shares)
-    load         count the rows that chose each column
+    load         count the rows that chose each column (of fewer than 2**31 rows)
 
     scores are float32, float16 or bfloat16, of at most 1024 columns; top and groups are at most 32. The order is that
     of the keys in 64 bits, equal keys by lower index. Columns of score -inf are closed; slots that no open column fills
@@ -309,6 +310,8 @@ def route(scores: torch.Tensor, top: int, *, kind: str = "softmax", bias: torch.
         raise ValueError(f"top must lie in 1 .. {MAX_CHOICES} and not exceed the columns of the open groups")
     if not abs(scale) < 1e30:
         raise ValueError("scale must be finite")
+    if load and rows >= 2 ** 31:
+        raise ValueError("load counts fewer than 2**31 rows")
     bias = _small(bias, cols, "bias", s)
     forward = _Route.apply if s.requires_grad and torch.is_grad_enabled() else _route_forward
     return Routing(*forward(s, scores.shape[:-1], int(top), _KIND[kind], bias, _BIAS_ON[bias_on], int(groups),
