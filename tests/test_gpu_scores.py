@@ -258,6 +258,21 @@ def test_log_probs_longest_row():
         assert ((grad[0, j:j + step].double() - want).abs() <= want * (2.0 ** -8 + 2 * sums)).all()
 
 
+def test_log_probs_most_rows():
+    """More rows than one launch takes (2^30): the rows on both sides of the border, with the gradient of lse (p)."""
+    rows, border = 2 ** 30 + 37, 2 ** 30
+    s = torch.randn(rows, 2, generator=gen(6), device="cuda", dtype=torch.bfloat16).requires_grad_()
+    r = scores.log_probs(s)
+    grad, = torch.autograd.grad(r.lse, s, torch.ones_like(r.lse))
+    for part in (slice(0, 1000), slice(border - 1000, rows)):
+        x = s.detach()[part].double()
+        lse, p = x.logsumexp(-1), x.softmax(-1)
+        # lse = m + log(sum): sum in [1, 2], off by 8 roundings and ex2's 2 u; the sum of m and the log rounded once more
+        assert ((r.lse[part].detach().double() - lse).abs() <= (GAMMA + lse.abs()) * U).all()
+        assert ((r.entropy[part].detach().double() + (p * p.log()).sum(-1)).abs() <= 8 * GAMMA * U).all()
+        assert ((grad[part].double() - p).abs() <= p * (2.0 ** -8 + 32 * U)).all()
+
+
 # gradient -------------------------------------------------------------------------------------------------------------
 
 def upstream(rows, n, dtype, seed):
