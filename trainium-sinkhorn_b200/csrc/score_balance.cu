@@ -21,7 +21,8 @@ int sm_count(int device) {
   return n;
 }
 
-constexpr size_t kCounterBytes = 256;
+// the counter and the fixed-point sums
+size_t zeroed_bytes(int cols) { return 256 + (size_t)3 * ((cols + 3) & ~3) * sizeof(unsigned long long); }
 
 }  // namespace
 
@@ -35,15 +36,16 @@ int balance_grid(int device, int rows, int cols) {
 }
 
 size_t balance_workspace_bytes(int device, int rows, int cols) {
-  return kCounterBytes + (size_t)4 * balance_grid(device, rows, cols) * ((cols + 3) & ~3) * sizeof(float);
+  return zeroed_bytes(cols) + (size_t)4 * balance_grid(device, rows, cols) * ((cols + 3) & ~3) * sizeof(float);
 }
 
 cudaError_t balance_launch(int device, int type, const BalanceProblem& p, void* ws, cudaStream_t stream) {
-  const BalanceWork wk{static_cast<unsigned*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes),
-                       device_error_word(), p.b ? 0.0 : log2((double)p.cols),
+  char* const at = static_cast<char*>(ws);
+  const BalanceWork wk{reinterpret_cast<unsigned*>(at), reinterpret_cast<unsigned long long*>(at + 256),
+                       reinterpret_cast<float*>(at + zeroed_bytes(p.cols)), device_error_word(), p.b ? 0.0 : log2((double)p.cols),
                        (p.b ? 1.0 : (double)p.cols) / (p.a ? 1.0 : (double)p.rows)};
   if (balance_grid(device, p.rows, p.cols) > 1) {
-    const cudaError_t e = cudaMemsetAsync(ws, 0, sizeof(unsigned), stream);
+    const cudaError_t e = cudaMemsetAsync(ws, 0, zeroed_bytes(p.cols), stream);
     if (e != cudaSuccess) return e;
   }
   switch (type) {

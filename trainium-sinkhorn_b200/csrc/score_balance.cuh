@@ -72,6 +72,10 @@ __device__ __forceinline__ bool grid_barrier(unsigned* counter, unsigned target,
 
 constexpr int NT = kBalanceThreads, NW = NT / 32;
 
+// Fixed-point sums k_j 2^40 over the CTAs count from 2^-8, where 148 roundings are 2^-25 of them, to below 2^14. A part
+// that is larger (or NaN) adds 2^14 and so takes the sum out of that range.
+constexpr unsigned long long kTotalLeast = 1ull << 32, kTotalMost = 1ull << 54;
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -333,6 +337,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
     const size_t plane = (size_t)gridDim.x * cols4;
     float* sums = wk.parts + (size_t)(it & 1) * 2 * plane;
     float* peaks = sums + plane;
+    unsigned long long* totals = wk.totals + it % 3 * cols4;
     for (int j = tid; j < cols; j += NT) {
       float v = red[j];
 #pragma unroll
@@ -341,10 +346,17 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
         red[j] = v;                                         // (column j of `red` is this thread's alone)
       } else {
         __stcg(sums + (size_t)blockIdx.x * cols4 + j, v);
-        if (first) __stcg(peaks + (size_t)blockIdx.x * cols4 + j, v == 0.f ? -INFINITY : peaks_s[j]);
+        if (first) {
+          __stcg(peaks + (size_t)blockIdx.x * cols4 + j, v == 0.f ? -INFINITY : peaks_s[j]);
+        } else {
+          const double k = (double)v * per_b[j];
+          atomicAdd(totals + j, k < 0x1p14 ? (unsigned long long)__double2ll_rn(k * 0x1p40) : kTotalMost);
+        }
       }
     }
     int slices = 1;
+    unsigned long long total[2];
+    bool fixed = false;
     if (!alone) {
       if (!grid_barrier(wk.counter, (unsigned)(it + 1) * gridDim.x, wk.error_word, &flag)) {
         // gave up: no potentials
@@ -353,6 +365,20 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
           for (int j = tid; j < cols; j += NT) p.g[j] = NAN;
         return;
       }
+      // the fixed-point sums, where every column's is in their range; those of the last iteration, read by all, are cleared
+      if (blockIdx.x == 0 && !first)
+        for (int j = tid; j < cols; j += NT) __stcg(wk.totals + (it + 2) % 3 * cols4 + j, 0ull);
+      bool in_range = !first;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int j = tid + i * NT;
+        if (j >= cols || first) break;
+        total[i] = __ldcg(totals + j);
+        in_range = in_range && (!open[j] || (total[i] >= kTotalLeast && total[i] < kTotalMost));
+      }
+      fixed = __syncthreads_and(in_range);
+    }
+    if (!alone && !fixed) {
       // of all CTAs, in the same order in each: four columns per thread, the CTAs in `slices` interleaved parts
       const int quads = cols4 / 4, slice = tid / quads, quad = tid - slice * quads;
       slices = min(NT / quads, 16);                         // (few enough for the columns' threads to join)
@@ -399,7 +425,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
     for (int i = 0; i < 2; ++i) {
       const int j = tid + i * NT;
       if (j >= cols) break;
-      float2 v = alone ? make_float2(peaks_s[j], red[j]) : slice_sums[j];
+      float2 v = alone ? make_float2(peaks_s[j], red[j]) : fixed ? make_float2(0.f, 1.f) : slice_sums[j];
       if (first) {
         for (int k = 1; k < slices; ++k) lse2_add(v.x, v.y, slice_sums[(size_t)k * cols4 + j].x, slice_sums[(size_t)k * cols4 + j].y);
         open[j] = v.y != 0.f;
@@ -408,7 +434,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
 #pragma unroll 8
         for (int k = 1; k < slices; ++k) v.y += slice_sums[(size_t)k * cols4 + j].y;
         // k_j (a sum that underflows, for masses beyond float32's range from one another, counts as 2^-126)
-        const float step = log2_near_1(v.y == 0.f ? 0x1p-126 : (double)v.y * per_b[j]);
+        const float step = log2_near_1(fixed ? (double)total[i] * 0x1p-40 : v.y == 0.f ? 0x1p-126 : (double)v.y * per_b[j]);
         // the last potentials are not rounded to float32 before the common part goes back
         if (last && blockIdx.x == 0)
           p.g[j] = open[j] ? (float)(((double)us[j] - lb[j] - (double)step + shift) * eps_per) : 0.f;
