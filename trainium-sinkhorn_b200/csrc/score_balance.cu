@@ -36,7 +36,7 @@ int balance_grid(int device, int rows, int cols) {
 }
 
 size_t balance_workspace_bytes(int device, int rows, int cols) {
-  return zeroed_bytes(cols) + (size_t)4 * balance_grid(device, rows, cols) * ((cols + 3) & ~3) * sizeof(float);
+  return zeroed_bytes(cols) + (size_t)2 * balance_grid(device, rows, cols) * ((cols + 3) & ~3) * sizeof(float);
 }
 
 cudaError_t balance_launch(int device, int type, const BalanceProblem& p, void* ws, cudaStream_t stream) {

@@ -57,7 +57,7 @@ __device__ __forceinline__ bool grid_barrier(unsigned* counter, unsigned target,
     unsigned seen;
     for (;;) {
       asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
-      if (seen >= target) break;
+      if ((int)(seen - target) >= 0) break;                 // (the count may pass 2^32)
       if (globaltimer_ns() - t0 > kWaitLimitNs) {
         atomicOr(error_word, (int)kErrWaitTimeout);
         ok = 0;
@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
   for (int k = 0; k < C; ++k)
     if (column(k) < cols && p.b && p.b[column(k)] == 0.f) closed |= 1u << k;
 
+  unsigned arrivals = 0;                                    // at the grid's barrier, up to the next one's end
   for (int it = 0; it < p.iters; ++it) {
     const bool first = it == 0, last = it == p.iters - 1;
     float acc[C];
@@ -334,51 +335,55 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
     fold(Plus{});
 
     const bool alone = gridDim.x == 1;
-    const size_t plane = (size_t)gridDim.x * cols4;
-    float* sums = wk.parts + (size_t)(it & 1) * 2 * plane;
-    float* peaks = sums + plane;
     unsigned long long* totals = wk.totals + it % 3 * cols4;
-    for (int j = tid; j < cols; j += NT) {
+    unsigned long long total[2];
+    bool fixed = false;
+    auto column_sum = [&](int j) {
       float v = red[j];
 #pragma unroll
       for (int k = 1; k < NW; ++k) v += red[k * cols + j];
-      if (alone) {
-        red[j] = v;                                         // (column j of `red` is this thread's alone)
-      } else {
-        __stcg(sums + (size_t)blockIdx.x * cols4 + j, v);
-        if (first) {
-          __stcg(peaks + (size_t)blockIdx.x * cols4 + j, v == 0.f ? -INFINITY : peaks_s[j]);
-        } else {
-          const double k = (double)v * per_b[j];
-          atomicAdd(totals + j, k < 0x1p14 ? (unsigned long long)__double2ll_rn(k * 0x1p40) : kTotalMost);
-        }
+      return v;
+    };
+    auto barrier = [&]() {
+      arrivals += gridDim.x;
+      if (grid_barrier(wk.counter, arrivals, wk.error_word, &flag)) return true;
+      for (long long i = r0 + tid; i < r1; i += NT) p.f[i] = NAN;       // gave up: no potentials
+      if (blockIdx.x == 0)
+        for (int j = tid; j < cols; j += NT) p.g[j] = NAN;
+      return false;
+    };
+    if (alone) {
+      for (int j = tid; j < cols; j += NT) red[j] = column_sum(j);       // (column j of `red` is this thread's alone)
+    } else if (!first) {
+      for (int j = tid; j < cols; j += NT) {
+        const double k = (double)column_sum(j) * per_b[j];
+        atomicAdd(totals + j, k < 0x1p14 ? (unsigned long long)__double2ll_rn(k * 0x1p40) : kTotalMost);
       }
-    }
-    int slices = 1;
-    unsigned long long total[2];
-    bool fixed = false;
-    if (!alone) {
-      if (!grid_barrier(wk.counter, (unsigned)(it + 1) * gridDim.x, wk.error_word, &flag)) {
-        // gave up: no potentials
-        for (long long i = r0 + tid; i < r1; i += NT) p.f[i] = NAN;
-        if (blockIdx.x == 0)
-          for (int j = tid; j < cols; j += NT) p.g[j] = NAN;
-        return;
-      }
-      // the fixed-point sums, where every column's is in their range; those of the last iteration, read by all, are cleared
-      if (blockIdx.x == 0 && !first)
+      if (!barrier()) return;
+      // (those of the last iteration, which every CTA has read, are cleared)
+      if (blockIdx.x == 0)
         for (int j = tid; j < cols; j += NT) __stcg(wk.totals + (it + 2) % 3 * cols4 + j, 0ull);
-      bool in_range = !first;
+      fixed = true;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int j = tid + i * NT;
-        if (j >= cols || first) break;
+        if (j >= cols) break;
         total[i] = __ldcg(totals + j);
-        in_range = in_range && (!open[j] || (total[i] >= kTotalLeast && total[i] < kTotalMost));
+        fixed = fixed && (!open[j] || (total[i] >= kTotalLeast && total[i] < kTotalMost));
       }
-      fixed = __syncthreads_and(in_range);
+      fixed = __syncthreads_and(fixed);                     // the same in every CTA
     }
+    int slices = 1;
     if (!alone && !fixed) {
+      // the first iteration, and sums out of that range: every CTA's float32 sums, behind a barrier of their own
+      float* sums = wk.parts;
+      float* peaks = sums + (size_t)gridDim.x * cols4;
+      for (int j = tid; j < cols; j += NT) {
+        const float v = column_sum(j);
+        __stcg(sums + (size_t)blockIdx.x * cols4 + j, v);
+        if (first) __stcg(peaks + (size_t)blockIdx.x * cols4 + j, v == 0.f ? -INFINITY : peaks_s[j]);
+      }
+      if (!barrier()) return;
       // of all CTAs, in the same order in each: four columns per thread, the CTAs in `slices` interleaved parts
       const int quads = cols4 / 4, slice = tid / quads, quad = tid - slice * quads;
       slices = min(NT / quads, 16);                         // (few enough for the columns' threads to join)
