@@ -22,7 +22,7 @@ int sm_count(int device) {
 }
 
 // the counter and the fixed-point sums
-size_t zeroed_bytes(int cols) { return 256 + (size_t)3 * ((cols + 3) & ~3) * sizeof(unsigned long long); }
+size_t zeroed_bytes(int cols) { return 256 + (size_t)2 * ((cols + 3) & ~3) * sizeof(unsigned long long); }
 
 }  // namespace
 
@@ -31,7 +31,7 @@ size_t zeroed_bytes(int cols) { return 256 + (size_t)3 * ((cols + 3) & ~3) * siz
 int balance_grid(int device, int rows, int cols) {
   const long long steps = ((long long)rows * lanes_per_row(cols) + kBalanceThreads - 1) / kBalanceThreads;
   if (steps <= 2) return 1;
-  const int most = sm_count(device);
+  const int most = sm_count(device) < 255 ? sm_count(device) : 255;    // (counted in a byte)
   return steps < most ? (int)steps : most;
 }
 

@@ -16,12 +16,14 @@
 // One cooperative launch runs all iterations. A CTA owns a block of rows and keeps as many of them as fit in shared
 // memory as they were read in the first pass (the rest come from L2 in every pass). L neighbouring lanes share a row, up
 // to 32 columns each, so a row's maximum and sum take log2 L shuffles for the warp's 32 / L rows together, and a lane
-// sums its columns over its rows in registers. Per iteration the CTAs exchange their column sums through global memory
-// and one grid barrier, and each adds up all of them in the same order; what one CTA takes in two steps of its warps stays
-// in one, without the barrier. Bound by the pass's instructions for many rows, by the exchange's latency for few. Measured
-// per iteration: 65536 x 256 bfloat16 12.2 us (7 us the pass, of which 3.7 us are exponentials at 16 per clock and SM, the
-// rest the exchange), 65536 x 16 3.8 us, 8192 x 64 4.4 us, 509 x 24 in one CTA 2.2 us; a call of one iteration, which
-// passes twice and reads the scores from DRAM, 39 us for 65536 x 256.
+// sums its columns over its rows in registers. Per iteration the CTAs add their column sums up in fixed point, one atomic
+// addition of a 64-bit word per column and CTA: whole numbers, so their order does not matter, and the word counts the
+// CTAs, so there is no other barrier. (Every CTA's sums in float32, behind a barrier and added in the same order by all,
+// took 3 to 5 us of an iteration; they are left for the first one and for sums outside the fixed point's range.) What one
+// CTA takes in two steps of its warps stays in one. Bound by the pass's instructions for many rows, by the exchange's
+// latency for few. Measured per iteration: 65536 x 256 bfloat16 10.7 us (7 us the pass, of which 3.7 us are exponentials
+// at 16 per clock and SM, the rest the exchange), 65536 x 16 2.6 us, 8192 x 64 3.3 us, 509 x 24 in one CTA 2.2 us; a call
+// of one iteration, which passes twice and reads the scores from DRAM, 39 us for 65536 x 256.
 #pragma once
 
 #include <math.h>
@@ -72,9 +74,9 @@ __device__ __forceinline__ bool grid_barrier(unsigned* counter, unsigned target,
 
 constexpr int NT = kBalanceThreads, NW = NT / 32;
 
-// Fixed-point sums k_j 2^40 over the CTAs count from 2^-8, where 148 roundings are 2^-25 of them, to below 2^14. A part
-// that is larger (or NaN) adds 2^14 and so takes the sum out of that range.
-constexpr unsigned long long kTotalLeast = 1ull << 32, kTotalMost = 1ull << 54;
+// Fixed-point sums k_j 2^40 over the CTAs (at most 255, counted in the top byte) serve from 2^-8, where 148 roundings are
+// 2^-25 of them, to below 2^8. A part that is larger (or no number) adds 2^8 and so takes the sum out of that range.
+constexpr unsigned long long kTotalLeast = 1ull << 32, kTotalMost = 1ull << 48, kTotalOne = 1ull << 56;
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -153,6 +155,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
     if (j >= cols) us[j] = -INFINITY;
     peaks_s[j] = off_s[j] = 0.f;
   }
+  if (tid == 0) flag = 1;
   some_closed = __syncthreads_or(some_closed);
   unsigned closed = 0;                                      // the lane's columns of mass 0
 #pragma unroll
@@ -160,6 +163,9 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
     if (column(k) < cols && p.b && p.b[column(k)] == 0.f) closed |= 1u << k;
 
   unsigned arrivals = 0;                                    // at the grid's barrier, up to the next one's end
+  // The words of the fixed-point sums are never cleared: an iteration's sum is the difference to what the thread read two
+  // iterations ago (a CTA adds to a word again only when every CTA has read the one in between, and so this one before).
+  unsigned long long seen[2][2] = {{0, 0}, {0, 0}};
   for (int it = 0; it < p.iters; ++it) {
     const bool first = it == 0, last = it == p.iters - 1;
     float acc[C];
@@ -335,7 +341,6 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
     fold(Plus{});
 
     const bool alone = gridDim.x == 1;
-    unsigned long long* totals = wk.totals + it % 3 * cols4;
     unsigned long long total[2];
     bool fixed = false;
     auto column_sum = [&](int j) {
@@ -344,34 +349,53 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
       for (int k = 1; k < NW; ++k) v += red[k * cols + j];
       return v;
     };
-    auto barrier = [&]() {
-      arrivals += gridDim.x;
-      if (grid_barrier(wk.counter, arrivals, wk.error_word, &flag)) return true;
-      for (long long i = r0 + tid; i < r1; i += NT) p.f[i] = NAN;       // gave up: no potentials
+    auto gave_up = [&]() {                                  // no potentials
+      for (long long i = r0 + tid; i < r1; i += NT) p.f[i] = NAN;
       if (blockIdx.x == 0)
         for (int j = tid; j < cols; j += NT) p.g[j] = NAN;
-      return false;
     };
     if (alone) {
       for (int j = tid; j < cols; j += NT) red[j] = column_sum(j);       // (column j of `red` is this thread's alone)
     } else if (!first) {
+      // in fixed point: a column's word counts the CTAs in its top byte, so whoever reads it knows when it has all of them
+      unsigned long long* totals = wk.totals + (it & 1) * cols4;
       for (int j = tid; j < cols; j += NT) {
         const double k = (double)column_sum(j) * per_b[j];
-        atomicAdd(totals + j, k < 0x1p14 ? (unsigned long long)__double2ll_rn(k * 0x1p40) : kTotalMost);
+        atomicAdd(totals + j, kTotalOne + (k >= 0.0 && k < 0x1p8 ? (unsigned long long)__double2ll_rn(k * 0x1p40) : kTotalMost));
       }
-      if (!barrier()) return;
-      // (those of the last iteration, which every CTA has read, are cleared)
-      if (blockIdx.x == 0)
-        for (int j = tid; j < cols; j += NT) __stcg(wk.totals + (it + 2) % 3 * cols4 + j, 0ull);
+      const unsigned long long t0 = globaltimer_ns();
+      auto complete = [&](int i) {                          // the thread's i-th word, once every CTA has added to it
+        unsigned long long now;
+        for (unsigned spin = 1;; ++spin) {
+          asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(now) : "l"(totals + tid + i * NT) : "memory");
+          if ((now - seen[it & 1][i]) / kTotalOne == gridDim.x) break;
+          if (spin % 64 == 0 && globaltimer_ns() - t0 > kWaitLimitNs) {
+            atomicOr(wk.error_word, (int)kErrWaitTimeout);
+            flag = 0;
+            break;
+          }
+        }
+        return now;
+      };
+      // One lane per warp waits for its own first where many threads would wait: their reads hold up the sums that are to
+      // come. Per iteration so / all at once: 65536 x 256 10.7 / 11.7 us, 65536 x 64 4.7 / 5.1 us, but 65536 x 16
+      // 2.7 / 2.6 us, 8192 x 64 (32 CTAs) 3.5 / 3.3 us.
+      if (cols * (int)gridDim.x > 4096) {
+        if (lane == 0 && tid < cols) complete(0);
+        __syncwarp();
+      }
       fixed = true;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int j = tid + i * NT;
         if (j >= cols) break;
-        total[i] = __ldcg(totals + j);
+        const unsigned long long now = complete(i);
+        total[i] = (now - seen[it & 1][i]) % kTotalOne;
+        seen[it & 1][i] = now;
         fixed = fixed && (!open[j] || (total[i] >= kTotalLeast && total[i] < kTotalMost));
       }
       fixed = __syncthreads_and(fixed);                     // the same in every CTA
+      if (!flag) return gave_up();
     }
     int slices = 1;
     if (!alone && !fixed) {
@@ -383,7 +407,8 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
         __stcg(sums + (size_t)blockIdx.x * cols4 + j, v);
         if (first) __stcg(peaks + (size_t)blockIdx.x * cols4 + j, v == 0.f ? -INFINITY : peaks_s[j]);
       }
-      if (!barrier()) return;
+      arrivals += gridDim.x;
+      if (!grid_barrier(wk.counter, arrivals, wk.error_word, &flag)) return gave_up();
       // of all CTAs, in the same order in each: four columns per thread, the CTAs in `slices` interleaved parts
       const int quads = cols4 / 4, slice = tid / quads, quad = tid - slice * quads;
       slices = min(NT / quads, 16);                         // (few enough for the columns' threads to join)

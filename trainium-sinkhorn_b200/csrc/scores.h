@@ -47,7 +47,7 @@ struct BalanceProblem {
 
 struct BalanceWork {
   unsigned* counter;       // arrivals at the barrier, 0 at the start
-  unsigned long long* totals;  // (3, cols rounded up to 4): by iteration, k_j in units of 2^-40, 0 at the start
+  unsigned long long* totals;  // (2, cols rounded up to 4): by parity, k_j in units of 2^-40, 0 at the start
   float* parts;            // (2, CTAs, cols rounded up to 4): the CTAs' column sums, and their maxima in the first iteration
   int* error_word;
   double log_cols, k_scale;  // log2 cols and cols / rows for uniform masses, where rows are summed without 1 / cols and
