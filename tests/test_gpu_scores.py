@@ -462,6 +462,38 @@ def test_balance_more_rows_than_shared_memory_holds():
     check_balance(make(40000, 301, torch.bfloat16, scale=1.0), 0.3, 3)
 
 
+@pytest.mark.parametrize("rows,cols", [(5000, 16), (3001, 100), (40000, 256), (700, 1000)])
+def test_balance_far_columns_over_several_ctas(rows, cols):
+    """Sums far from 1 in the first iterations, which the CTAs do not exchange in fixed point, and near 1 later."""
+    far = torch.linspace(-40, 0, cols, device="cuda")[torch.randperm(cols, generator=gen(0), device="cuda")]
+    s = make(rows, cols, torch.float32, scale=0.5) + far
+    s[: rows // 3] += 2 * far.flip(0)                      # (two kinds of rows: iterations that do not converge at once)
+    for iters in (2, 3, 4, 9):
+        check_balance(s, 0.5, iters)
+    check_balance(s, 0.5, 3, g=torch.linspace(3, -60, cols, device="cuda"))
+
+
+@pytest.mark.parametrize("rows,cols", [(5000, 16), (30000, 90), (2000, 1000)])
+def test_balance_masses_and_masks_over_several_ctas(rows, cols):
+    s = make(rows, cols, torch.bfloat16, scale=1.0)
+    a = torch.rand(rows, generator=gen(1), device="cuda")
+    a[-rows // 5:] = 0
+    b = torch.rand(cols, generator=gen(2), device="cuda") ** 4 + 1e-6
+    b[7] = 0
+    g = 0.1 * make(1, cols, torch.float32)[0]
+    check_balance(s, 0.2, 6, a / a.sum(), b / b.sum(), g)
+    check_balance(s, 0.2, 6, 1000 * a / a.sum(), b / b.sum(), g)        # sums that do not agree: k = 1000 throughout
+    s[40] = -INF
+    s[:, 3] = -INF
+    s[::2, 5] = -INF
+    check_balance(s, 0.2, 6)
+    check_balance(s, 0.2, 6, a / a.sum(), b / b.sum(), g)
+    check_balance(torch.full((rows, cols), -INF, device="cuda"), 0.2, 3)
+    s[rows // 2, 2] = float("nan")
+    r = scores.balance(s, eps=0.2, iters=4)
+    assert r.g[2].isnan() and r.f[rows // 2].isnan()
+
+
 def test_balance_most_rows():
     """2^31 - 1 rows of one column: f = -S and g = 0. Column sums are of 28,341 terms a lane, then of 512 lanes in 148
     CTAs: N = 28,341 + 200 roundings at most, which move g by eps N u; f besides by three roundings of |S| log2(e) / eps."""
