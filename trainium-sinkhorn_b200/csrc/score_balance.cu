@@ -26,8 +26,9 @@ size_t zeroed_bytes(int cols) { return 256 + (size_t)2 * ((cols + 3) & ~3) * siz
 
 }  // namespace
 
-// CTAs: one for problems that it takes in two steps, else up to one per SM with a step's rows each. Per iteration, one CTA
-// against several: 1024 x 24 (two steps) 3.5 / 4.2 us, 512 x 64 3.6 / 4.4 us, 2000 x 24 (four steps) 5.5 / 4.3 us.
+// CTAs: one for problems that it takes in two steps, else up to one per SM with a step's rows each. Two steps in one CTA
+// against two CTAs: 2 iterations of 1000 x 8 8.2 / 12.3 us, of 512 x 64 16.4 / 17.8 us; 12 iterations 25 / 29 us and
+// 51 / 48 us. (Four steps in one CTA, 2000 x 24: 5.5 us an iteration; four CTAs' steps cost 3 us.)
 int balance_grid(int device, int rows, int cols) {
   const long long steps = ((long long)rows * lanes_per_row(cols) + kBalanceThreads - 1) / kBalanceThreads;
   if (steps <= 2) return 1;
