@@ -1,0 +1,97 @@
+"""The score-matrix operators where single rows, columns or sizes lie far from the others: finite masks, masses of zero,
+infinite starting potentials, far scores and small temperatures. Against 64-bit formulas, as in test_gpu_scores.py, but with
+a tolerance per row and column from that row's or column's own size."""
+
+import math
+
+import pytest
+import torch
+
+from trnopt import scores
+from test_gpu_scores import GAMMA, INF, U, close, gen, make
+
+pytestmark = pytest.mark.gpu
+
+
+# balance -------------------------------------------------------------------------------------------------------------
+
+def reference(s, eps, iters, a, b, g):
+    """The half-steps in 64 bits. A constant added to a row only moves its f by the same amount back, so each row's largest
+    finite score is taken off first; a row or column without terms has potential 0."""
+    s = s.double()
+    n, e = s.shape
+    top = torch.where(torch.isfinite(s), s, -INF).amax(1)
+    top = torch.where(top == -INF, 0.0, top)
+    s = s - top[:, None]
+    la = torch.full((n,), -math.log(n), dtype=torch.float64, device="cuda") if a is None else a.double().log()
+    lb = torch.full((e,), -math.log(e), dtype=torch.float64, device="cuda") if b is None else b.double().log()
+    g = torch.zeros(e, dtype=torch.float64, device="cuda") if g is None else g.double()
+    for _ in range(iters):
+        f = -eps * torch.logsumexp(lb + (g + s) / eps, 1)
+        f = torch.where(torch.isinf(f), top, f)                  # (0 once the row's constant is back)
+        g = -eps * torch.logsumexp(la[:, None] + (f[:, None] + s) / eps, 0)
+        g = torch.where(torch.isinf(g), 0.0, g)
+    return f - top, g, s
+
+
+def check(s, eps, iters, a=None, b=None, g=None, far=()):
+    """`far`: columns whose scores or potentials lie far from the others'. As in test_gpu_scores.py each of the 2 iters
+    half-steps adds the roundings of terms of size z (now over the ordinary columns, relative to each row's largest score)
+    and of a sum's chain; a potential itself rounds to float32, and a far column's terms round by their own size."""
+    r = scores.balance(s, eps=eps, iters=iters, a=a, b=b, g=g)
+    f, w, rest = reference(s, eps, iters, a, b, g)
+    near = torch.ones(s.shape[1], dtype=torch.bool, device="cuda")
+    near[list(far)] = False
+    rest = rest[:, near]
+    top = lambda t: torch.where(torch.isfinite(t), t, 0.0).abs().max().item()
+    base = rest + f[:, None] * 0
+    size = (top(base) + top(w[near]) + (0 if g is None else top(g.double()[near]))) / eps + 16
+    tol = U * eps * 2 * iters * (4 * size + GAMMA + max(s.shape) / 32)
+    fin = lambda t: torch.where(torch.isfinite(t), t, 0.0).abs()
+    close(r.f, f, tol + 8 * U * fin(f), "f")
+    close(r.g[near], w[near], tol + 8 * U * fin(w[near]), "g")
+    close(r.g[~near], w[~near], tol + 8 * U * fin(w[~near]) + 8 * U * (0 if g is None else fin(g.double()[~near])), "far g")
+    return r
+
+
+SHAPES = [(400, 16), (1000, 24), (20000, 16), (3000, 64), (6000, 200)]
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("iters", [1, 2, 3, 9])
+@pytest.mark.parametrize("low", [-25.0, -400.0, 25.0])
+def test_balance_zero_masses_far_apart(rows, cols, iters, low):
+    """Rows of mass 0 send nothing, however far a column of mass 0 lies above their others; it still gets its potential."""
+    s = make(rows, cols, torch.float32, seed=rows, scale=1.0)
+    a, b = torch.ones(rows, device="cuda"), torch.ones(cols, device="cuda")
+    a[1::7] = 0
+    b[[5, cols - 2]] = 0
+    s[1::7] += low
+    s[1::7, 5] -= low
+    check(s, 0.25, iters, a / a.sum(), b / b.sum())
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("start", [-6.0, 0.0, 6.0])
+@pytest.mark.parametrize("iters", [1, 2, 7])
+def test_balance_rows_open_to_columns_without_mass(rows, cols, start, iters):
+    """Rows whose only scores are on columns of mass 0 have potential 0, and their terms reach those columns, whether the
+    others' potentials lie far above or below."""
+    s = make(rows, cols, torch.float32, seed=rows, scale=0.5)
+    b = torch.ones(cols, device="cuda")
+    b[[2, 6]] = 0
+    shut = torch.ones(cols, dtype=torch.bool, device="cuda")
+    shut[[2, 6]] = False
+    for row in (4, 5, rows - 1):
+        s[row, shut] = -INF
+    s[11] = -INF
+    check(s, 0.05, iters, None, b / b.sum(), torch.full((cols,), start, device="cuda"), far=[2, 6])
+
+
+def test_balance_tiny_masses():
+    s = make(900, 12, torch.float32, scale=1.0)
+    a, b = torch.rand(900, generator=gen(1), device="cuda"), torch.ones(12, device="cuda")
+    a[5::9] *= 1e-36
+    b[3] = 0
+    s[5::9, 3] += 20.0
+    check(s, 0.3, 6, a / a.sum(), b / b.sum())

@@ -143,13 +143,16 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
 
   // what float32 potentials are relative to: 0, or the given potential of column 0; later its potential after one iteration
   double shift = p.g0 && fabsf(p.g0[0]) < INFINITY ? (double)p.g0[0] * per_eps : 0.0;
-  bool some_closed = false;                                 // columns of mass 0: out of the rows' sums, log2 b = 0
+  // Columns of mass 0 add nothing to the rows' sums, so their potentials matter to nobody else: they are found in the last
+  // iteration, from its f, like the first iteration's from any g (every column's maximum before its sum: nothing keeps such
+  // a column's terms below the rows' maxima).
+  bool some_closed = false;
   for (int j = tid; j < cols; j += NT) {
     const float b = p.b ? p.b[j] : 1.f;                     // (1 / cols each: log2 cols in a row's sum instead)
     some_closed = some_closed || b == 0.f;
     lb[j] = b == 0.f || b == 1.f ? 0.0 : log2((double)b);
     per_b[j] = b == 0.f ? wk.k_scale : wk.k_scale / (double)b;
-    us[j] = (float)((p.g0 ? (double)p.g0[j] * per_eps - shift : 0.0) + lb[j]);
+    us[j] = b == 0.f ? 0.f : (float)((p.g0 ? (double)p.g0[j] * per_eps - shift : 0.0) + lb[j]);
   }
   for (int j = tid; j < L * 32; j += NT) {
     if (j >= cols) us[j] = -INFINITY;
@@ -167,9 +170,10 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
   // iterations ago (a CTA adds to a word again only when every CTA has read the one in between, and so this one before).
   unsigned long long seen[2][2] = {{0, 0}, {0, 0}};
   for (int it = 0; it < p.iters; ++it) {
-    const bool first = it == 0, last = it == p.iters - 1;
+    const bool first = it == 0, last = it == p.iters - 1, maxima = first || (last && some_closed);
     float acc[C];
-    // Modes: 0 column sums; in the first iteration 1 the columns' maxima and then 2 their sums relative to those.
+    // Modes: 0 column sums, without the columns of mass 0 (u = -inf); or, where the columns' maxima are found, 1 these and
+    // then 2 the sums relative to them, of all columns (u = 0 for those of mass 0, which the rows' sums leave out).
     auto pass = [&](auto mode_, auto closed_) {
       constexpr int kMode = decltype(mode_)::value;
       constexpr bool kClosed = decltype(closed_)::value;
@@ -197,7 +201,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
             if (at < cols && (L == 1 || at + q * V < cols)) read(v[r], at);
           }
         };
-        if (kMode != 1 && keep) {
+        if (keep && !(kMode == 1 && first)) {
           runs([&](Vec<T>& x, int at) { x = *reinterpret_cast<const Vec<T>*>(here + at); });
         } else {
           if (vectors) {
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
                 if (at + q * V + i < cols) x.set(i, s[at + i]);
             });
           }
-          if (kMode == 1 && keep) {
+          if (kMode == 1 && keep && first) {
 #pragma unroll
             for (int r = 0; r < C / V; ++r)
               if (r * L * V + q * V < cols) *reinterpret_cast<Vec<T>*>(here + r * L * V) = v[r];
@@ -250,26 +254,14 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
 #pragma unroll
         for (int o = 1; o < L; o *= 2) l += __shfl_xor_sync(kAll, l, o);
         const float a = !there ? 0.f : masses ? __ldg(masses + row) : 1.f;
-        const bool empty = l == 0.f;                        // f = 0: the terms 2^(S c + u) as they are
+        const bool empty = l == 0.f;                        // f = 0
         if (kMode != 1 && last && q == 0 && there)
           p.f[r0 + row] = empty ? 0.f : (float)((wk.log_cols - ((double)m + (double)log2f(l) + shift)) * eps_per);
         if constexpr (kMode == 0) {
-          if (!__any_sync(kAll, empty && a != 0.f)) {
-            const float weight = empty ? 0.f : a / l;
-            const uint64_t w2 = pack2(weight, weight);
+          const float weight = empty ? 0.f : a / l;         // (an empty row's terms are 0: no column of mass 0 is among them)
+          const uint64_t w2 = pack2(weight, weight);
 #pragma unroll
-            for (int k = 0; k < C / 2; ++k) acc2[k] = fma2(z2[k], w2, acc2[k]);
-          } else if (a != 0.f) {
-#pragma unroll
-            for (int k = 0; k < C; k += 2) {
-              float x, y;
-              unpack2(z2[k / 2], x, y);
-              auto term = [&](float e) {
-                return !empty ? e * (a / l) : e > 0.f ? a * exp2f(log2f(e) + ((float)shift - log_cols)) : 0.f;
-              };
-              acc2[k / 2] = add2(acc2[k / 2], pack2(term(x), term(y)));
-            }
-          }
+          for (int k = 0; k < C / 2; ++k) acc2[k] = fma2(z2[k], w2, acc2[k]);
         } else {
           // x = S c + f c + log2 a, in the gauge of u - shift: z - u - log2 l + log2 a (and log2 cols, as in mode 0); mode 2
           // takes it relative to the column's maximum, off_s = -u - maximum. (Columns with u = -inf: no number, passed over
@@ -319,7 +311,12 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
         if (k < have && column(from + k) < cols) red[w * cols + column(from + k)] = acc[k];
       __syncthreads();
     };
-    if (first) {
+    if (maxima) {
+      if (!first) {
+        for (int j = tid; j < cols; j += NT)
+          if (p.b[j] == 0.f) us[j] = 0.f;
+        __syncthreads();
+      }
       if (some_closed) pass(std::integral_constant<int, 1>{}, std::true_type{});
       else pass(std::integral_constant<int, 1>{}, std::false_type{});
       fold(Larger{});
@@ -333,8 +330,6 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
       __syncthreads();
       if (some_closed) pass(std::integral_constant<int, 2>{}, std::true_type{});
       else pass(std::integral_constant<int, 2>{}, std::false_type{});
-    } else if (some_closed) {
-      pass(std::integral_constant<int, 0>{}, std::true_type{});
     } else {
       pass(std::integral_constant<int, 0>{}, std::false_type{});
     }
@@ -356,7 +351,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
     };
     if (alone) {
       for (int j = tid; j < cols; j += NT) red[j] = column_sum(j);       // (column j of `red` is this thread's alone)
-    } else if (!first) {
+    } else if (!maxima) {
       // in fixed point: a column's word counts the CTAs in its top byte, so whoever reads it knows when it has all of them
       unsigned long long* totals = wk.totals + (it & 1) * cols4;
       for (int j = tid; j < cols; j += NT) {
@@ -399,13 +394,18 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
     }
     int slices = 1;
     if (!alone && !fixed) {
-      // the first iteration, and sums out of that range: every CTA's float32 sums, behind a barrier of their own
+      // iterations with maxima, and sums out of that range: every CTA's float32 sums, behind a barrier of their own (and where
+      // no fixed-point sums came before, behind one more: the other CTAs may still read the last ones)
+      if (maxima && !first) {
+        arrivals += gridDim.x;
+        if (!grid_barrier(wk.counter, arrivals, wk.error_word, &flag)) return gave_up();
+      }
       float* sums = wk.parts;
       float* peaks = sums + (size_t)gridDim.x * cols4;
       for (int j = tid; j < cols; j += NT) {
         const float v = column_sum(j);
         __stcg(sums + (size_t)blockIdx.x * cols4 + j, v);
-        if (first) __stcg(peaks + (size_t)blockIdx.x * cols4 + j, v == 0.f ? -INFINITY : peaks_s[j]);
+        if (maxima) __stcg(peaks + (size_t)blockIdx.x * cols4 + j, v == 0.f ? -INFINITY : peaks_s[j]);
       }
       arrivals += gridDim.x;
       if (!grid_barrier(wk.counter, arrivals, wk.error_word, &flag)) return gave_up();
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
       float2* part = slice_sums + (size_t)slice * cols4 + 4 * quad;     // (`red` is free again)
       if (slice < slices) {
         float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (first) {
+        if (maxima) {
 #pragma unroll 4
           for (int k = slice; k < (int)gridDim.x; k += slices) {
             const float4 om = __ldcg(reinterpret_cast<const float4*>(peaks + (size_t)k * cols4) + quad);
@@ -449,17 +449,18 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
       }
       __syncthreads();
     }
-    double full[2];                                         // first iteration: u of the thread's columns (at most 2)
+    double full[2];                                         // with maxima: u of the thread's columns (at most 2)
     double* base = reinterpret_cast<double*>(&slice_sums[0]);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int j = tid + i * NT;
       if (j >= cols) break;
       float2 v = alone ? make_float2(peaks_s[j], red[j]) : fixed ? make_float2(0.f, 1.f) : slice_sums[j];
-      if (first) {
+      if (maxima) {
         for (int k = 1; k < slices; ++k) lse2_add(v.x, v.y, slice_sums[(size_t)k * cols4 + j].x, slice_sums[(size_t)k * cols4 + j].y);
-        open[j] = v.y != 0.f;
+        open[j] = v.y != 0.f && !(p.b && p.b[j] == 0.f);    // takes part from here on
         full[i] = v.y == 0.f ? 0.0 : shift - ((double)v.x + log2((double)v.y * wk.k_scale));
+        if (last && blockIdx.x == 0) p.g[j] = (float)(full[i] * eps_per);
       } else {
 #pragma unroll 8
         for (int k = 1; k < slices; ++k) v.y += slice_sums[(size_t)k * cols4 + j].y;
@@ -480,8 +481,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
       for (int i = 0; i < 2; ++i) {
         const int j = tid + i * NT;
         if (j >= cols) break;
-        us[j] = (float)(full[i] - shift + lb[j]);
-        if (last && blockIdx.x == 0) p.g[j] = (float)(full[i] * eps_per);
+        us[j] = p.b && p.b[j] == 0.f ? -INFINITY : (float)(full[i] - shift + lb[j]);
       }
     }
     __syncthreads();
