@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from trnopt import scores
-from test_gpu_scores import GAMMA, INF, U, close, gen, make
+from test_gpu_scores import GAMMA, INF, TYPES, U, close, gen, make
 
 pytestmark = pytest.mark.gpu
 
@@ -55,6 +55,59 @@ def check(s, eps, iters, a=None, b=None, g=None, far=()):
 
 
 SHAPES = [(400, 16), (1000, 24), (20000, 16), (3000, 64), (6000, 200)]
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("column", [0, 5, -1])
+@pytest.mark.parametrize("value,eps,dtype", [(-1e4, 0.1, "f32"), (-65504.0, 0.1, "f16"), (-65504.0, 0.02, "f32"),
+                                             (-3.3895e38, 2.0, "bf16")])
+def test_balance_masked_column_without_mass(rows, cols, column, value, eps, dtype):
+    """A column of mass 0 closed by a large finite score."""
+    s = make(rows, cols, TYPES[dtype], seed=rows, scale=1.0)
+    s[:, column] = value
+    b = torch.full((cols,), 1 / (cols - 1), device="cuda")
+    b[column] = 0
+    for iters in (1, 2, 8):
+        check(s, eps, iters, None, b, far=[column])
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("column", [0, 5])
+@pytest.mark.parametrize("value,eps,dtype", [(-1e4, 0.1, "f32"), (-65504.0, 0.1, "bf16"), (3e4, 0.5, "f16")])
+def test_balance_far_column_with_mass(rows, cols, column, value, eps, dtype):
+    """Its potential makes up for the scores; the others' keep their accuracy."""
+    s = make(rows, cols, TYPES[dtype], seed=rows, scale=1.0)
+    s[:, column] = value
+    for iters in (1, 2, 8):
+        check(s, eps, iters, far=[column])
+    check(s, eps, 3, g=torch.where(torch.arange(cols, device="cuda") == column, -value, 0.5), far=[column])
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_balance_far_rows(rows, cols, dtype):
+    """Rows of nothing but the lowest value or -65504, and rows far above: a row's constant does not move the columns."""
+    s = make(rows, cols, TYPES[dtype], seed=rows, scale=1.0)
+    s[3::50] = -65504.0
+    s[7::50] = torch.finfo(s.dtype).min
+    s[9::50] += 30000.0
+    s[11::50, 1::2] = torch.finfo(s.dtype).min
+    for iters in (1, 2, 8):
+        check(s, 0.1, iters)
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_balance_scores_below_the_range_close_a_column(rows, cols):
+    """Scores whose multiple by log2(e) / eps passes float32's range are as good as -inf."""
+    s = make(rows, cols, torch.bfloat16, seed=rows, scale=1.0)
+    b = torch.rand(cols, generator=gen(1), device="cuda") + 0.5
+    b[0] = 0
+    for column in (0, 5):
+        x, y = s.clone(), s.clone()
+        x[:, column], y[:, column] = torch.finfo(torch.bfloat16).min, -INF
+        for iters in (1, 3):
+            u, v = (scores.balance(z, eps=0.1, iters=iters, b=b / b.sum()) for z in (x, y))
+            assert torch.equal(u.f, v.f) and torch.equal(u.g, v.g) and u.g[column] == 0
 
 
 @pytest.mark.parametrize("rows,cols", SHAPES)
