@@ -148,3 +148,26 @@ def test_balance_tiny_masses():
     b[3] = 0
     s[5::9, 3] += 20.0
     check(s, 0.3, 6, a / a.sum(), b / b.sum())
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("iters", [1, 2, 6])
+@pytest.mark.parametrize("mass", [True, False])
+def test_balance_start_of_minus_infinity(rows, cols, iters, mass):
+    """g = -inf leaves a column out of the first row sums only."""
+    s = make(rows, cols, torch.bfloat16, seed=rows, scale=1.0)
+    g = 0.3 * make(1, cols, torch.float32, seed=2)[0]
+    g[[0, 7]] = -INF
+    b = torch.rand(cols, generator=gen(3), device="cuda") + 0.5
+    if not mass:
+        b[7] = 0
+    check(s, 0.2, iters, None, b / b.sum(), g)
+
+
+def test_balance_start_that_is_no_number():
+    s = make(700, 16, torch.float32, scale=1.0)
+    for bad in (math.nan, INF):
+        g = torch.zeros(16, device="cuda")
+        g[3] = bad
+        r = scores.balance(s, eps=0.2, iters=2, g=g)
+        assert torch.isnan(r.f).all() and torch.isnan(r.g).all()

@@ -158,7 +158,7 @@ __host__ __device__ inline size_t exchange_bytes(int cols) {
 }
 __host__ __device__ inline size_t fixed_bytes(int cols) {
   const size_t pad = (size_t)lanes_per_row(cols) * 32;
-  return (exchange_bytes(cols) + 4 * pad * sizeof(float) + cols * (2 * sizeof(double) + 1) + 15) & ~(size_t)15;
+  return (exchange_bytes(cols) + 4 * pad * sizeof(float) + cols * (2 * sizeof(double) + 2) + 15) & ~(size_t)15;
 }
 // A kept row: an odd number of 16-byte units, so that lanes on neighbouring rows meet different banks.
 __host__ __device__ inline int row_bytes(int cols, int size) { return (((cols * size + 15) >> 4) | 1) << 4; }
@@ -193,6 +193,7 @@ struct FarRows {
   long long ld;
   int pitch, kept_rows, n, cols;
   const float *us, *ul, *peaks, *masses, *b;
+  const unsigned char* out;
   float *f, *red;
   double per_eps, eps_per, log_cols, shift;
   float c, c_low;
@@ -206,11 +207,11 @@ __device__ __noinline__ void far_pass(const FarRows<T>& p, int mode, bool last) 
   constexpr int V = Vec<T>::kN, G = 32 / L;
   const int lane = threadIdx.x & 31, q = lane & (L - 1), group = lane / L;
   auto column = [&](int k) { return (k / V) * (L * V) + q * V + k % V; };
-  unsigned closed = 0;                                      // columns of mass 0
-  if (mode != 0 && p.b) {
+  unsigned closed = 0;                                      // columns that the row sums leave out
+  if (mode != 0) {
 #pragma unroll
     for (int k = 0; k < C; ++k)
-      if (column(k) < p.cols && p.b[column(k)] == 0.f) closed |= 1u << k;
+      if (column(k) < p.cols && p.out[column(k)]) closed |= 1u << k;
   }
   auto counts = [&](int k) { return !(closed >> k & 1); };               // in the row's sum
   float acc[C];
@@ -323,6 +324,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
   double* per_b = reinterpret_cast<double*>(ul + L * 32);      // 1 / b, with the rows' and columns' counts in it
   double* lb = per_b + p.cols;
   unsigned char* open = reinterpret_cast<unsigned char*>(lb + p.cols);
+  unsigned char* out = open + p.cols;                               // whether the rows' sums leave a column out
   T* kept = reinterpret_cast<T*>(smem + fixed_bytes(p.cols));       // (kept_rows, pitch)
   // whether a wait was in time; whether float32 is too coarse for a column that takes part; the least potential
   __shared__ int flag, far_columns, least;
@@ -340,13 +342,16 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
   // Columns of mass 0 add nothing to the rows' sums, so their potentials matter to nobody else: they are found in the last
   // iteration, from its f, like the first iteration's from any g (every column's maximum before its sum: nothing keeps such
   // a column's terms below the rows' maxima).
-  bool some_closed = false;
+  // (A column that starts from -inf is one of these in the first iteration.)
+  bool some_closed = false, some_out = false;               // of mass 0; left out in the first iteration
   for (int j = tid; j < cols; j += NT) {
     const float b = p.b ? p.b[j] : 1.f;                     // (1 / cols each: log2 cols in a row's sum instead)
     some_closed = some_closed || b == 0.f;
     lb[j] = b == 0.f || b == 1.f ? 0.0 : log2((double)b);
     per_b[j] = b == 0.f ? wk.k_scale : wk.k_scale / (double)b;
-    open[j] = b != 0.f;
+    out[j] = b == 0.f || (p.g0 && p.g0[j] == -INFINITY);
+    open[j] = !out[j];
+    some_out = some_out || out[j];
   }
   for (int j = tid; j < L * 32; j += NT) {
     if (j >= cols) us[j] = -INFINITY;
@@ -356,10 +361,11 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
     flag = 1;
     far_columns = 0;
     least = order_of(INFINITY);
-    rows_s = {scores - q * V, kept, p.ld, pitch, kept_rows, n, cols, us, ul, peaks_s, masses, p.b, p.f + r0, red, per_eps,
+    rows_s = {scores - q * V, kept, p.ld, pitch, kept_rows, n, cols, us, ul, peaks_s, masses, p.b, out, p.f + r0, red, per_eps,
               p.eps * 0.6931471805599453, wk.log_cols, 0.0, c, (float)(per_eps - (double)c), vectors};
   }
   some_closed = __syncthreads_or(some_closed);
+  some_out = __syncthreads_or(some_out);
   // What float32 potentials are relative to: 0, or the least one that takes part, by a given g, then by the potentials after
   // one iteration. So a column that a large finite score masks (its potential lies far above) does not cost the others their
   // accuracy.
@@ -387,11 +393,11 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
     else us[j] = ul[j] = 0.f;
   }
   __syncthreads();
-  auto closed_columns = [&]() {                             // the lane's columns of mass 0
+  auto closed_columns = [&]() {                             // the lane's columns that the rows' sums leave out
     unsigned closed = 0;
 #pragma unroll
     for (int k = 0; k < C; ++k)
-      if (column(k) < cols && p.b && p.b[column(k)] == 0.f) closed |= 1u << k;
+      if (column(k) < cols && out[column(k)]) closed |= 1u << k;
     return closed;
   };
 
@@ -412,7 +418,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
       bool empties = false;                                   // whether the thread has met rows with a maximum of -inf
       float farthest = 0.f;                                   // the largest |maximum| of its other rows
       // Modes: 0 column sums, without the columns of mass 0 (u = -inf); or, where the columns' maxima are found, 1 these and
-      // then 2 the sums relative to them, of all columns (u = 0 for those of mass 0, which the rows' sums leave out).
+      // then 2 the sums relative to them, of all columns (u = 0 for those that the rows' sums leave out).
       auto pass = [&](auto mode_, auto closed_) {
         constexpr int kMode = decltype(mode_)::value;
         constexpr bool kClosed = decltype(closed_)::value;
@@ -524,14 +530,14 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
       if (maxima) {
         if (!first) {
           for (int j = tid; j < cols; j += NT)
-            if (p.b[j] == 0.f) us[j] = 0.f;
+            if (out[j]) us[j] = 0.f;
           __syncthreads();
         }
         if constexpr (kExact) {
           far_pass<T, L, C>(rows_s, 1, false);
           __syncthreads();
         } else {
-          if (some_closed) pass(std::integral_constant<int, 1>{}, std::true_type{});
+          if (some_out) pass(std::integral_constant<int, 1>{}, std::true_type{});
           else pass(std::integral_constant<int, 1>{}, std::false_type{});
           fold(Larger{});
           bool out_of_range = false;                        // (the vote and what follows it: by the whole warp)
@@ -552,7 +558,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
           far_pass<T, L, C>(rows_s, 2, last);
         } else {
           if (__syncthreads_or(far)) return true;
-          if (some_closed) pass(std::integral_constant<int, 2>{}, std::true_type{});
+          if (some_out) pass(std::integral_constant<int, 2>{}, std::true_type{});
           else pass(std::integral_constant<int, 2>{}, std::false_type{});
           fold(Plus{});
         }
@@ -724,7 +730,8 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
         for (int i = 0; i < 2; ++i) {
           const int j = tid + i * NT;
           if (j >= cols) break;
-          if (p.b && p.b[j] == 0.f) {
+          out[j] = p.b && p.b[j] == 0.f;
+          if (out[j]) {
             us[j] = -INFINITY;
             ul[j] = 0.f;
           } else {

@@ -207,7 +207,7 @@ def balance(scores: torch.Tensor, *, eps: float = 0.05, iters: int = 20, a: torc
     scores   float32, float16 or bfloat16, at most 1024 columns
     a, b     row and column masses, float32, >= 0 (None: 1 / rows, 1 / columns). Padding rows have mass 0: they move no
              column, and still get their f. Masses are used as given (their sums should agree)
-    g        a starting potential, for instance the last step's
+    g        a starting potential, for instance the last step's; -inf leaves a column out of the first f
     A row or column whose terms are all zero (scores -inf, masses 0) has potential 0; a score more than 2.3e38 eps below
     its row's largest is as good as -inf. Rows and columns masked by large finite scores do not cost the others accuracy
     (but time: beyond about 700 eps from the others, terms are formed from pairs of float32). The potentials are constants
