@@ -10,8 +10,8 @@
 // few rows; each thread works on 64 bytes of scores at a time, which it brings through shared memory itself (asynchronous
 // copies, one or two more chunks in flight, no barrier), and keeps its own state: the largest score m, and with M = m c
 // rounded (c = log2 e / T, or 1 / T in float64) the sums s = sum exp(x c - M) and t = sum exp(x c - M) (x c - M), both
-// rescaled when m rises. M is a shift like any other, so its rounding cancels. Rows whose M would not be an ordinary
-// number (scores near the type's lowest value throughout) are summed again by the differences x - m.
+// rescaled when m rises. M is a shift like any other, so its rounding cancels. Rows whose M is so large that it rounds by
+// more than 1 (|m| / T beyond 1e7, 9e15 in float64) are summed again by the differences x - m.
 // The best columns come out of the same pass: a bound below the K-th largest score is kept from the threads' running
 // maxima (the K / warps-th largest of each warp's 32: at least K scores reach the smallest of these), raised after 1, 2,
 // 4, 8, ... chunks, and each warp lists the few 16-byte vectors whose largest score reaches it. The K best scores lie in
@@ -39,7 +39,6 @@ constexpr unsigned kAll = 0xffffffffu;
 constexpr int LP_VECS = 4;          // 16-byte vectors a thread holds of a chunk
 constexpr int LP_TOP = 64;          // most best columns
 constexpr int LP_LIST = 96;         // vectors with candidates for them that a warp lists (more than LP_TOP)
-constexpr float kWide = 1e30f;      // shifts M beyond this are not used
 
 // exp and log in the units of the sums: base 2 for float32, base e for float64. unit() turns such a logarithm into nats.
 struct Base2 {
@@ -48,6 +47,7 @@ struct Base2 {
   static __device__ __forceinline__ float unit() { return 0.6931471805599453f; }
   static __device__ __forceinline__ float per_unit() { return 1.4426950408889634f; }
   static float scale(double t) { return (float)(1.4426950408889634 / t); }
+  static __device__ __forceinline__ float wide() { return 0x1p24f; }       // shifts M beyond this are off by more than 1
 };
 struct BaseE {
   static __device__ __forceinline__ double exp(double x) { return ::exp(x); }
@@ -55,6 +55,7 @@ struct BaseE {
   static __device__ __forceinline__ double unit() { return 1.0; }
   static __device__ __forceinline__ double per_unit() { return 1.0; }
   static double scale(double t) { return 1.0 / t; }
+  static __device__ __forceinline__ double wide() { return 0x1p53; }
 };
 template <typename T> struct Base { using type = Base2; };
 template <> struct Base<double> { using type = BaseE; };
@@ -493,8 +494,9 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW)
 
   const bool empty = a.m == -inf, bad = !(a.m < inf);
   A past = fma(a.m, c, -shift(a.m, c));                       // m c - M: s is relative to M, log_s below to m c
-  if (!empty && !bad && !(fabs(shift(a.m, c)) <= (A)kWide)) {
-    // M is not an ordinary number: s and t once more, by the differences x - m
+  if (!empty && !bad && !(fabs(shift(a.m, c)) <= B::wide())) {
+    // M rounds m c by up to half its spacing, which may carry the terms out of range: s and t once more, by the differences
+    // x - m
     past = 0;
     A s = 0, t = 0;
     for (long long j = tid; j < p.cols; j += NT) {
