@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from trnopt import scores
-from test_gpu_scores import GAMMA, INF, TYPES, U, close, gen, make
+from test_gpu_scores import GAMMA, INF, TYPES, U, check_log_probs, close, gen, make
 
 pytestmark = pytest.mark.gpu
 
@@ -171,3 +171,21 @@ def test_balance_start_that_is_no_number():
         g[3] = bad
         r = scores.balance(s, eps=0.2, iters=2, g=g)
         assert torch.isnan(r.f).all() and torch.isnan(r.g).all()
+
+
+# log_probs -----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cols", [40, 3001, 70000])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("offset,temperature", [(-3e9, 1.0), (-1e10, 1.0), (7e11, 1.0), (0.0, 1e-10), (-1e20, 1.7), (1e28, 0.3)])
+def test_log_probs_far_scores(cols, dtype, offset, temperature):
+    """Scores whose multiple by log2(e) / T rounds by more than the exponential's range, on rows of equal scores, too."""
+    if dtype == "f16" and offset:
+        offset, temperature = math.copysign(30000.0, offset), temperature * 3e4 / abs(offset)
+    s = make(5, cols, torch.float32, seed=cols).double()
+    s[1:] += offset
+    s[2] = offset * 1.0001
+    s[3, ::2] = -INF
+    s[4] = torch.where(torch.arange(cols, device="cuda") % 3 == 0, offset + abs(offset) * 2.0 ** -7, offset)
+    t = torch.randint(cols, (5, 2), generator=gen(1), device="cuda")
+    check_log_probs(s.to(TYPES[dtype]), t, 5, temperature)
