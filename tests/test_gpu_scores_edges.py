@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from trnopt import scores
-from test_gpu_scores import GAMMA, INF, TYPES, U, check_log_probs, close, gen, make
+from test_gpu_scores import GAMMA, INF, TYPES, U, check_gradient, check_log_probs, close, gen, lp_reference, make
 
 pytestmark = pytest.mark.gpu
 
@@ -189,3 +189,46 @@ def test_log_probs_far_scores(cols, dtype, offset, temperature):
     s[4] = torch.where(torch.arange(cols, device="cuda") % 3 == 0, offset + abs(offset) * 2.0 ** -7, offset)
     t = torch.randint(cols, (5, 2), generator=gen(1), device="cuda")
     check_log_probs(s.to(TYPES[dtype]), t, 5, temperature)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("temperature", [1e-10, 1e-25])
+def test_log_probs_gradient_of_masked_rows_at_small_temperatures(dtype, temperature):
+    s = make(6, 1003, torch.float32, seed=4, scale=2.0 * temperature)
+    s[1:, ::3] = -INF
+    s[2] = -INF
+    s[3, 5:] = torch.finfo(torch.float32).min
+    check_gradient(s.to(TYPES[dtype]), torch.randint(1003, (6, 2), generator=gen(7), device="cuda"), 3, temperature)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_log_probs_gradient_of_masked_rows_with_large_upstream_values(dtype):
+    """A scaled loss: 2^24 on the entropy at T = 0.02. The gradient is p (log p + H) g / T in 64 bits, p off by
+    (8 |log p| + the chain + 2 GAMMA) u and log p + H by 8 u of its terms."""
+    s = make(4, 2003, TYPES[dtype], seed=4, scale=0.05)
+    s[1:, ::3] = -INF
+    s[2, 4:] = -INF
+    leaf = s.detach().requires_grad_()
+    r = scores.log_probs(leaf, temperature=0.02)
+    up = torch.full_like(r.entropy, 2.0 ** (3 if dtype == "f16" else 24))
+    grad, = torch.autograd.grad(r.entropy, leaf, up)
+    w = lp_reference(s, torch.zeros(4, 1, dtype=torch.int64, device="cuda"), 1, 0.02)
+    log_p = torch.where(w["p"] > 0, w["log_p"], 0.0)
+    each = w["p"] * up.double()[:, None] / 0.02
+    want = -each * (log_p + w["h"][:, None])
+    u = 2.0 ** -53 if dtype == "f64" else U
+    size = log_p.abs() + w["h"][:, None] + 1
+    tol = each * size * u * (8 * log_p.abs() + 2003 / 256 + 8 + 2 * GAMMA + 8 * size)
+    tol = (tol + torch.finfo(s.dtype).eps / 2 * want.abs()) * (1 + torch.finfo(s.dtype).eps)
+    close(grad, want, tol + torch.finfo(s.dtype).smallest_normal, "grad")
+    assert (grad[s == -INF] == 0).all()
+
+
+def test_log_probs_gradient_of_a_row_that_is_no_number():
+    s = make(3, 300, torch.float32)
+    s[1, 7] = math.nan
+    s[2, 9] = INF
+    leaf = s.requires_grad_()
+    r = scores.log_probs(leaf, torch.zeros(3, dtype=torch.int64, device="cuda"))
+    grad, = torch.autograd.grad((r.log_prob.sum() + r.entropy.sum()), leaf)
+    assert torch.isfinite(grad[0]).all() and torch.isnan(grad[1:]).all()

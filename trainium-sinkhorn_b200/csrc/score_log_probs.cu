@@ -64,6 +64,10 @@ template <> struct Base<double> { using type = BaseE; };
 __device__ __forceinline__ float floored(float d) { return fmaxf(d, -1e30f); }
 __device__ __forceinline__ double floored(double d) { return fmax(d, -1e30); }
 
+// A logarithm of p: from below where exp() is 0, so that its products with other numbers stay finite.
+__device__ __forceinline__ float log_floored(float d) { return fmaxf(d, -200.f); }
+__device__ __forceinline__ double log_floored(double d) { return fmax(d, -1000.0); }
+
 // M: the rounded product itself, never contracted into what uses it.
 __device__ __forceinline__ float shift(float m, float c) { return __fmul_rn(m, c); }
 __device__ __forceinline__ double shift(double m, double c) { return __dmul_rn(m, c); }
@@ -541,11 +545,11 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW)
 }
 
 // Gradient: a CTA of one warp takes `chunks` x 32 x LP_VECS vectors of one row, placed on the gradient's 16-byte
-// boundaries, the next chunk on its way while one is worked on. With the row's m and log s a score needs no sum: p (A + B log p), with
-// A = -(g + g_H H) / T, B = -g_H / T and g the sum of the upstream gradients of the row's given and best columns (less
-// that of lse). Those columns are written once more, by the first entry that names them, with the entries that repeat it
-// added in order. Bound by the two matrices' bytes: 8192 x 32768 bfloat16 (2 x 0.54 GB) 171 us, 164 us at the copy
-// rate. (CTAs of 256 threads: 174 us, but 8192 x 1000 70 us against 12 us.)
+// boundaries, the next chunk on its way while one is worked on. With the row's m and log s a score needs no sum:
+// p (A + B log p) / T, with A = -(g + g_H H), B = -g_H and g the sum of the upstream gradients of the row's given and best
+// columns (less that of lse). Those columns are written once more, by the first entry that names them, with the entries that
+// repeat it added in order. Bound by the two matrices' bytes: 8192 x 32768 bfloat16 (2 x 0.54 GB) 171 us, 164 us at the
+// copy rate. (CTAs of 256 threads: 174 us, but 8192 x 1000 70 us against 12 us.)
 template <typename T>
 __global__ void __launch_bounds__(32, 32) log_probs_grad_kernel(LogProbsGradProblem p, int parts, int chunks,
                                                                typename Acc<T>::type c, typename Acc<T>::type inv_t) {
@@ -605,10 +609,10 @@ __global__ void __launch_bounds__(32, 32) log_probs_grad_kernel(LogProbsGradProb
   total = warp_sum(total);
   if (p.d_lse) total -= static_cast<const A*>(p.d_lse)[row];
   const bool empty = m == -inf;
-  const A ls = log_s * B::per_unit(), fa = -inv_t * (total + gh * h), fb = -inv_t * gh * B::unit();
+  const A ls = log_s * B::per_unit(), fa = -(total + gh * h), fb = -gh * B::unit();
   auto dense = [&](A x) {
-    const A lp = floored(fma(x - m, c, -ls));
-    return B::exp(lp) * fma(fb, lp, fa);
+    const A lp = log_floored(fma(x - m, c, -ls));
+    return B::exp(lp) * fma(fb, lp, fa);                   // (times 1 / T last: a p of 0 stays 0 whatever T)
   };
   for (long long v = v0; v < v1; v += kChunk) {
     Vec<T> next[LP_VECS];
@@ -620,13 +624,13 @@ __global__ void __launch_bounds__(32, 32) log_probs_grad_kernel(LogProbsGradProb
         if constexpr (sizeof(A) == 4) {
           float a, b;
           unpack2(fma2(add2(pack2(q[i].get(e), q[i].get(e + 1)), pack2(-m, -m)), pack2(c, c), pack2(-ls, -ls)), a, b);
-          a = floored(a);
-          b = floored(b);
+          a = log_floored(a);
+          b = log_floored(b);
           const uint64_t f = fma2(pack2(a, b), pack2(fb, fb), pack2(fa, fa));
-          unpack2(mul2(pack2(B::exp(a), B::exp(b)), f), a, b);
+          unpack2(mul2(mul2(pack2(B::exp(a), B::exp(b)), f), pack2(inv_t, inv_t)), a, b);
           q[i].set_pair(e, a, b);
         } else {
-          q[i].set_pair(e, dense(q[i].get(e)), dense(q[i].get(e + 1)));
+          q[i].set_pair(e, dense(q[i].get(e)) * inv_t, dense(q[i].get(e + 1)) * inv_t);
         }
       }
       if (empty) q[i].q = make_uint4(0, 0, 0, 0);
@@ -663,7 +667,7 @@ __global__ void __launch_bounds__(32, 32) log_probs_grad_kernel(LogProbsGradProb
     A g = upstream(k);
     for (int r = k + 1; r < extra; ++r)
       if (column(r) == j) g += upstream(r);
-    narrow(fma(g, inv_t, dense(widen(s[j]))), out + j);
+    narrow((g + dense(widen(s[j]))) * inv_t, out + j);
   }
 }
 
