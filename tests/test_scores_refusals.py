@@ -112,3 +112,22 @@ def test_cpu_tensors_are_refused():
 
 def test_route_load_counts_in_32_bits():
     assert route(rows=1 << 31, load=A) == INVALID
+
+
+def test_forward_mode_derivatives_are_refused():
+    """log_probs and route have no forward-mode derivative: a dual tensor would come back without its tangent."""
+    s = torch.zeros(3, 4)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(s, torch.ones_like(s))
+        for call in (lambda: scores.log_probs(dual), lambda: scores.route(dual, 1)):
+            with pytest.raises(ValueError, match="forward"):
+                call()
+        with pytest.raises(ValueError, match="CUDA tensor"):          # a tensor without a tangent is as elsewhere
+            scores.log_probs(s)
+
+
+def test_tracing_is_refused():
+    """torch.jit.trace records the outputs' allocation and not the call that fills them."""
+    for fn in (lambda s: scores.log_probs(s).lse, lambda s: scores.balance(s).g, lambda s: scores.route(s, 1).weight):
+        with pytest.raises(ValueError, match="trace"):
+            torch.jit.trace(fn, torch.zeros(3, 4), check_trace=False)

@@ -15,9 +15,10 @@ log_probs(S) tells how decided the rows are. trnopt.plan.descendants applies log
 
 Scores are CUDA tensors of any leading shape and row pitch (a last dimension that is not contiguous is copied first).
 The calls queue on the scores' device, on that device's current stream, return without waiting, and can be captured into
-a CUDA graph (backward() as torch asks for it: on a side stream, with no eager graph of the same leaves alive). There is
-no CPU path. What a call rejects it rejects before anything is queued, with ValueError; values on the device (an index
-out of range, NaN) never raise and show in the results as described.
+a CUDA graph (backward() as torch asks for it: on a side stream, with no eager graph of the same leaves alive), but not
+traced (torch.jit.trace is refused, as are forward-mode tangents: derivatives are backward's). There is no CPU path. What a
+call rejects it rejects before anything is queued, with ValueError; values on the device (an index out of range, NaN)
+never raise and show in the results as described.
 """
 
 from __future__ import annotations
@@ -26,6 +27,7 @@ from functools import lru_cache
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi
 
@@ -58,8 +60,13 @@ class Routing(NamedTuple):
     load: torch.Tensor | None           # (columns,) int32: rows that chose each column
 
 
-def _matrix(scores: torch.Tensor, double: bool) -> torch.Tensor:
+def _matrix(scores: torch.Tensor, double: bool, differentiable: bool = True) -> torch.Tensor:
     """The scores as a 2-d view with unit column stride (a copy only where there is no such view)."""
+    if torch.jit.is_tracing():
+        raise ValueError("the score kernels cannot be traced (torch.jit.trace would record empty outputs)")
+    if differentiable and forward_ad._current_level >= 0 and isinstance(scores, torch.Tensor) and \
+            forward_ad.unpack_dual(scores).tangent is not None:
+        raise ValueError("the score kernels have no forward-mode derivatives")
     if not isinstance(scores, torch.Tensor) or not scores.is_cuda:
         raise ValueError("scores must be a CUDA tensor (the score kernels have no CPU path)")
     if scores.dtype not in _TYPE or (scores.dtype == torch.float64 and not double):
@@ -212,7 +219,7 @@ def balance(scores: torch.Tensor, *, eps: float = 0.05, iters: int = 20, a: torc
     its row's largest is as good as -inf. Rows and columns masked by large finite scores do not cost the others accuracy
     (but time: beyond about 700 eps from the others, terms are formed from pairs of float32). The potentials are constants
     to autograd."""
-    s = _matrix(scores, False)
+    s = _matrix(scores, False, False)
     rows, cols = s.shape
     if cols > MAX_COLUMNS:
         raise ValueError(f"at most {MAX_COLUMNS} columns")
