@@ -311,7 +311,8 @@ int trnopt_log_probs(int type, const void* scores, long long ld, long long rows,
 /* The gradient of trnopt_log_probs: grad (rows, cols; pitch ld_grad >= cols; the scores' type) from the upstream
  * gradients of its outputs (each NULL where there is none) and the forward call's row_max, log_sum, entropy and
  * top_index. Columns named more than once add up; padding and out-of-range targets add nothing; rows of nothing but
- * -inf have gradient 0. Deterministic. n_targets + top <= 1088. */
+ * -inf have gradient 0. Deterministic. n_targets + top <= 1088. grad must not share elements with scores (refused where
+ * their ranges overlap, unless both have one pitch and the rows of one lie between the other's). */
 int trnopt_log_probs_grad(int type, const void* scores, long long ld, long long rows, int cols, double temperature,
                           const long long* targets, int n_targets, const long long* top_index, int top,
                           const void* row_max, const void* log_sum, const void* entropy, const void* d_log_prob,
@@ -351,8 +352,8 @@ int trnopt_route(int type, const void* scores, long long ld, long long rows, int
                  float scale, long long* index, float* weight, int* load, void* stream);
 
 /* The gradient of trnopt_route's weights with respect to the scores (the choice itself is constant): grad (rows, cols;
- * pitch ld_grad >= cols; the scores' type). Slots of index outside [0, cols) add nothing; a row that chose nothing has
- * gradient 0. */
+ * pitch ld_grad >= cols; the scores' type; no elements in common with scores, as for trnopt_log_probs_grad). Slots of index
+ * outside [0, cols) add nothing; a row that chose nothing has gradient 0. */
 int trnopt_route_grad(int type, const void* scores, long long ld, long long rows, int cols, int top, int kind,
                       int renormalize, float scale, const long long* index, const float* d_weight, void* grad,
                       long long ld_grad, void* stream);

@@ -177,7 +177,8 @@ def test_balance_start_that_is_no_number():
 
 @pytest.mark.parametrize("cols", [40, 3001, 70000])
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("offset,temperature", [(-3e9, 1.0), (-1e10, 1.0), (7e11, 1.0), (0.0, 1e-10), (-1e20, 1.7), (1e28, 0.3)])
+@pytest.mark.parametrize("offset,temperature", [(-3e9, 1.0), (-1e10, 1.0), (7e11, 1.0), (0.0, 1e-10), (-1e20, 1.7),
+                                                (1e28, 0.3)])
 def test_log_probs_far_scores(cols, dtype, offset, temperature):
     """Scores whose multiple by log2(e) / T rounds by more than the exponential's range, on rows of equal scores, too."""
     if dtype == "f16" and offset:
@@ -232,3 +233,31 @@ def test_log_probs_gradient_of_a_row_that_is_no_number():
     r = scores.log_probs(leaf, torch.zeros(3, dtype=torch.int64, device="cuda"))
     grad, = torch.autograd.grad((r.log_prob.sum() + r.entropy.sum()), leaf)
     assert torch.isfinite(grad[0]).all() and torch.isnan(grad[1:]).all()
+
+
+def test_gradient_rows_between_the_scores_rows():
+    """Scores and gradient as the halves of one buffer's rows, through the C calls."""
+    from trnopt import _capi
+    rows, cols = 37, 200
+    buf = torch.zeros(rows, 2 * cols + 8, device="cuda")
+    s, grad = buf[:, :cols], buf[:, cols + 4:2 * cols + 4]
+    s.copy_(make(rows, cols, torch.float32, seed=3))
+    buf[:, 2 * cols + 4:] = 7.0
+    leaf = s.clone().requires_grad_()
+    t = torch.randint(cols, (rows,), generator=gen(1), device="cuda")
+    up = torch.randn(rows, generator=gen(2), device="cuda")
+    want, = torch.autograd.grad(scores.log_probs(leaf, t).log_prob, leaf, up)
+    numbers = [torch.empty(rows, device="cuda") for _ in range(5)]
+    at, pitch, stream = [n.data_ptr() for n in numbers], buf.stride(0), torch.cuda.current_stream().cuda_stream
+    _capi.check(_capi.lib.trnopt_log_probs(0, s.data_ptr(), pitch, rows, cols, 1.0, t.data_ptr(), 1, 0, at[0], at[1], at[2],
+                                           None, None, at[3], at[4], stream), "log_probs")
+    _capi.check(_capi.lib.trnopt_log_probs_grad(0, s.data_ptr(), pitch, rows, cols, 1.0, t.data_ptr(), 1, None, 0, at[3], at[4],
+                                                at[1], up.data_ptr(), None, None, None, grad.data_ptr(), pitch, stream),
+                "log_probs_grad")
+    assert torch.equal(grad, want) and torch.equal(s, leaf) and (buf[:, cols:cols + 4] == 0).all()
+    r = scores.route(leaf, 3)
+    d = torch.randn(rows, 3, generator=gen(4), device="cuda")
+    want, = torch.autograd.grad(r.weight, leaf, d)
+    _capi.check(_capi.lib.trnopt_route_grad(0, s.data_ptr(), pitch, rows, cols, 3, 0, 1, 1.0, r.index.data_ptr(), d.data_ptr(),
+                                            grad.data_ptr(), pitch, stream), "route_grad")
+    assert torch.equal(grad, want) and torch.equal(s, leaf) and (buf[:, 2 * cols + 4:] == 7).all()

@@ -131,3 +131,16 @@ def test_tracing_is_refused():
     for fn in (lambda s: scores.log_probs(s).lse, lambda s: scores.balance(s).g, lambda s: scores.route(s, 1).weight):
         with pytest.raises(ValueError, match="trace"):
             torch.jit.trace(fn, torch.zeros(3, 4), check_trace=False)
+
+
+@pytest.mark.parametrize("grad_call", [log_probs_grad, route_grad])
+def test_gradient_in_the_scores_place_is_refused(grad_call):
+    """Scores are read after parts of the gradient are written, so the two must not share elements."""
+    row = dict(rows=1, ld=0)
+    for offset in (0, 4, 28):                          # the same rows, and rows that begin inside the scores' rows
+        assert grad_call(cols=8, ld=8, ld_grad=8, grad=A + offset) == INVALID
+    assert grad_call(cols=8, ld=16, ld_grad=16, grad=A + 28) == INVALID
+    assert grad_call(cols=8, ld=16, ld_grad=16, grad=A + 36) == INVALID
+    assert grad_call(cols=8, ld=16, ld_grad=24, grad=A + 40) == INVALID       # other pitches: the whole ranges
+    assert grad_call(cols=8, ld_grad=8, grad=A + 28, **row) == INVALID
+    assert grad_call(cols=8, ld=8, ld_grad=8, grad=A - 4 * 8 * 4 + 4) == INVALID

@@ -447,12 +447,25 @@ int trnopt_plan_log_rows(const double* x, int n, const double* y, int m, int d, 
                                           reinterpret_cast<cudaStream_t>(stream)));
 }
 
+static size_t score_size(int type) { return type == TRNOPT_F64 ? 8 : type == TRNOPT_F32 ? 4 : 2; }
+
 // Shared checks of the score-matrix calls: a known type, sizes, and the alignment of the type.
 static int check_scores(int type, const void* scores, long long ld, long long rows, int cols, bool f64_ok) {
   if (type < TRNOPT_F32 || type > (f64_ok ? TRNOPT_F64 : TRNOPT_BF16)) return TRNOPT_ERR_UNSUPPORTED;
   if (rows < 0 || cols < 1 || ld < 0 || (rows > 0 && !scores)) return TRNOPT_ERR_INVALID_ARGUMENT;
-  const size_t size = type == TRNOPT_F64 ? 8 : type == TRNOPT_F32 ? 4 : 2;
-  return aligned(scores, size) ? TRNOPT_OK : TRNOPT_ERR_ALIGNMENT;
+  return aligned(scores, score_size(type)) ? TRNOPT_OK : TRNOPT_ERR_ALIGNMENT;
+}
+
+// Whether scores and their gradient, rows x cols elements each, may share an element: never where their ranges are apart or,
+// for equal pitches, where the gradient's rows lie in the scores' gaps.
+static bool may_overlap(const void* scores, long long ld, const void* grad, long long ld_grad, long long rows, int cols,
+                        size_t size) {
+  const __int128 s = reinterpret_cast<uintptr_t>(scores), g = reinterpret_cast<uintptr_t>(grad);
+  const auto bytes = [&](long long pitch) { return ((__int128)(rows - 1) * pitch + cols) * (__int128)size; };
+  if (s + bytes(ld) <= g || g + bytes(ld_grad) <= s) return false;
+  if (rows == 1 || ld != ld_grad) return true;
+  const long long by = (long long)((g - s) / (long long)size % ld), place = by < 0 ? by + ld : by;
+  return place < cols || place > ld - cols;
 }
 
 static bool temperature_ok(double t) { return t >= 1e-30 && t <= 1e30; }
@@ -495,6 +508,7 @@ int trnopt_log_probs_grad(int type, const void* scores, long long ld, long long 
       !aligned(entropy, size) || !aligned(d_log_prob, size) || !aligned(d_entropy, size) || !aligned(d_lse, size) ||
       !aligned(d_top_log_prob, size))
     return TRNOPT_ERR_ALIGNMENT;
+  if (may_overlap(scores, ld, grad, ld_grad, rows, cols, score_size(type))) return TRNOPT_ERR_INVALID_ARGUMENT;
   const LogProbsGradProblem p{scores, ld, rows, cols, temperature, targets, n_targets, top_index, top, row_max,
                               log_sum, entropy, d_log_prob, d_entropy, d_lse, d_top_log_prob, grad, ld_grad};
   return cuda_status(log_probs_grad_launch(type, p, reinterpret_cast<cudaStream_t>(stream)));
@@ -550,6 +564,7 @@ int trnopt_route_grad(int type, const void* scores, long long ld, long long rows
       (kind != TRNOPT_ROUTE_SOFTMAX && kind != TRNOPT_ROUTE_SIGMOID) || (rows > 0 && (!index || !d_weight)))
     return TRNOPT_ERR_INVALID_ARGUMENT;
   if (!aligned(index, 8) || !aligned(d_weight, 4)) return TRNOPT_ERR_ALIGNMENT;
+  if (rows > 0 && may_overlap(scores, ld, grad, ld_grad, rows, cols, score_size(type))) return TRNOPT_ERR_INVALID_ARGUMENT;
   const RouteGradProblem p{scores, ld, rows, cols, top, kind, renormalize, scale, index, d_weight, grad, ld_grad};
   return cuda_status(route_grad_launch(type, p, reinterpret_cast<cudaStream_t>(stream)));
 }
