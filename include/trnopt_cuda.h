@@ -323,8 +323,8 @@ int trnopt_log_probs_grad(int type, const void* scores, long long ld, long long 
  *     f_i = -eps LSE_j(log b_j + (g_j + S_ij) / eps),   g_j = -eps LSE_i(log a_i + (f_i + S_ij) / eps)
  * (the half-steps of sinkhorn.py:108-119 for the cost -S), from g = g0 (NULL: 0). a (rows,) and b (cols,) are masses
  * >= 0 (NULL: 1 / rows, 1 / cols); rows or columns of mass 0 send nothing and still get their potential. A row or
- * column whose terms are all zero has potential 0; a score more than 2.3e38 eps below its row's largest is as good as
- * -inf. f (rows,) and g (cols,) are float32. 1 <= iters <= 2^24, cols <= 1024;
+ * column whose terms are all zero has potential 0; a score more than 2.3e38 eps below its row's largest (among columns
+ * with mass) is as good as -inf. f (rows,) and g (cols,) are float32. 1 <= iters <= 2^24, cols <= 1024;
  * types F32, F16, BF16. Deterministic. One cooperative launch, whose CTAs wait for one another (bounded: after the
  * limit f and g are NaN and the device error word has bit 1). Workspace of trnopt_balance_workspace_size bytes
  * (256-byte aligned, no initialisation); one workspace per call in flight. */

@@ -164,6 +164,19 @@ def test_balance_start_of_minus_infinity(rows, cols, iters, mass):
     check(s, 0.2, iters, None, b / b.sum(), g)
 
 
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("value", [-1e4, 2e4])
+def test_balance_start_of_minus_infinity_on_a_far_column(rows, cols, value):
+    """Its first terms are its own size, which the later row sums must not see."""
+    s = make(rows, cols, torch.float32, seed=rows, scale=1.0)
+    s[:, 3] += value
+    s[5, torch.arange(cols, device="cuda") != 3] = -INF
+    g = torch.zeros(cols, device="cuda")
+    g[3] = -INF
+    for iters in (1, 2, 6):
+        check(s, 0.15, iters, g=g, far=[3])
+
+
 def test_balance_start_that_is_no_number():
     s = make(700, 16, torch.float32, scale=1.0)
     for bad in (math.nan, INF):

@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(NT, 1) balance_kernel(BalanceProblem p, Balanc
           m = fabsf(m) < INFINITY ? m : 0.f;
           peaks_s[j] = m;
           off_s[j] = us[j] == -INFINITY ? 0.f : -us[j] - m;
-          far = far || (open[j] && fabsf(m) > kNear);
+          far = far || (!(p.b && p.b[j] == 0.f) && fabsf(m) > kNear);       // (also of one that starts from -inf)
         }
         if constexpr (kExact) {
           __syncthreads();

@@ -216,7 +216,7 @@ def balance(scores: torch.Tensor, *, eps: float = 0.05, iters: int = 20, a: torc
              column, and still get their f. Masses are used as given (their sums should agree)
     g        a starting potential, for instance the last step's; -inf leaves a column out of the first f
     A row or column whose terms are all zero (scores -inf, masses 0) has potential 0; a score more than 2.3e38 eps below
-    its row's largest is as good as -inf. Rows and columns masked by large finite scores do not cost the others accuracy
+    its row's largest (among columns with mass) is as good as -inf. Rows and columns masked by large finite scores do not cost the others accuracy
     (but time: beyond about 700 eps from the others, terms are formed from pairs of float32). The potentials are constants
     to autograd."""
     s = _matrix(scores, False, False)
