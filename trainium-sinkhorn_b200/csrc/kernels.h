@@ -7,26 +7,9 @@
 #include <atomic>
 
 #include "common.cuh"
+#include "smem_attr.h"
 
 namespace trnopt {
-
-constexpr int kMaxDevices = 64;
-
-// cudaFuncSetAttribute(MaxDynamicSharedMemorySize) acts on the calling thread's current device only. `done` holds,
-// per device, the largest size already set for `fn`, so a process that drives several GPUs sets it on each of them.
-inline cudaError_t smem_attr_once(const void* fn, int bytes, std::atomic<int>* done) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev >= 0 && dev < kMaxDevices && done[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
-  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev >= 0 && dev < kMaxDevices) {
-    int cur = done[dev].load(std::memory_order_relaxed);
-    while (cur < bytes && !done[dev].compare_exchange_weak(cur, bytes, std::memory_order_release)) {
-    }
-  }
-  return e;
-}
 
 // FFMA tile path (half_step_ffma.cu)
 size_t ffma_smem_bytes(int d);
