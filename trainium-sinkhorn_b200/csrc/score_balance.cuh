@@ -6,27 +6,29 @@
 // A row or column without mass to exchange (all its terms zero) takes potential 0.
 //
 // Both half-steps of an iteration come from one exponential per score. In base 2, with c = log2 e / eps and the column
-// potentials u_j = g_j c, a row's terms are e_j = 2^(S_ij c + u_j - m_i) and its sum l_i = sum_j b_j e_j, so
-// f_i c = -(m_i + log2 l_i); the column sums k_j = sum_i a_i e_ij / l_i then give the next potentials,
-// u_j <- u_j - log2 k_j. After an iteration every column's k_j would be 1, so the next one's lies between the smallest
-// a_i / (row sum) and the largest, far from underflow; only the first iteration, from any g, finds each column's maximum
-// before its sum. Potentials are pairs of float32, relative (after the first iteration) to the least of those that take part,
-// and terms are formed from their high parts: differences of a few units, where the potentials themselves may be hundreds.
-// Once a row's maximum or such a column's potential lies 2^10 or more from 0 (finite masks, offsets), a CTA forms all its
-// terms from the pairs, less their row's own constant: 65536 x 256 bfloat16 102 us an iteration in place of 11. A score more
-// than float32's range (2.3e38 eps) below its row's largest is as good as -inf.
+// potentials u_j = g_j c, a row's terms are e_j = 2^(S_ij c + u_j - m_i) and its sum l_i = sum_j b_j e_j, so f_i c =
+// -(m_i + log2 l_i); the column sums k_j = sum_i a_i e_ij / l_i then give the next potentials, u_j <- u_j - log2 k_j.
+// After an iteration every column's k_j would be 1, so the next one's lies between the smallest a_i / (row sum) and the
+// largest, far from underflow; only the first iteration, from any g, finds each column's maximum before its sum (and
+// the last one, where columns of mass 0 need theirs). Potentials are pairs of float32, relative (after the first
+// iteration) to the least of those that take part, and terms are formed from their high parts: differences of a few
+// units, where the potentials themselves may be hundreds. Once a row's maximum or such a column's potential lies 2^10
+// or more from 0 (finite masks, offsets), a CTA forms all its terms from the pairs, less their row's own constant:
+// 65536 x 256 bfloat16 94 us an iteration in place of 11. A score more than float32's range (2.3e38 eps) below its
+// row's largest is as good as -inf.
 //
 // One cooperative launch runs all iterations. A CTA owns a block of rows and keeps as many of them as fit in shared
-// memory as they were read in the first pass (the rest come from L2 in every pass). L neighbouring lanes share a row, up
-// to 32 columns each, so a row's maximum and sum take log2 L shuffles for the warp's 32 / L rows together, and a lane
-// sums its columns over its rows in registers. Per iteration the CTAs add their column sums up in fixed point, one atomic
-// addition of a 64-bit word per column and CTA: whole numbers, so their order does not matter, and the word counts the
-// CTAs, so there is no other barrier. (Every CTA's sums in float32, behind a barrier and added in the same order by all,
-// took 3 to 5 us of an iteration; they are left for the first one and for sums outside the fixed point's range.) What one
-// CTA takes in two steps of its warps stays in one. Bound by the pass's instructions for many rows, by the exchange's
-// latency for few. Measured per iteration: 65536 x 256 bfloat16 10.7 us (7 us the pass, of which 3.7 us are exponentials
-// at 16 per clock and SM, the rest the exchange), 65536 x 16 2.6 us, 8192 x 64 3.3 us, 509 x 24 in one CTA 2.2 us; a call
-// of one iteration, which passes twice and reads the scores from DRAM, 39 us for 65536 x 256.
+// memory as they were read in the first pass (the rest come from L2 in every pass). L neighbouring lanes share a row,
+// up to 32 columns each, so a row's maximum and sum take log2 L shuffles for the warp's 32 / L rows together, and a
+// lane sums its columns over its rows in registers. Per iteration the CTAs add their column sums up in fixed point, one
+// atomic addition of a 64-bit word per column and CTA: whole numbers, so their order does not matter, and the word
+// counts the CTAs, so there is no other barrier. (Every CTA's sums in float32, behind a barrier and added in the same
+// order by all, took 3 to 5 us of an iteration; they are left for iterations with maxima and for sums outside the fixed
+// point's range.) What one CTA takes in two steps of its warps stays in one. Bound by the pass's instructions for many
+// rows, by the exchange's latency for few. Measured per iteration: 65536 x 256 bfloat16 10.9 us (7 us the pass, of
+// which 3.7 us are exponentials at 16 per clock and SM, the rest the exchange), 65536 x 16 2.7 us, 8192 x 64 3.4 us,
+// 509 x 24 in one CTA 2.5 us; a call of one iteration, which passes twice and reads the scores from DRAM, 38 us for
+// 65536 x 256.
 #pragma once
 
 #include <math.h>

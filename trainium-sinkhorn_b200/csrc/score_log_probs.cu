@@ -549,7 +549,8 @@ __global__ void __launch_bounds__(32 * NW, (sizeof(T) == 8 ? 16 : 32) / NW)
 // p (A + B log p) / T, with A = -(g + g_H H), B = -g_H and g the sum of the upstream gradients of the row's given and best
 // columns (less that of lse). Those columns are written once more, by the first entry that names them, with the entries that
 // repeat it added in order. Bound by the two matrices' bytes: 8192 x 32768 bfloat16 (2 x 0.54 GB) 171 us, 164 us at the
-// copy rate. (CTAs of 256 threads: 174 us, but 8192 x 1000 70 us against 12 us.)
+// copy rate. (CTAs of 256 threads: 174 us, but 8192 x 1000 70 us against 12 us.) Named columns cost next to nothing up to
+// some dozens, but grow with their square: 4096 x 1000 with 128 / 512 / 1024 targets a row 90 / 1,090 / 4,190 us.
 template <typename T>
 __global__ void __launch_bounds__(32, 32) log_probs_grad_kernel(LogProbsGradProblem p, int parts, int chunks,
                                                                typename Acc<T>::type c, typename Acc<T>::type inv_t) {
@@ -729,8 +730,9 @@ cudaError_t launch(const LogProbsProblem& p, cudaStream_t stream) {
   // The fewest warps per row that fill half of the SMs' 32 warp slots, and no more than the row has chunks for: what a
   // row costs besides its scores (ranking, joining sums) grows with its warps. Measured at 8 / 4 / 2 / 1 warps, bfloat16,
   // 5 best columns: 8192 x 32768 166 / 129 / 109 / 104 us, 8192 x 1000 115 / 59 / 33 / 18 us, 600 x 5000
-  // 15 / 12 / 10 / 12 us, 300 x 131072 29 / 35 / 47 / 68 us. A warp vouches for 24 best columns at most (of its 32
-  // lanes' maxima the 32nd is a poor bound): 2048 x 32000 with 64 best columns 72 / 76 / 126 / 237 us.
+  // 15 / 12 / 10 / 12 us, 300 x 131072 29 / 35 / 47 / 68 us. (600 x 5000 takes 4 warps by this rule, 2 us more than with 2.)
+  // A warp vouches for 24 best columns at most (of its 32 lanes' maxima the 32nd is a poor bound): 2048 x 32000 with 64 best
+  // columns 72 / 76 / 126 / 237 us.
   const long long warp_cols = 32LL * LP_VECS * Vec<T>::kN;
   int nw = 1;
   while (nw < 8 && (p.rows * nw < 148 * 16 || p.top > 24 * nw) && (long long)p.cols > nw * warp_cols) nw *= 2;

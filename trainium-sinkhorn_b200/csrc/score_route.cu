@@ -214,7 +214,7 @@ __device__ __noinline__ int choose_exact(const RouteProblem& p, const T* s, doub
 struct RouteLayout {
   int lanes, run, size;
   bool vectors;                // runs are whole 16-byte (or shorter) vectors on their boundaries
-  bool exact;                  // no such layout (or float64 asked for): every row by 64-bit keys
+  bool exact;                  // no such layout: every row by 64-bit keys
 };
 
 template <typename T, int C>
