@@ -295,10 +295,12 @@ __device__ __forceinline__ bool far_scores(const FarRows<T>& p) {
   constexpr int G = 32 / L;
   const int lane = threadIdx.x & 31;
   bool found = false;
+  __syncwarp();                                             // (kept rows: other lanes' runs, too)
   for (int base = (threadIdx.x >> 5) * G; base < p.n; base += NW * G) {
-    const T* s = p.scores + min(base + lane / L, p.n - 1) * p.ld;
+    const int row = min(base + lane / L, p.n - 1);
+    const T* s = base + G <= p.kept_rows ? p.kept + row * p.pitch : p.scores + row * p.ld;
     float top = -INFINITY;
-#pragma unroll 1
+#pragma unroll 8
     for (int j = lane & (L - 1); j < p.cols; j += L)
       if (!(p.b && p.b[j] == 0.f)) top = fmaxf(top, widen(s[j]));
 #pragma unroll
