@@ -177,6 +177,26 @@ def test_balance_start_of_minus_infinity_on_a_far_column(rows, cols, value):
         check(s, 0.15, iters, g=g, far=[3])
 
 
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_balance_start_of_minus_infinity_beside_scores_below_the_range(rows, cols):
+    """Rows whose only normal score is on the column that starts from -inf: the lowest values beside it are as good as -inf,
+    also where other rows, of nothing but the lowest value, have their terms formed from pairs of float32."""
+    s = make(rows, cols, torch.bfloat16, seed=rows, scale=1.0)
+    low, g = torch.finfo(torch.bfloat16).min, torch.zeros(cols, device="cuda")
+    g[2] = -INF
+    s[4::9, torch.arange(cols, device="cuda") != 2] = low
+    want = torch.where(s == low, -INF, s)
+    s[3::9], want[3::9] = low, 0.0
+    for iters in (1, 2, 5):
+        r = scores.balance(s, eps=0.2, iters=iters, g=g)
+        f, w, _ = reference(want, 0.2, iters, None, None, g)
+        f[3::9] -= low                                           # (a row's constant)
+        # as in `check`: |S + f + g| below 10 of the ordinary rows and columns
+        tol = U * 0.2 * 2 * iters * (4 * (10 / 0.2 + 16) + GAMMA + max(s.shape) / 32)
+        close(r.g, w, tol + 8 * U * w.abs(), "g")
+        close(r.f, f, tol + 8 * U * f.abs(), "f")
+
+
 def test_balance_start_that_is_no_number():
     s = make(700, 16, torch.float32, scale=1.0)
     for bad in (math.nan, INF):

@@ -14,7 +14,7 @@
 // iteration) to the least of those that take part, and terms are formed from their high parts: differences of a few
 // units, where the potentials themselves may be hundreds. Once a row's maximum or such a column's potential lies 2^10
 // or more from 0 (finite masks, offsets), a CTA forms all its terms from the pairs, less their row's own constant:
-// 65536 x 256 bfloat16 94 us an iteration in place of 11. A score more than float32's range (2.3e38 eps) below its
+// 65536 x 256 bfloat16 103 us an iteration in place of 11. A score more than float32's range (2.3e38 eps) below its
 // row's largest is as good as -inf.
 //
 // One cooperative launch runs all iterations. A CTA owns a block of rows and keeps as many of them as fit in shared
@@ -216,6 +216,8 @@ __device__ __noinline__ void far_pass(const FarRows<T>& p, int mode, bool last) 
       if (column(k) < p.cols && p.out[column(k)]) closed |= 1u << k;
   }
   auto counts = [&](int k) { return !(closed >> k & 1); };               // in the row's sum
+  // (with mass: also one that starts from -inf, so that what is out of range below it is so in the first iteration, too)
+  auto mass = [&](int k) { return counts(k) || !(p.b && p.b[column(k)] == 0.f); };
   float acc[C];
 #pragma unroll
   for (int k = 0; k < C; ++k) acc[k] = mode == 1 ? -INFINITY : 0.f;
@@ -230,11 +232,10 @@ __device__ __noinline__ void far_pass(const FarRows<T>& p, int mode, bool last) 
     float top = -INFINITY;                                  // the row's constant
 #pragma unroll
     for (int k = 0; k < C; ++k)
-      if (counts(k) && column(k) < p.cols && p.us[column(k)] != -INFINITY) top = fmaxf(top, v[k / V].get(k % V));
+      if (column(k) < p.cols && p.us[column(k)] != -INFINITY && mass(k)) top = fmaxf(top, v[k / V].get(k % V));
 #pragma unroll
     for (int o = 1; o < L; o *= 2) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
-    const bool some = top != -INFINITY;
-    if (!some) top = 0.f;
+    if (top == -INFINITY) top = 0.f;
     // (S - top) c of the lane's k-th column as a high part and (added to `low`) what that is off by
     auto scaled = [&](int k, float& low) {
       const Two x = two_sum(v[k / V].get(k % V), -top);
@@ -251,7 +252,7 @@ __device__ __noinline__ void far_pass(const FarRows<T>& p, int mode, bool last) 
     }
 #pragma unroll
     for (int o = 1; o < L; o *= 2) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
-    if (!some) m = 0.f;
+    if (m == -INFINITY) m = top = 0.f;                      // nothing in the sum
     float l = 0.f, d[C], less[C];                           // less: without the columns' potentials
 #pragma unroll
     for (int k = 0; k < C; ++k) {
